@@ -35,6 +35,10 @@ extern "C" {
 
 #define ALSMI_F32 0
 #define ALSMI_F64 1
+/* taken by the ranking operators (alsmi_mx4_*, alsmi_adjust_scores, alsmi_topk_rows) only */
+#define ALSMI_F16 2
+#define ALSMI_BF16 3
+#define ALSMI_MX4 4 /* alsmi_mx4_scores: activations as codes and scales */
 
 #define ALSMI_OK 0
 #define ALSMI_EINVAL (-1)   /* bad argument (shape, dtype, rank, null pointer) */
@@ -175,6 +179,91 @@ size_t alsmi_topk_workspace_bytes(int dtype, int64_t n_sel, int64_t n_items);
 int alsmi_topk_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
                      const void *user_factors, const void *item_factors, int64_t n_items, int k,
                      int32_t *items_out, void *scores_out, void *workspace, void *stream);
+
+/* The dense score block that alsmi_topk_items ranks: out [n_sel x n_items] of dtype,
+ * out[p, i] = <user_factors[users[p]], item_factors[i]>, by the same kernels (ALSMI_F32: scaled fp16
+ * split, fp32 accuracy).  For callers that change the scores before they select from them.
+ * workspace: 16 bytes, aligned to 4. */
+int alsmi_score_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
+                      const void *user_factors, const void *item_factors, int64_t n_items,
+                      void *scores_out, void *workspace, void *stream);
+
+/* ---- ranking operators: a catalogue in 4 bits, scores changed before the selection, the
+ * selection itself.  The reference stops at predict_all (src/als.py:347-364): no counterparts.
+ * They take fp32, fp64, fp16 and bf16 elements (ALSMI_F32 .. ALSMI_BF16) unless said otherwise, any
+ * row strides (in elements, >= the row's length) and any element alignment; no call allocates,
+ * synchronises or records a memset, so all of them can be captured into a graph.  Calls that are
+ * in flight together need output and workspace memory of their own. -----------------------------
+ *
+ * 4-bit microscaled tables: a row of `width` elements is cut into nb = ceil(width / 32) blocks of 32
+ * (the last one padded by zeros); codes [n_rows x 16 nb] hold two four-bit codes per byte (the
+ * element of even index in the low half), scales [n_rows x nb] one byte per block.  A code is a
+ * sign bit and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6; byte b scales by 2^(b - 127).
+ * alsmi_mx4_quantize: b - 127 = floor(log2 max|x|) - 2, held to -127 .. 127 (-127 for a block of
+ * zeros); the code nearest to |x| / 2^(b-127), ties to the even code, above 6 as 6.  A block with an
+ * infinity or a NaN gets byte 255 and codes 0.  1 <= width <= 2^20, codes aligned to 4 bytes.
+ * alsmi_mx4_dequantize: out row i = row rows[i] of the table (row i where rows is NULL); byte 255
+ * reads as NaN, and so does a row id outside 0 .. n_rows-1.  Exact in fp32, fp64 and bf16; fp16
+ * rounds and overflows to infinity. */
+int alsmi_mx4_quantize(int dtype, int64_t n_rows, int64_t width, const void *x, int64_t ld_x,
+                       uint8_t *codes, uint8_t *scales, void *stream);
+int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows,
+                         int64_t width, const uint8_t *codes, const uint8_t *scales, void *out,
+                         int64_t ld_out, void *stream);
+
+/* out[i, j] = sum_k a[i, k] table[j, k] for i < n_sel, j < n_items; out [n_sel x n_items] of
+ * out_dtype (ALSMI_F32, F16 or BF16).  `a` has n_rows rows of `width` elements of dtype ALSMI_F32,
+ * F16 or BF16 (every product exact, fp32 sums), or with ALSMI_MX4 is a table's codes and a_scales
+ * its scales (a_scales is ignored otherwise).  rows as in alsmi_mx4_dequantize: a row of NaN where
+ * there is no such row. */
+int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, const void *a,
+                     int64_t ld_a, const uint8_t *a_scales, int64_t n_items, int64_t width,
+                     const uint8_t *codes, const uint8_t *scales, int out_dtype, void *out,
+                     int64_t ld_out, void *stream);
+
+/* Penalties, exclusion, biases and masks of score rows.  For row r and item i, with c = the
+ * occurrences of i in the row's history:
+ *   c > 0:  x = -inf if `exclude`, else x = s > 0 ? s / repetition : s * repetition and
+ *           x -= frequency * c + presence;      c == 0: x = s
+ *   x += item_bias[i];  x += the value of the last entry of i in the row's bias list
+ *   x = -inf where the row's mask has no bit i (bit i % 32 of word i / 32 set: i is on offer)
+ * worked in fp32 (fp64 for ALSMI_F64), rounded once.  `out` may be `scores` itself.
+ * Any pointer may be NULL: no history / bias list / item bias / mask.  repetition, frequency and
+ * presence are [n_rows] fp32 arrays, or NULL for the *_value fields.  The history of row r is list
+ * history_rows[r] of the n_history_rows lists (list r where history_rows is NULL; none where it is
+ * outside), the mask of row r row mask_rows[r] (where mask_rows is NULL row r, or the
+ * only one; a negative id: no mask; one past the masks: nothing is on offer).  List r is entries [ptr[r], ptr[r+1]) of the ids;
+ * ids outside 0 .. n_items-1 are skipped, so lists may be padded.  Lists need no order and may
+ * repeat an id.  repetition > 0. */
+typedef struct alsmi_adjust {
+    int64_t n_rows, n_items, ld_scores, ld_out;
+    const int64_t *history_ptr;
+    const int32_t *history_ids;
+    int64_t n_history; /* entries of history_ids */
+    const int32_t *history_rows;
+    int64_t n_history_rows;
+    const float *repetition, *frequency, *presence;
+    double repetition_value, frequency_value, presence_value;
+    const float *item_bias; /* [n_items] */
+    const int64_t *bias_ptr; /* [n_rows + 1] */
+    const int32_t *bias_ids;
+    const float *bias_values;
+    int64_t n_bias; /* entries of bias_ids */
+    const uint32_t *mask; /* [n_masks x ceil(n_items / 32)] */
+    int64_t n_masks;
+    const int32_t *mask_rows;
+    int exclude;
+} alsmi_adjust;
+int alsmi_adjust_scores(int dtype, const alsmi_adjust *args, const void *scores, void *out,
+                        void *stream);
+
+/* The k largest scores of every row, best first, ties by the smaller index: items_out [n_rows x k]
+ * int32, scores_out [n_rows x k] of dtype.  1 <= k <= min(1024, n_items); the order of scores is that
+ * of alsmi_topk_items.  workspace: alsmi_topk_rows_workspace_bytes() bytes, aligned to 16. */
+size_t alsmi_topk_rows_workspace_bytes(int dtype, int64_t n_rows, int64_t n_items, int k);
+int alsmi_topk_rows(int dtype, int64_t n_rows, int64_t n_items, const void *scores,
+                    int64_t ld_scores, int k, int32_t *items_out, void *scores_out, void *workspace,
+                    void *stream);
 
 /* Row index of every stored entry of rows [row_begin,row_end) (the `users`
  * array of data.nonzero(), src/als.py:161), written to rows_out[0 .. nnz_local). */

@@ -8,6 +8,9 @@ import os
 
 F32 = 0
 F64 = 1
+F16 = 2
+BF16 = 3
+MX4 = 4
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('ALSMI_LIB', os.path.join(_HERE, 'libalsmi.so'))
@@ -17,6 +20,20 @@ _lib = None
 
 class AlsmiError(RuntimeError):
     """A libalsmi entry point returned a non-zero status."""
+
+
+class Adjust(ctypes.Structure):
+    """``alsmi_adjust`` of the header."""
+    _i64, _vp, _dbl = ctypes.c_int64, ctypes.c_void_p, ctypes.c_double
+    _fields_ = [('n_rows', _i64), ('n_items', _i64), ('ld_scores', _i64), ('ld_out', _i64),
+                ('history_ptr', _vp), ('history_ids', _vp), ('n_history', _i64),
+                ('history_rows', _vp), ('n_history_rows', _i64),
+                ('repetition', _vp), ('frequency', _vp), ('presence', _vp),
+                ('repetition_value', _dbl), ('frequency_value', _dbl), ('presence_value', _dbl),
+                ('item_bias', _vp),
+                ('bias_ptr', _vp), ('bias_ids', _vp), ('bias_values', _vp), ('n_bias', _i64),
+                ('mask', _vp), ('n_masks', _i64), ('mask_rows', _vp),
+                ('exclude', ctypes.c_int)]
 
 
 def load():
@@ -53,6 +70,17 @@ def load():
         'alsmi_topk_workspace_bytes': (ctypes.c_size_t, [c_int, c_i64, c_i64]),
         'alsmi_topk_items': (c_int, [c_int, c_int, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_vp,
                                      c_vp, c_vp, c_vp]),
+        'alsmi_score_items': (c_int, [c_int, c_int, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp,
+                                      c_vp]),
+        'alsmi_mx4_quantize': (c_int, [c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp]),
+        'alsmi_mx4_dequantize': (c_int, [c_int, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp,
+                                         c_i64, c_vp]),
+        'alsmi_mx4_scores': (c_int, [c_int, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64,
+                                     c_vp, c_vp, c_int, c_vp, c_i64, c_vp]),
+        'alsmi_adjust_scores': (c_int, [c_int, ctypes.POINTER(Adjust), c_vp, c_vp, c_vp]),
+        'alsmi_topk_rows_workspace_bytes': (ctypes.c_size_t, [c_int, c_i64, c_i64, c_int]),
+        'alsmi_topk_rows': (c_int, [c_int, c_i64, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_vp,
+                                    c_vp]),
         'alsmi_expand_rows': (c_int, [c_vp, c_i64, c_i64, c_vp, c_vp]),
         'alsmi_sparse_workspace_bytes': (ctypes.c_size_t, [c_i64]),
         'alsmi_build_csr': (c_int, [c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp,
@@ -78,6 +106,9 @@ EXPORTS = ('alsmi_version', 'alsmi_last_error', 'alsmi_padded_rank', 'alsmi_plan
            'alsmi_half_sweep_err',
            'alsmi_normal_equations', 'alsmi_sddmm_workspace_bytes', 'alsmi_sddmm',
            'alsmi_sddmm_noalloc', 'alsmi_topk_workspace_bytes', 'alsmi_topk_items',
+           'alsmi_score_items', 'alsmi_mx4_quantize', 'alsmi_mx4_dequantize',
+           'alsmi_mx4_scores', 'alsmi_adjust_scores', 'alsmi_topk_rows_workspace_bytes',
+           'alsmi_topk_rows',
            'alsmi_expand_rows', 'alsmi_sparse_workspace_bytes', 'alsmi_build_csr',
            'alsmi_csr_to_csc', 'alsmi_imc_padded_width', 'alsmi_imc_workspace_bytes',
            'alsmi_imc_eval', 'alsmi_imc_project')

@@ -15,8 +15,12 @@ from sklearn.base import BaseEstimator
 from sklearn.utils.validation import check_is_fitted, check_random_state
 
 from . import device as dev
+from . import ranking
 from .engine import AlsEngine, default_group as _default_group
 from .utils import _check_x, _check_y, root_mean_squared_error
+
+# scores of one block of users in ``recommend`` (1 or 2 GiB)
+_BLOCK_SCORES = 1 << 28
 
 
 class ALS(BaseEstimator):
@@ -77,6 +81,7 @@ class ALS(BaseEstimator):
         state = dict(self.__dict__)
         state.pop('_data_dev', None)
         state.pop('_tables', None)
+        state.pop('_mx4', None)
         return state
 
     def _build_data(self, X, y, shape):
@@ -336,7 +341,7 @@ class ALS(BaseEstimator):
         editing ``user_feats`` / ``item_feats`` in place in a way the signature check cannot
         see: the check compares the array objects, their shapes and the sums of the first and
         last row and column."""
-        self._tables = None
+        self._tables = self._mx4 = None
 
     def _cached_tables(self):
         """The device copies of the factor tables if they still belong to the host arrays
@@ -365,23 +370,107 @@ class ALS(BaseEstimator):
         items = np.arange(m)
         return self._predict((users, items))
 
-    def recommend(self, users, k=10):
+    def recommend(self, users, k=10, exclude_seen=False, item_bias=None, allowed=None,
+                  catalogue='factors'):
         """The k items with the highest predicted rating for each of `users`: ``(items,
         scores)`` arrays of shape (len(users), k), best first (ties: smaller item id).
         The ranking the reference leaves to the caller of ``predict_all``
-        (src/als.py:347-364), done on the device for a batch of users."""
+        (src/als.py:347-364), done on the device for a batch of users.
+
+        exclude_seen : leave out the items a user has a stored rating for.
+        item_bias : array [n_items] added to every user's predictions before the ranking.
+        allowed : truth values [n_items], or [len(users), n_items]: the items on offer.
+        catalogue : 'factors', or 'mx4' to score against the item factors held in 4-bit
+            microscaled floating point (an eighth of the fp32 table's bytes to read; made once
+            per fit; user factors in float32), with scores as far off as those factors are.
+
+        Where fewer than k items are left for a user the list ends with items of score -inf."""
         check_is_fitted(self, ['item_feats', 'user_feats'])
         import torch
-        device = dev.require_gpu()
+        if catalogue not in ('factors', 'mx4'):
+            raise ValueError("catalogue must be 'factors' or 'mx4', got %r" % (catalogue,))
         users = np.atleast_1d(np.asarray(users)).ravel()
-        n = self.user_feats.shape[1]
+        n, m = self.user_feats.shape[1], self.item_feats.shape[1]
         if users.size and (users.min() < -n or users.max() >= n):
             raise IndexError('user index out of range')
         users = np.where(users < 0, users + n, users).astype(np.int32)
+        if item_bias is not None:
+            item_bias = np.ascontiguousarray(item_bias, dtype=np.float32)
+            if item_bias.shape != (m,):
+                raise ValueError('item_bias must have %d entries' % m)
+        if allowed is not None:
+            allowed = np.asarray(allowed, dtype=bool)
+            if allowed.shape != (m,) and allowed.shape != (users.size, m):
+                raise ValueError('allowed must have shape (%d,) or (%d, %d)' % (m, users.size, m))
+        seen = self._seen_lists(users) if exclude_seen else None
+        device = dev.require_gpu()
         self._pair_predictions(users[:0], users[:0])  # makes sure the device tables exist
         U, V = self._cached_tables()[:2]
-        items, scores = dev.topk_items(self.rank, torch.from_numpy(users).to(device), U, V, int(k))
+        d_users = torch.from_numpy(users).to(device)
+        if not (exclude_seen or item_bias is not None or allowed is not None) and \
+                catalogue == 'factors':
+            items, scores = dev.topk_items(self.rank, d_users, U, V, int(k))
+        else:
+            items, scores = self._ranked(d_users, U, V, int(k), seen, item_bias, allowed,
+                                         catalogue)
         return items.cpu().numpy(), scores.to(torch.float64).cpu().numpy()
+
+    def _seen_lists(self, users):
+        """The stored items of `users`: (ptr, ids, row of each user's list or None) on the host
+        or, when the ratings are still there, on the device."""
+        if getattr(self, '_data_dev', None) is not None:
+            (indptr, indices, _), _ = self._data_dev
+            return indptr, indices, users
+        if self.data is None:
+            raise ValueError('exclude_seen needs the ratings, which fit_sharded does not keep')
+        rows = self.data[users]
+        return rows.indptr.astype(np.int64), rows.indices.astype(np.int32), None
+
+    def _ranked(self, d_users, U, V, k, seen, item_bias, allowed, catalogue):
+        """Scores of blocks of users, changed and then ranked (alsmi.ranking)."""
+        import torch
+        device, m = V.device, self.item_feats.shape[1]
+        up = lambda a: a if a is None or torch.is_tensor(a) else torch.from_numpy(a).to(device)
+        if not 1 <= k <= min(ranking.MAX_K, m):
+            raise ValueError('k must be between 1 and min(%d, number of items), got %r'
+                             % (ranking.MAX_K, k))
+        item_bias = up(item_bias)
+        ptr, ids, list_rows = (up(a) for a in seen) if seen is not None else (None, None, None)
+        if catalogue == 'mx4':
+            held = getattr(self, '_mx4', None)  # quantised once for these item factors
+            if held is None or held[0] is not V:
+                held = self._mx4 = (V, ranking.mx4_quantize(V[:, :self.rank]))
+            table, users32 = held[1], U[:, :self.rank].to(torch.float32)
+        n = int(d_users.numel())
+        items = torch.empty((n, k), dtype=torch.int32, device=device)
+        best = torch.empty((n, k), dtype=torch.float32 if catalogue == 'mx4' else U.dtype,
+                           device=device)
+        block = max(1, _BLOCK_SCORES // m)
+        mask = None
+        if allowed is not None and allowed.ndim == 1:
+            mask = up(ranking.pack_mask(allowed))
+        for lo in range(0, n, block):
+            hi = min(n, lo + block)
+            part = d_users[lo:hi]
+            if catalogue == 'mx4':
+                s = ranking.mx4_scores(users32, table, rows=part)
+            else:
+                s = dev.score_items(self.rank, part, U, V)
+            kw = {}
+            if seen is not None:
+                if list_rows is not None:
+                    kw = {'history': (ptr, ids), 'history_rows': list_rows[lo:hi]}
+                else:
+                    kw = {'history': (ptr[lo:hi + 1], ids)}
+                kw['exclude'] = True
+            if mask is not None:
+                kw['mask'] = mask
+            elif allowed is not None:
+                kw['mask'] = up(ranking.pack_mask(allowed[lo:hi]))
+            if kw or item_bias is not None:
+                ranking.adjust_scores(s, item_bias=item_bias, out=s, **kw)
+            items[lo:hi], best[lo:hi] = ranking.topk_rows(s, k)
+        return items, best
 
     def score(self, X, y):
         """NEGATIVE root mean squared error on the given pairs (src/als.py:366-388)."""
@@ -416,7 +505,7 @@ class ALS(BaseEstimator):
         out = V.new_zeros((1, V.shape[1]))
         plan.half_sweep(V, out, self.alpha)
         self.user_feats[:, user] = dev.factors_to_host(out, self.rank)[:, 0]
-        self._tables = None  # the host factors changed: rebuild the device copy on next use
+        self._tables = self._mx4 = None  # the host factors changed: rebuilt on next use
         plan.close()
 
     def add_user(self):
@@ -427,4 +516,4 @@ class ALS(BaseEstimator):
         self.data = sps.vstack([self.data, sps.csr_matrix((1, shape[1]))], format='csr')
         new_col = np.zeros((self.rank, 1))
         self.user_feats = np.hstack((self.user_feats, new_col))
-        self._tables = None
+        self._tables = self._mx4 = None

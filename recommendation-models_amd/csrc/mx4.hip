@@ -1,0 +1,696 @@
+// 4-bit microscaled factor tables: quantisation, reading back, and the score product.
+//
+// A row is cut into blocks of 32 elements (the last one padded by zeros).  A block is held as one
+// power of two, 2^e with e = floor(log2 max|x|) - 2 in a byte (e + 127), and 32 four-bit codes: a
+// sign and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 (two bits of exponent, one of mantissa), the nearest
+// to |x| / 2^e, ties to the even code, anything above 6 as 6.  17 bytes for 32 elements.  A block
+// that holds an infinity or a NaN is held as scale byte 255 and reads back as NaN throughout.
+#include "alsmi_common.h"
+#include "elem.h"
+
+namespace alsmi {
+
+constexpr int MX4_BLOCK = 32;
+constexpr int64_t MX4_MAX_WIDTH = 1 << 20;
+
+// 2^(byte - 127) as a float; 255 gives an infinity, which the conversion instructions below take
+// as "not a number" for every code of the block.
+__device__ __forceinline__ float scale_value(unsigned byte) {
+    return __builtin_bit_cast(float, byte ? byte << 23 : 0x00400000u);
+}
+
+// ---- quantisation ------------------------------------------------------------------------------
+// Scale byte of a block from the bit pattern of its largest |x| (which orders like an unsigned
+// integer and puts NaN above infinity above every number).
+__device__ __forceinline__ unsigned scale_byte(unsigned max_bits) {
+    const unsigned e = max_bits >> 23;  // floor(log2) + 127 (0: below 2^-126)
+    return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+__device__ __forceinline__ unsigned scale_byte(unsigned long long max_bits) {
+    const int e = (int)(max_bits >> 52);  // floor(log2) + 1023
+    if (e == 2047) return 255u;
+    const int b = e - 1023 - 2 + 127;
+    return (unsigned)(b < 0 ? 0 : (b > 254 ? 254 : b));
+}
+__device__ __forceinline__ unsigned abs_bits(float x) {
+    return __builtin_bit_cast(unsigned, x) & 0x7fffffffu;
+}
+__device__ __forceinline__ unsigned long long abs_bits(double x) {
+    return __builtin_bit_cast(unsigned long long, x) & 0x7fffffffffffffffull;
+}
+
+// Eight elements to eight codes, element 0 in the lowest four bits.
+__device__ __forceinline__ unsigned to_codes(const float (&x)[8], unsigned byte) {
+    const float s = scale_value(byte);
+    unsigned c = 0;  // (x / s rounded to nearest even and saturated by the instruction)
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], s, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], s, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], s, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], s, 3);
+    return byte == 255u ? 0u : c;
+}
+// fp64 elements are compared with the midpoints in fp64: a first rounding to fp32 could carry a
+// value onto a midpoint.
+__device__ __forceinline__ unsigned to_codes(const double (&x)[8], unsigned byte) {
+    if (byte == 255u) return 0u;
+    unsigned c = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double v = ldexp(fabs(x[i]), 127 - (int)byte);
+        unsigned m = (v > 0.25) + (v >= 0.75) + (v > 1.25) + (v >= 1.75) + (v > 2.5) + (v >= 3.5) +
+                     (v > 5.0);
+        m |= (unsigned)(__builtin_bit_cast(unsigned long long, x[i]) >> 63) << 3;
+        c |= m << (4 * i);
+    }
+    return c;
+}
+
+// A lane takes eight consecutive elements, four neighbouring lanes a block: 32 bytes of fp32 per
+// lane in, four bytes out.  `upr` = lanes per row (4 per block); a workgroup takes `rpb` whole rows, or
+// 256 lanes' worth of one row (blockIdx.y) where a row is longer than that.  Bound by HBM.
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(int64_t n_rows, int width,
+                                                           const T *__restrict__ x, int64_t ldx,
+                                                           uint8_t *__restrict__ codes,
+                                                           uint8_t *__restrict__ scales, int upr,
+                                                           int rpb) {
+    typedef typename Elem<T>::wide W;
+    const unsigned rl = threadIdx.x / (unsigned)upr;  // (0 where upr >= 256)
+    if (rl >= (unsigned)rpb) return;                  // whole groups of four lanes leave together
+    const int64_t row = (int64_t)blockIdx.x * rpb + rl;
+    const int sub = (int)(threadIdx.x - rl * upr) + (int)blockIdx.y * 256;
+    if (row >= n_rows || sub >= upr) return;
+    W v[8];
+    load8<T>(v, x + row * ldx + (int64_t)sub * 8, width - sub * 8);
+    auto m = abs_bits(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        const auto b = abs_bits(v[i]);
+        m = b > m ? b : m;
+    }
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+        const auto b = __shfl_xor(m, off);
+        m = b > m ? b : m;
+    }
+    const unsigned byte = scale_byte(m);
+    const int64_t at = row * upr + sub;
+    reinterpret_cast<unsigned *>(codes)[at] = to_codes(v, byte);
+    if ((sub & 3) == 0) scales[at >> 2] = (uint8_t)byte;
+}
+
+// ---- reading back --------------------------------------------------------------------------------
+__device__ __forceinline__ void from_codes(unsigned c, unsigned byte, float (&v)[8]) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const float s = scale_value(byte);
+    const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
+    const f2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
+    const f2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
+    const f2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
+    v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
+}
+// (fp64: 6 x 2^127 is past fp32's range, so the scale is applied in fp64)
+__device__ __forceinline__ void from_codes(unsigned c, unsigned byte, double (&v)[8]) {
+    float f[8];
+    from_codes(c, byte == 255u ? 255u : 127u, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ldexp((double)f[i], (int)byte - 127);
+}
+
+// Row i of the output is row rows[i] of the table (row i where rows is null), NaN where there is
+// no such row.  Lanes as in mx4_quantize_kernel.
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t n_sel,
+                                                             const int32_t *__restrict__ rows,
+                                                             int64_t n_rows, int width,
+                                                             const uint8_t *__restrict__ codes,
+                                                             const uint8_t *__restrict__ scales,
+                                                             T *__restrict__ out, int64_t ldo,
+                                                             int upr, int rpb) {
+    typedef typename Elem<T>::wide W;
+    const unsigned rl = threadIdx.x / (unsigned)upr;
+    if (rl >= (unsigned)rpb) return;
+    const int64_t i = (int64_t)blockIdx.x * rpb + rl;
+    const int sub = (int)(threadIdx.x - rl * upr) + (int)blockIdx.y * 256;
+    if (i >= n_sel || sub >= upr) return;
+    const int64_t row = rows ? (int64_t)rows[i] : i;
+    unsigned c = 0, byte = 255u;
+    if (row >= 0 && row < n_rows) {
+        const int64_t at = row * upr + sub;
+        c = reinterpret_cast<const unsigned *>(codes)[at];
+        byte = scales[at >> 2];
+    }
+    W v[8];
+    from_codes(c, byte, v);
+    store8<T>(out + i * ldo + (int64_t)sub * 8, v, width - sub * 8);
+}
+
+// ---- scores: out[i, j] = sum_k a[i, k] table[j, k] -----------------------------------------------
+// The table's elements have three significant bits and are exact in bf16 once scaled, so the
+// product runs on the bf16 matrix cores with fp32 sums.  The activations are split exactly into bf16
+// parts: fp32 = 3 parts of 8 significant bits each (cut, not rounded), fp16 = 2, bf16 = 1; every
+// product is then exact and the result has the accuracy of fp32 sums of the fp32 products.  (A
+// two-way fp16 split as in the half-sweep would take 2 parts for fp32, but needs the table's
+// scales applied after each block of 32 and the largest |a| beforehand.)
+// Matrix operands: the items are the rows of the result tile, the activations its columns, so a lane
+// ends with four consecutive items of one output row.  The contraction index may be spread over
+// lane groups and steps in any way both operands share: lane group g takes NBL * 8 consecutive
+// elements, one contiguous load of codes and one scale.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Parts;  // bf16 parts of one activation
+template <>
+struct Parts<float> {
+    static constexpr int N = 3;
+};
+template <>
+struct Parts<_Float16> {
+    static constexpr int N = 2;
+};
+template <>
+struct Parts<__bf16> {
+    static constexpr int N = 1;
+};
+
+// upper halves of two floats' bit patterns, the first in the low half
+__device__ __forceinline__ unsigned high_halves(float a, float b) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a),
+                                 0x07060302u);
+}
+
+template <int N>
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&h)[N]) {
+    u32x4 w[N];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float a = x[2 * j], b = x[2 * j + 1];
+#pragma unroll
+        for (int p = 0; p < N; ++p) {
+            if constexpr (N > 1) {
+                if (p == 0) {
+                    // a NaN keeps a bit in its upper half; an infinity has no further parts
+                    a = a != a ? __builtin_nanf("") : a;
+                    b = b != b ? __builtin_nanf("") : b;
+                }
+            }
+            w[p][j] = high_halves(a, b);
+            if (p + 1 < N) {
+                const float ta = __builtin_bit_cast(float, w[p][j] << 16);
+                const float tb = __builtin_bit_cast(float, w[p][j] & 0xffff0000u);
+                a = __builtin_isfinite(a) ? a - ta : 0.0f;
+                b = __builtin_isfinite(b) ? b - tb : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < N; ++p) h[p] = __builtin_bit_cast(bf16x8, w[p]);
+}
+
+// eight codes to bf16
+__device__ __forceinline__ bf16x8 codes_to_bf16(unsigned c, float s) {
+    u32x4 w;
+    w[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0));
+    w[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1));
+    w[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2));
+    w[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3));
+    return __builtin_bit_cast(bf16x8, w);
+}
+
+// NW words of codes; a block behind the row's end is zero
+template <int NW>
+__device__ __forceinline__ void load_codes(unsigned (&c)[NW], const uint8_t *p) {
+    typedef unsigned vec_t __attribute__((ext_vector_type(NW), aligned(4)));
+    if constexpr (NW == 1) {
+        c[0] = *reinterpret_cast<const unsigned *>(p);
+    } else {
+        const vec_t v = *reinterpret_cast<const vec_t *>(p);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) c[i] = v[i];
+    }
+}
+
+// The activations of a call: their rows may be picked out of a larger table.
+struct Rows {
+    int64_t n_sel, n_rows, ld;
+    const int32_t *ids;  // null: row i is row i
+    // row of selected row i, or -1 where there is none
+    __device__ __forceinline__ int64_t of(int64_t i) const {
+        const int64_t r = ids ? (int64_t)ids[i] : i;
+        return r >= 0 && r < n_rows ? r : -1;
+    }
+};
+
+struct ScoreStore {
+    void *out;
+    int64_t ld, n_sel, n_items;
+    int type;  // ALSMI_F32 / F16 / BF16
+    // four consecutive items of one output row
+    __device__ __forceinline__ void put(int64_t row, int64_t item, f32x4 v) const {
+        if (row >= n_sel || item >= n_items) return;
+        const int64_t at = row * ld + item;
+        const int n = n_items - item < 4 ? (int)(n_items - item) : 4;
+        if (type == ALSMI_F32) store_n<float>(static_cast<float *>(out) + at, v, n);
+        else if (type == ALSMI_BF16) store_n<__bf16>(static_cast<__bf16 *>(out) + at, v, n);
+        else store_n<_Float16>(static_cast<_Float16 *>(out) + at, v, n);
+    }
+    template <typename T>
+    static __device__ __forceinline__ void store_n(T *p, f32x4 v, int n) {
+        typedef T vec_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        if (n == 4) {
+            *reinterpret_cast<vec_t *>(p) = __builtin_convertvector(v, vec_t);
+        } else {
+            for (int i = 0; i < n; ++i) p[i] = (T)v[i];
+        }
+    }
+};
+
+// Rows of at most four blocks (rank <= 128): UT tiles of 16 activation rows stay in registers,
+// split once, and the wave walks `tpw` tiles of 16 items.  Bound by the table's bytes for a few
+// rows, by the write of the scores for many.
+template <typename T, int NBL, int UT>
+__global__ __launch_bounds__(256) void mx4_scores_narrow_kernel(Rows rows, const T *__restrict__ a,
+                                                                int width,
+                                                                const uint8_t *__restrict__ codes,
+                                                                const uint8_t *__restrict__ scales,
+                                                                int nb, ScoreStore o, int groups,
+                                                                int tpw) {
+    constexpr int NP = Parts<T>::N;
+    const int lane = threadIdx.x & 63;
+    const int g = lane >> 4, q = lane & 15;
+    const unsigned chunk = blockIdx.x / (unsigned)groups;
+    const int64_t row_base = (int64_t)(blockIdx.x - chunk * groups) * (16 * UT);
+    const int64_t n_tiles = (o.n_items + 15) / 16;
+    const int64_t t0 = ((int64_t)chunk * 4 + (threadIdx.x >> 6)) * tpw;
+    const int64_t t1 = t0 + tpw < n_tiles ? t0 + tpw : n_tiles;
+    if (t0 >= t1) return;
+    const int blk = (g * NBL) >> 2;  // this lane's block
+    bf16x8 af[UT][NBL][NP];
+#pragma unroll
+    for (int t = 0; t < UT; ++t) {
+        int64_t i = row_base + 16 * t + q;
+        i = i < rows.n_sel ? i : rows.n_sel - 1;  // (rows past the end are not stored)
+        const int64_t r = rows.of(i);
+#pragma unroll
+        for (int j = 0; j < NBL; ++j) {
+            const int k = (g * NBL + j) * 8;
+            float x[8];
+            load8<T>(x, a + (r < 0 ? 0 : r) * rows.ld + k, width - k);
+            if (r < 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __builtin_nanf("");
+            }
+            split8<NP>(x, af[t][j]);
+        }
+    }
+    for (int64_t tile = t0; tile < t1; ++tile) {
+        int64_t item = 16 * tile + q;
+        item = item < o.n_items ? item : o.n_items - 1;
+        unsigned c[NBL];
+        float s = 1.0f;
+#pragma unroll
+        for (int j = 0; j < NBL; ++j) c[j] = 0;
+        if (blk < nb) {
+            load_codes<NBL>(c, codes + item * (16 * (int64_t)nb) + g * NBL * 4);
+            s = scale_value(scales[item * nb + blk]);
+        }
+        f32x4 acc[UT];
+#pragma unroll
+        for (int t = 0; t < UT; ++t) acc[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < NBL; ++j) {
+            const bf16x8 b = codes_to_bf16(c[j], s);
+#pragma unroll
+            for (int p = NP - 1; p >= 0; --p)  // small parts first
+#pragma unroll
+                for (int t = 0; t < UT; ++t)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, af[t][j][p], acc[t], 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < UT; ++t) o.put(row_base + 16 * t + q, 16 * tile + 4 * g, acc[t]);
+    }
+}
+
+// Rows of any width: a wave forms MT x NT tiles (16 activation rows x 16 items each) in steps of
+// four blocks.  KW = 1: the four waves of a workgroup take neighbouring items; KW = 4: they share
+// one tile group and take a quarter of the steps each, joined in wave order through LDS, where
+// there are too few tiles to fill the chip.
+template <typename T, int MT, int NT, int KW>
+__global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T *__restrict__ a,
+                                                              int width,
+                                                              const uint8_t *__restrict__ codes,
+                                                              const uint8_t *__restrict__ scales,
+                                                              int nb, ScoreStore o, int groups) {
+    constexpr int NP = Parts<T>::N;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, q = lane & 15;
+    const unsigned chunk = blockIdx.x / (unsigned)groups;
+    const int64_t row_base = (int64_t)(blockIdx.x - chunk * groups) * (16 * MT);
+    const int64_t item_base = (KW == 1 ? (int64_t)chunk * 4 + wave : (int64_t)chunk) * (16 * NT);
+    const int steps = (nb + 3) / 4;
+    int s0 = 0, s1 = steps;
+    if constexpr (KW > 1) {
+        const int per = (steps + KW - 1) / KW;
+        s0 = wave * per < steps ? wave * per : steps;
+        s1 = s0 + per < steps ? s0 + per : steps;
+    }
+    const T *ar[MT];
+    bool no_row[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        int64_t i = row_base + 16 * t + q;
+        i = i < rows.n_sel ? i : rows.n_sel - 1;
+        const int64_t r = rows.of(i);
+        no_row[t] = r < 0;
+        ar[t] = a + (r < 0 ? 0 : r) * rows.ld;
+    }
+    int64_t it[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int64_t i = item_base + 16 * n + q;
+        it[n] = i < o.n_items ? i : o.n_items - 1;
+    }
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0, 0, 0, 0};
+    if (item_base < o.n_items) {
+        for (int s = s0; s < s1; ++s) {
+            const int blk = 4 * s + g;
+            unsigned c[NT][4];
+            float sc[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                sc[n] = 1.0f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[n][j] = 0;
+                if (blk < nb) {
+                    load_codes<4>(c[n], codes + (it[n] * nb + blk) * 16);
+                    sc[n] = scale_value(scales[it[n] * nb + blk]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = blk * 32 + 8 * j;
+                bf16x8 b[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) b[n] = codes_to_bf16(c[n][j], sc[n]);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    float x[8];
+                    load8<T>(x, ar[t] + k, width - k);
+                    bf16x8 h[NP];
+                    split8<NP>(x, h);
+#pragma unroll
+                    for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[n], h[p], acc[t][n],
+                                                                                0, 0, 0);
+                }
+            }
+        }
+    }
+    if constexpr (KW > 1) {
+        __shared__ f32x4 part[KW - 1][MT * NT][64];
+        if (wave > 0) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) part[wave - 1][t * NT + n][lane] = acc[t][n];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 0; w < KW - 1; ++w)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[t][n] += part[w][t * NT + n][lane];
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            f32x4 v = acc[t][n];
+            if (no_row[t]) v = f32x4{} + __builtin_nanf("");
+            o.put(row_base + 16 * t + q, item_base + 16 * n + 4 * g, v);
+        }
+}
+
+// Both sides in 4 bits: v_mfma_scale_f32_16x16x128_f8f6f4 takes 32 codes per lane (one block) and
+// its scale byte, four blocks per instruction.
+template <int MT, int NT>
+__global__ __launch_bounds__(256) void mx4_scores_both_kernel(Rows rows,
+                                                              const uint8_t *__restrict__ acodes,
+                                                              const uint8_t *__restrict__ ascales,
+                                                              const uint8_t *__restrict__ codes,
+                                                              const uint8_t *__restrict__ scales,
+                                                              int nb, ScoreStore o, int groups) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, q = lane & 15;
+    const unsigned chunk = blockIdx.x / (unsigned)groups;
+    const int64_t row_base = (int64_t)(blockIdx.x - chunk * groups) * (16 * MT);
+    const int64_t item_base = ((int64_t)chunk * 4 + wave) * (16 * NT);
+    if (item_base >= o.n_items) return;
+    int64_t ai[MT], it[NT];
+    bool no_row[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        int64_t i = row_base + 16 * t + q;
+        i = i < rows.n_sel ? i : rows.n_sel - 1;
+        const int64_t r = rows.of(i);
+        no_row[t] = r < 0;
+        ai[t] = (r < 0 ? 0 : r) * nb;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int64_t i = item_base + 16 * n + q;
+        it[n] = (i < o.n_items ? i : o.n_items - 1) * nb;
+    }
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0, 0, 0, 0};
+    for (int blk = g; blk - g < nb; blk += 4) {
+        const bool in = blk < nb;
+        i32x8 af[MT], bf[NT];
+        int as[MT], bs[NT];
+        auto fetch = [&](const uint8_t *c, const uint8_t *s, int64_t at, i32x8 &f, int &e) {
+            unsigned w[4] = {0, 0, 0, 0};
+            e = 127;
+            if (in) {
+                load_codes<4>(w, c + (at + blk) * 16);
+                e = s[at + blk];
+            }
+            f = i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+        };
+#pragma unroll
+        for (int t = 0; t < MT; ++t) fetch(acodes, ascales, ai[t], af[t], as[t]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) fetch(codes, scales, it[n], bf[n], bs[n]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                acc[t][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                    bf[n], af[t], acc[t][n], 4, 4, 0, bs[n], 0, as[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            f32x4 v = acc[t][n];
+            if (no_row[t]) v = f32x4{} + __builtin_nanf("");
+            o.put(row_base + 16 * t + q, item_base + 16 * n + 4 * g, v);
+        }
+}
+
+// ---- launches ------------------------------------------------------------------------------------
+struct RowGrid {
+    int upr, rpb;
+    dim3 grid;
+};
+static RowGrid row_grid(int64_t n_rows, int nb) {
+    RowGrid r;
+    r.upr = 4 * nb;
+    r.rpb = r.upr < 256 ? 256 / r.upr : 1;
+    r.grid = dim3((unsigned)((n_rows + r.rpb - 1) / r.rpb), (unsigned)((r.upr + 255) / 256));
+    return r;
+}
+
+template <typename T, int NBL, int UT>
+static int launch_narrow(const Rows &rows, const void *a, int width, const uint8_t *codes,
+                         const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
+    const int64_t groups = (rows.n_sel + 16 * UT - 1) / (16 * UT);
+    const int64_t n_tiles = (o.n_items + 15) / 16;
+    // long walks once there is enough work for 8192 waves
+    int64_t tpw = n_tiles * groups / 8192;
+    tpw = tpw < 1 ? 1 : (tpw > 32 ? 32 : tpw);
+    const int64_t blocks = (n_tiles + 4 * tpw - 1) / (4 * tpw) * groups;
+    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
+    hipLaunchKernelGGL((mx4_scores_narrow_kernel<T, NBL, UT>), dim3((unsigned)blocks), dim3(256), 0, st,
+                       rows, static_cast<const T *>(a), width, codes, scales, nb, o, (int)groups,
+                       (int)tpw);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
+template <typename T, int MT, int NT, int KW>
+static int launch_wide(const Rows &rows, const void *a, int width, const uint8_t *codes,
+                       const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
+    const int64_t groups = (rows.n_sel + 16 * MT - 1) / (16 * MT);
+    const int64_t per = 16 * NT * (KW == 1 ? 4 : 1);
+    const int64_t blocks = (o.n_items + per - 1) / per * groups;
+    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
+    hipLaunchKernelGGL((mx4_scores_wide_kernel<T, MT, NT, KW>), dim3((unsigned)blocks), dim3(256), 0,
+                       st, rows, static_cast<const T *>(a), width, codes, scales, nb, o, (int)groups);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
+template <int MT, int NT>
+static int launch_both(const Rows &rows, const void *a, const uint8_t *a_scales, const uint8_t *codes,
+                       const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
+    const int64_t groups = (rows.n_sel + 16 * MT - 1) / (16 * MT);
+    const int64_t per = 64 * NT;
+    const int64_t blocks = (o.n_items + per - 1) / per * groups;
+    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
+    hipLaunchKernelGGL((mx4_scores_both_kernel<MT, NT>), dim3((unsigned)blocks), dim3(256), 0, st, rows,
+                       static_cast<const uint8_t *>(a), a_scales, codes, scales, nb, o, (int)groups);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
+template <typename T>
+static int run_scores(const Rows &rows, const void *a, int width, const uint8_t *codes,
+                      const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
+    const bool one = rows.n_sel <= 16;
+    if (nb == 1)
+        return one ? launch_narrow<T, 1, 1>(rows, a, width, codes, scales, nb, o, st)
+                   : launch_narrow<T, 1, 4>(rows, a, width, codes, scales, nb, o, st);
+    if (nb == 2)
+        return one ? launch_narrow<T, 2, 1>(rows, a, width, codes, scales, nb, o, st)
+                   : launch_narrow<T, 2, 4>(rows, a, width, codes, scales, nb, o, st);
+    // (three parts of four tiles at four blocks would need 192 registers)
+    if (nb <= 4)
+        return one ? launch_narrow<T, 4, 1>(rows, a, width, codes, scales, nb, o, st)
+                   : launch_narrow<T, 4, 2>(rows, a, width, codes, scales, nb, o, st);
+    const int64_t tiles = (rows.n_sel + 15) / 16 * ((o.n_items + 15) / 16);
+    if (one)
+        return tiles < 32768 ? launch_wide<T, 1, 2, 4>(rows, a, width, codes, scales, nb, o, st)
+                             : launch_wide<T, 1, 4, 1>(rows, a, width, codes, scales, nb, o, st);
+    return tiles < 16384 ? launch_wide<T, 2, 2, 4>(rows, a, width, codes, scales, nb, o, st)
+                         : launch_wide<T, 4, 4, 1>(rows, a, width, codes, scales, nb, o, st);
+}
+
+}  // namespace alsmi
+
+extern "C" {
+
+int alsmi_mx4_quantize(int dtype, int64_t n_rows, int64_t width, const void *x, int64_t ldx,
+                       uint8_t *codes, uint8_t *scales, void *stream) {
+    using namespace alsmi;
+    ALSMI_REQUIRE(dtype >= ALSMI_F32 && dtype <= ALSMI_BF16, "alsmi_mx4_quantize: bad dtype %d", dtype);
+    ALSMI_REQUIRE(n_rows >= 0 && n_rows <= INT32_MAX, "alsmi_mx4_quantize: bad row count %lld",
+                  (long long)n_rows);
+    ALSMI_REQUIRE(width >= 1 && width <= MX4_MAX_WIDTH, "alsmi_mx4_quantize: width %lld outside 1..%lld",
+                  (long long)width, (long long)MX4_MAX_WIDTH);
+    if (n_rows == 0) return ALSMI_OK;
+    ALSMI_REQUIRE(ldx >= width || n_rows == 1, "alsmi_mx4_quantize: row stride %lld below the width",
+                  (long long)ldx);
+    ALSMI_REQUIRE(x && codes && scales, "alsmi_mx4_quantize: null pointer");
+    ALSMI_REQUIRE((uintptr_t)codes % 4 == 0, "alsmi_mx4_quantize: codes must be aligned to 4 bytes");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
+    const RowGrid rg = row_grid(n_rows, nb);
+#define ALSMI_CASE(T)                                                                                \
+    hipLaunchKernelGGL((mx4_quantize_kernel<T>), rg.grid, dim3(256), 0, st, n_rows, (int)width,      \
+                       static_cast<const T *>(x), ldx, codes, scales, rg.upr, rg.rpb)
+    if (dtype == ALSMI_F32) ALSMI_CASE(float);
+    else if (dtype == ALSMI_F64) ALSMI_CASE(double);
+    else if (dtype == ALSMI_F16) ALSMI_CASE(_Float16);
+    else ALSMI_CASE(__bf16);
+#undef ALSMI_CASE
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
+int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, int64_t width,
+                         const uint8_t *codes, const uint8_t *scales, void *out, int64_t ldo,
+                         void *stream) {
+    using namespace alsmi;
+    ALSMI_REQUIRE(dtype >= ALSMI_F32 && dtype <= ALSMI_BF16, "alsmi_mx4_dequantize: bad dtype %d",
+                  dtype);
+    ALSMI_REQUIRE(n_rows >= 0 && n_rows <= INT32_MAX && n_sel >= 0 && n_sel <= INT32_MAX,
+                  "alsmi_mx4_dequantize: bad row count");
+    ALSMI_REQUIRE(rows || n_sel <= n_rows, "alsmi_mx4_dequantize: %lld rows of a table of %lld",
+                  (long long)n_sel, (long long)n_rows);
+    ALSMI_REQUIRE(width >= 1 && width <= MX4_MAX_WIDTH,
+                  "alsmi_mx4_dequantize: width %lld outside 1..%lld", (long long)width,
+                  (long long)MX4_MAX_WIDTH);
+    if (n_sel == 0) return ALSMI_OK;
+    ALSMI_REQUIRE(ldo >= width || n_sel == 1, "alsmi_mx4_dequantize: row stride %lld below the width",
+                  (long long)ldo);
+    ALSMI_REQUIRE(out && (n_rows == 0 || (codes && scales)), "alsmi_mx4_dequantize: null pointer");
+    ALSMI_REQUIRE((uintptr_t)codes % 4 == 0, "alsmi_mx4_dequantize: codes must be aligned to 4 bytes");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
+    const RowGrid rg = row_grid(n_sel, nb);
+#define ALSMI_CASE(T)                                                                                 \
+    hipLaunchKernelGGL((mx4_dequantize_kernel<T>), rg.grid, dim3(256), 0, st, n_sel, rows, n_rows,    \
+                       (int)width, codes, scales, static_cast<T *>(out), ldo, rg.upr, rg.rpb)
+    if (dtype == ALSMI_F32) ALSMI_CASE(float);
+    else if (dtype == ALSMI_F64) ALSMI_CASE(double);
+    else if (dtype == ALSMI_F16) ALSMI_CASE(_Float16);
+    else ALSMI_CASE(__bf16);
+#undef ALSMI_CASE
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
+int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, const void *a,
+                     int64_t lda, const uint8_t *a_scales, int64_t n_items, int64_t width,
+                     const uint8_t *codes, const uint8_t *scales, int out_dtype, void *out,
+                     int64_t ldo, void *stream) {
+    using namespace alsmi;
+    ALSMI_REQUIRE(dtype == ALSMI_F32 || dtype == ALSMI_F16 || dtype == ALSMI_BF16 || dtype == ALSMI_MX4,
+                  "alsmi_mx4_scores: bad dtype %d", dtype);
+    ALSMI_REQUIRE(out_dtype == ALSMI_F32 || out_dtype == ALSMI_F16 || out_dtype == ALSMI_BF16,
+                  "alsmi_mx4_scores: bad output dtype %d", out_dtype);
+    ALSMI_REQUIRE(n_rows >= 0 && n_rows <= INT32_MAX && n_sel >= 0 && n_sel <= INT32_MAX &&
+                      n_items >= 0 && n_items <= INT32_MAX,
+                  "alsmi_mx4_scores: bad row or item count");
+    ALSMI_REQUIRE(rows || n_sel <= n_rows, "alsmi_mx4_scores: %lld rows of a table of %lld",
+                  (long long)n_sel, (long long)n_rows);
+    ALSMI_REQUIRE(width >= 1 && width <= MX4_MAX_WIDTH, "alsmi_mx4_scores: width %lld outside 1..%lld",
+                  (long long)width, (long long)MX4_MAX_WIDTH);
+    if (n_sel == 0 || n_items == 0) return ALSMI_OK;
+    ALSMI_REQUIRE(n_rows > 0, "alsmi_mx4_scores: rows of an empty table");
+    ALSMI_REQUIRE(ldo >= n_items || n_sel == 1, "alsmi_mx4_scores: output stride %lld below n_items",
+                  (long long)ldo);
+    ALSMI_REQUIRE(dtype == ALSMI_MX4 || lda >= width || n_rows == 1,
+                  "alsmi_mx4_scores: row stride %lld below the width", (long long)lda);
+    ALSMI_REQUIRE(a && codes && scales && out && (dtype != ALSMI_MX4 || a_scales),
+                  "alsmi_mx4_scores: null pointer");
+    ALSMI_REQUIRE((uintptr_t)codes % 4 == 0 && (dtype != ALSMI_MX4 || (uintptr_t)a % 4 == 0),
+                  "alsmi_mx4_scores: codes must be aligned to 4 bytes");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
+    const Rows r = {n_sel, n_rows, lda, rows};
+    const ScoreStore o = {out, ldo, n_sel, n_items, out_dtype};
+    if (dtype == ALSMI_F32) return run_scores<float>(r, a, (int)width, codes, scales, nb, o, st);
+    if (dtype == ALSMI_F16) return run_scores<_Float16>(r, a, (int)width, codes, scales, nb, o, st);
+    if (dtype == ALSMI_BF16) return run_scores<__bf16>(r, a, (int)width, codes, scales, nb, o, st);
+    return n_sel <= 16 ? launch_both<1, 4>(r, a, a_scales, codes, scales, nb, o, st)
+                       : launch_both<4, 4>(r, a, a_scales, codes, scales, nb, o, st);
+}
+
+}  // extern "C"

@@ -843,6 +843,8 @@ __global__ __launch_bounds__(256) void topk_rescore_kernel(
     }
 }
 
+__global__ void topk_zero_kernel(unsigned *p) { p[threadIdx.x] = 0u; }
+
 static size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // Users per wave of the score kernel of (T, NV).
@@ -1050,9 +1052,70 @@ static int run_topk(int n_sel, const int32_t *sel, const void *U, const void *V,
     return ALSMI_OK;
 }
 
+// The dense score block alone (MODE 0 over all items).
+template <typename T, int NV>
+static int run_score_items(int n_sel, const int32_t *sel, const void *U, const void *V,
+                           int64_t n_items, void *out, void *workspace, hipStream_t st) {
+    const T *Ut = static_cast<const T *>(U), *Vt = static_cast<const T *>(V);
+    constexpr int UPW = score_users_per_wave<T, NV>();
+    const int64_t user_blocks = (n_sel + UPW - 1) / UPW;
+    const int64_t n_tiles = (n_items + 15) / 16;
+    const int itw = user_blocks >= 64 ? 32 : 4;
+    const int64_t chunks = (n_tiles + 4 * itw - 1) / (4 * itw);
+    ALSMI_REQUIRE(chunks <= 65535, "alsmi_score_items: too many items (%lld)", (long long)n_items);
+    unsigned *max_bits = static_cast<unsigned *>(workspace);
+    if constexpr (sizeof(T) == 4) {
+        const int kp = NV * 16;
+        auto blocks_for = [&](int64_t rows) {
+            const int64_t b = (rows * (kp / 4) + 255) / 256;
+            return (unsigned)(b < 1 ? 1 : (b > 512 ? 512 : b));
+        };
+        hipLaunchKernelGGL(topk_zero_kernel, dim3(1), dim3(2), 0, st, max_bits);
+        hipLaunchKernelGGL(topk_max_abs_kernel, dim3(blocks_for(n_sel)), dim3(256), 0, st,
+                           (int64_t)n_sel, sel, reinterpret_cast<const float *>(Ut), kp, max_bits);
+        hipLaunchKernelGGL(topk_max_abs_kernel, dim3(blocks_for(n_items)), dim3(256), 0, st, n_items,
+                           (const int32_t *)nullptr, reinterpret_cast<const float *>(Vt), kp,
+                           max_bits + 1);
+        ALSMI_HIP_CHECK(hipGetLastError());
+    }
+    ScoreOut<T> all = {};
+    all.scores = static_cast<T *>(out);
+    all.row_len = n_items;
+    launch_scores<T, NV, 0>(dim3((unsigned)user_blocks, (unsigned)chunks), st, n_sel, sel, Ut, Vt,
+                            n_items, all, itw, max_bits);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
 }  // namespace alsmi
 
 extern "C" {
+
+int alsmi_score_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
+                      const void *user_factors, const void *item_factors, int64_t n_items,
+                      void *scores_out, void *workspace, void *stream) {
+    using namespace alsmi;
+    ALSMI_REQUIRE(dtype == ALSMI_F32 || dtype == ALSMI_F64, "alsmi_score_items: bad dtype %d", dtype);
+    const int kp = alsmi_padded_rank(rank);
+    ALSMI_REQUIRE(kp > 0, "alsmi_score_items: rank %d outside 1..128", rank);
+    ALSMI_REQUIRE(n_sel >= 0 && n_sel < INT32_MAX && n_items >= 0 && n_items <= INT32_MAX,
+                  "alsmi_score_items: bad user or item count");
+    if (n_sel == 0 || n_items == 0) return ALSMI_OK;
+    ALSMI_REQUIRE(users && user_factors && item_factors && scores_out && workspace,
+                  "alsmi_score_items: null pointer");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+#define ALSMI_CASE(T, NV)                                                                         \
+    return run_score_items<T, NV>((int)n_sel, users, user_factors, item_factors, n_items, scores_out, \
+                                  workspace, st)
+    const bool f32 = dtype == ALSMI_F32;
+    switch (kp) {
+        case 16: if (f32) ALSMI_CASE(float, 1); else ALSMI_CASE(double, 1);
+        case 32: if (f32) ALSMI_CASE(float, 2); else ALSMI_CASE(double, 2);
+        case 64: if (f32) ALSMI_CASE(float, 4); else ALSMI_CASE(double, 4);
+        default: if (f32) ALSMI_CASE(float, 8); else ALSMI_CASE(double, 8);
+    }
+#undef ALSMI_CASE
+}
 
 size_t alsmi_topk_workspace_bytes(int dtype, int64_t n_sel, int64_t n_items) {
     if ((dtype != ALSMI_F32 && dtype != ALSMI_F64) || n_sel < 0 || n_items < 0) return 0;

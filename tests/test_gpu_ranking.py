@@ -1,0 +1,603 @@
+"""The ranking operators (alsmi.ranking) against their definitions in 64 bits (oracle.ranking_oracle).
+
+Tolerances.  Codes, scales, item lists and selected scores are exact.  A score is a sum of `width`
+exact products (up to three bf16 parts per fp32 activation) in fp32: each of at most 3 * width
+additions is off by at most one ulp (2^-23) of a partial sum, which is at most sum |a_k t_k|; the
+output type rounds once by half a step.  An adjusted score passes at most eight roundings (three
+parameters to fp32, division or product, product and sum of the penalty, two biases) relative to the
+largest magnitude met, then the output's half step."""
+import numpy as np
+import pytest
+import torch
+
+from alsmi import ranking as rk
+from oracle import ranking_oracle as ro
+
+pytestmark = pytest.mark.gpu
+
+F32, F64, F16, BF16 = torch.float32, torch.float64, torch.float16, torch.bfloat16
+NAN, INF = float('nan'), float('inf')
+
+
+def gpu(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return t if dtype is None else t.to(dtype)
+
+
+def host(t):
+    return t.detach().to(F64).cpu().numpy() if t.is_floating_point() else t.cpu().numpy()
+
+
+def strided(t, pad=3, offset=1):
+    """The same values in rows `pad` elements further apart, starting `offset` elements into the
+    memory."""
+    n, m = t.shape
+    flat = torch.full((offset + n * (m + pad),), 7.0, dtype=t.dtype, device=t.device)
+    view = flat[offset:].view(n, m + pad)[:, :m]
+    view.copy_(t)
+    return view, flat
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+# ------------------------------------------------------------------------------------ quantise
+SHAPES = [(1, 1), (3, 8), (5, 31), (4, 32), (7, 33), (300, 10), (17, 64), (9, 100), (130, 128),
+          (2, 1000), (3, 2047), (2, 2049), (1, 9000)]
+
+
+@pytest.mark.parametrize('dtype', [F32, F64, F16, BF16])
+@pytest.mark.parametrize('shape', SHAPES)
+def test_quantize_matches_definition(shape, dtype):
+    rng = np.random.default_rng(shape[0] * 1000 + shape[1])
+    x = rng.standard_normal(shape) * np.exp(rng.standard_normal((shape[0], 1)) * 3)
+    x[rng.random(shape) < 0.05] = 0.0
+    xd = gpu(x).to(dtype)
+    want_c, want_s = ro.mx4_quantize(host(xd))
+    for source in (xd, strided(xd)[0], strided(xd, 5, 2)[0]):
+        t = rk.mx4_quantize(source)
+        assert t.shape == shape and t.width == shape[1]
+        np.testing.assert_array_equal(t.scales.cpu().numpy(), want_s)
+        np.testing.assert_array_equal(t.codes.cpu().numpy(), want_c)
+    assert t.nbytes == 17 * shape[0] * ((shape[1] + 31) // 32)
+
+
+@pytest.mark.parametrize('dtype', [F32, F64, F16, BF16])
+def test_quantize_ties_extremes_and_non_finite(dtype):
+    """Every midpoint and its neighbours at scales from the smallest to the largest the type
+    has, blocks of zeros, and blocks with infinities and NaN beside ordinary ones."""
+    info = torch.finfo(dtype)
+    edge = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    rows = []
+    lo, hi = int(np.floor(np.log2(info.tiny))), int(np.floor(np.log2(info.max)))
+    for e in {lo - 2, lo, lo + 3, -20, 0, 7, hi - 3, hi - 2}:
+        with np.errstate(over='ignore'):
+            base = np.ldexp(np.concatenate((edge, edge * (1 + info.eps), edge * (1 - info.eps / 2),
+                                            [4.0, 6.0, 7.0, 0.0, 0.5, 1.0, 7.9, 4.5, 3.0, 2.0, 1.5])),
+                            e)
+        rows += [base, -base, base[::-1]]
+    x = torch.tensor(np.array(rows), dtype=F64).to(dtype)
+    extra = torch.zeros(8, 32, dtype=dtype)
+    extra[1] = -0.0
+    extra[2, 5], extra[3, 31], extra[4, 0] = INF, -INF, NAN
+    extra[5] = info.max
+    extra[6] = info.smallest_normal / 4
+    extra[7, 9] = info.smallest_normal * info.eps  # the smallest denormal
+    x = torch.cat((x, extra))
+    x = torch.cat((x, x.flip(0)), dim=1)  # two blocks a row
+    want_c, want_s = ro.mx4_quantize(host(x))
+    t = rk.mx4_quantize(x.cuda())
+    np.testing.assert_array_equal(t.scales.cpu().numpy(), want_s)
+    np.testing.assert_array_equal(t.codes.cpu().numpy(), want_c)
+    np.testing.assert_array_equal(host(rk.mx4_dequantize(t, F64)),
+                                  ro.mx4_values(want_c, want_s, 64))
+
+
+def test_quantize_fp64_is_not_rounded_twice():
+    """Values within 1e-12 of a midpoint, which fp32 could not tell from it."""
+    mid = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    row = np.concatenate((mid * (1 + 1e-12), mid * (1 - 1e-12), mid, [4.0]))
+    x = np.stack((row, -row, row * 2.0 ** 300, row * 2.0 ** -300))
+    want_c, want_s = ro.mx4_quantize(x)
+    t = rk.mx4_quantize(gpu(x))
+    np.testing.assert_array_equal(t.scales.cpu().numpy(), want_s)
+    np.testing.assert_array_equal(t.codes.cpu().numpy(), want_c)
+
+
+@pytest.mark.parametrize('dtype', [F32, F64, F16, BF16])
+@pytest.mark.parametrize('n,width', [(1, 1), (256, 40), (5, 33), (3, 2080), (40, 256)])
+def test_dequantize_every_code_and_scale(n, width, dtype):
+    rng = np.random.default_rng(width)
+    b = (width + 31) // 32
+    codes = rng.integers(0, 256, (n, 16 * b), dtype=np.uint8)
+    scales = rng.integers(0, 256, (n, b), dtype=np.uint8)
+    scales.ravel()[:4] = np.array([0, 255, 254, 127], dtype=np.uint8)[:scales.size]
+    t = rk.Mx4Table(gpu(codes), gpu(scales), width)
+    want = torch.from_numpy(ro.mx4_values(codes, scales, width)).to(dtype)
+    np.testing.assert_array_equal(host(rk.mx4_dequantize(t, dtype)), host(want))
+    ids = rng.integers(-2, n + 2, 50).astype(np.int32)
+    ids[:3] = (-2 ** 31, 2 ** 31 - 1, n - 1)
+    picked = torch.full((50, width), NAN, dtype=dtype)
+    ok = (ids >= 0) & (ids < n)
+    picked[torch.from_numpy(ok)] = want[torch.from_numpy(ids[ok].astype(np.int64))]
+    out, flat = strided(torch.zeros(50, width, dtype=dtype, device='cuda'))
+    rk.mx4_dequantize(t, dtype, rows=gpu(ids), out=out)
+    np.testing.assert_array_equal(host(out), host(picked))
+    gaps = flat[1:].view(50, width + 3)[:, width:]
+    assert bool((gaps == 7).all()) and float(flat[0]) == 7
+
+
+# -------------------------------------------------------------------------------------- scores
+def check_scores(got, a, values, out_dtype, parts=3):
+    ref = a @ values.T
+    with np.errstate(invalid='ignore'):
+        mag = np.abs(a) @ np.abs(values).T
+    tol = parts * a.shape[1] * 2.0 ** -23 * mag + half_step(out_dtype) * np.abs(ref)
+    tol += torch.finfo(out_dtype).smallest_normal  # fp16 results below its normal range
+    bad = ~(np.abs(got - ref) <= tol)
+    nan = np.isnan(ref)
+    assert (np.isnan(got) == nan).all()
+    assert not (bad & ~nan).any(), (np.abs(got - ref) / mag).max()
+
+
+SCORES = [(1, 1, 1), (1, 17, 31), (3, 100, 32), (16, 65, 33), (17, 50, 64), (40, 37, 65),
+          (70, 130, 96), (5, 63, 128), (64, 64, 128), (33, 70, 129), (100, 200, 160),
+          (130, 257, 512), (2, 300, 1000), (1, 1, 4097), (20, 500, 640), (150, 260, 1024),
+          (300, 520, 300)]
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'f16', 'mx4'])
+@pytest.mark.parametrize('m,n,width', SCORES)
+def test_scores_match_definition(m, n, width, kind):
+    rng = np.random.default_rng(m + 10 * n + 100 * width)
+    codes, scales = ro.mx4_quantize(rng.standard_normal((n, width)) *
+                                    np.exp(rng.standard_normal((n, 1))))
+    values = ro.mx4_values(codes, scales, width)
+    table = rk.Mx4Table(gpu(codes), gpu(scales), width)
+    a = gpu(rng.standard_normal((m, width)))
+    if kind == 'mx4':
+        ca, sa = ro.mx4_quantize(host(a))
+        at, av = rk.Mx4Table(gpu(ca), gpu(sa), width), ro.mx4_values(ca, sa, width)
+    else:
+        at = a.to({'f32': F32, 'bf16': BF16, 'f16': F16}[kind])
+        av = host(at)
+    for out_dtype in (F32, BF16, F16):
+        check_scores(host(rk.mx4_scores(at, table, out_dtype=out_dtype)), av, values, out_dtype)
+    got = rk.mx4_scores(at, table)
+    assert got.dtype == (F32 if kind == 'mx4' else at.dtype)
+    # rows by id, some of them missing; strided activations and output
+    ids = rng.integers(-1, m + 1, m + 3).astype(np.int32)
+    picked = np.full((m + 3, width), np.nan)
+    ok = (ids >= 0) & (ids < m)
+    picked[ok] = av[ids[ok]]
+    source = at if kind == 'mx4' else strided(at)[0]
+    out, flat = strided(torch.zeros(m + 3, n, device='cuda'), 5, 3)
+    rk.mx4_scores(source, table, rows=gpu(ids), out=out)
+    check_scores(host(out), picked, values, F32)
+    assert bool((flat[3:].view(m + 3, n + 5)[:, n:] == 7).all()) and bool((flat[:3] == 7).all())
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'mx4'])
+@pytest.mark.parametrize('m,n,width', [(1, 300001, 64), (3, 540000, 130), (20, 140000, 132),
+                                       (1, 70001, 200), (257, 9001, 128), (2048, 2049, 192),
+                                       (513, 2000, 2080)])
+def test_scores_large(m, n, width, kind):
+    """Sizes that take the long-walk and one-step forms; a strip of items against the definition,
+    the rest against another order of the same items."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(m + n)
+    table = rk.mx4_quantize(torch.randn(n, width, generator=g, device='cuda'))
+    a = torch.randn(m, width, generator=g, device='cuda')
+    at = rk.mx4_quantize(a) if kind == 'mx4' else a.to({'f32': F32, 'bf16': BF16}[kind])
+    av = host(rk.mx4_dequantize(at)) if kind == 'mx4' else host(at)
+    got = rk.mx4_scores(at, table, out_dtype=F32)
+    strip = torch.cat((torch.arange(0, min(n, 64)), torch.arange(n // 2, n // 2 + 40) % n,
+                       torch.arange(max(0, n - 70), n))).cuda()
+    values = ro.mx4_values(table.codes[strip].cpu().numpy(), table.scales[strip].cpu().numpy(), width)
+    check_scores(host(got[:, strip]), av, values, F32)
+    back = rk.Mx4Table(table.codes.flip(0).contiguous(), table.scales.flip(0).contiguous(), width)
+    assert torch.equal(rk.mx4_scores(at, back, out_dtype=F32).flip(1), got)
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'f16', 'mx4'])
+@pytest.mark.parametrize('width', [40, 200])
+def test_scores_with_infinities_nan_and_extreme_scales(width, kind):
+    """A block that is no number makes its item's scores NaN and no other's; infinite and NaN
+    activations stay in their rows; elements behind the width are never looked at."""
+    rng = np.random.default_rng(width)
+    n, m = 40, 20
+    codes, scales = ro.mx4_quantize(rng.standard_normal((n, width)))
+    codes |= (codes & 0x77 == 0).astype(np.uint8) * 0x11  # no zeros: 0 * inf is NaN
+    codes |= ((codes & 0x07) == 0).astype(np.uint8)
+    codes |= ((codes & 0x70) == 0).astype(np.uint8) * 0x10
+    scales[3, 1] = 255
+    scales[5] = 0
+    scales[6] = 200
+    values = ro.mx4_values(codes, scales, width)
+    table = rk.Mx4Table(gpu(codes), gpu(scales), width)
+    a = rng.standard_normal((m, width))
+    if kind == 'mx4':
+        ca, sa = ro.mx4_quantize(a)
+        sa[4, 0] = 255
+        sa[7] = 1
+        at, av = rk.Mx4Table(gpu(ca), gpu(sa), width), ro.mx4_values(ca, sa, width)
+    else:
+        dtype = {'f32': F32, 'bf16': BF16, 'f16': F16}[kind]
+        a[2, 0], a[4, width - 1], a[9, 33] = np.inf, np.nan, -np.inf
+        if kind == 'f32':
+            a[11] *= 1e-38
+            a[12] *= 1e30
+        full = torch.full((m, width + 8), NAN, dtype=dtype, device='cuda')
+        full[:, :width] = gpu(a)
+        at = full[:, :width]
+        av = host(at)
+    got = host(rk.mx4_scores(at, table, out_dtype=F32))
+    with np.errstate(invalid='ignore', over='ignore'):
+        ref = (av[:, None, :] * values[None]).sum(-1)
+        mag = np.abs(av[:, None, :] * values[None]).sum(-1)
+    # Finite operands whose products leave fp32's range: +inf and -inf may meet in an fp32 sum
+    # (2^73 from the scale times 1e30 = 2^99.7), so only "not finite or within the tolerance" holds
+    past = np.isfinite(mag) & (mag > np.finfo(np.float32).max)
+    assert not past[np.arange(m) != 12].any()
+    inf = np.isinf(ref)
+    assert (np.isnan(got) == np.isnan(ref))[~past].all()
+    assert (got[inf] == ref[inf]).all()
+    ok = np.isfinite(ref) & ~past
+    # An activation's last part is cut at bf16's smallest number, 2^-133, so each product may lose
+    # that times the table's element; products below fp32's normal range are off by 2^-149 at most.
+    with np.errstate(invalid='ignore'):
+        lost = 2.0 ** -133 * np.abs(values).max(1) + 3 * 2.0 ** -149
+        tol = width * (3 * 2.0 ** -23 * mag + lost)
+        worst = np.argwhere(ok & ~(np.abs(got - ref) <= tol))
+    assert worst.size == 0, [(i, j, got[i, j], ref[i, j], tol[i, j]) for i, j in worst[:8]]
+
+
+def test_scores_of_nothing():
+    table = rk.mx4_quantize(torch.randn(5, 40, device='cuda'))
+    none = rk.mx4_quantize(torch.randn(0, 40, device='cuda'))
+    assert len(none) == 0
+    assert rk.mx4_scores(torch.zeros(0, 40, device='cuda'), table).shape == (0, 5)
+    assert rk.mx4_scores(torch.zeros(2, 40, device='cuda'), none).shape == (2, 0)
+    assert rk.mx4_dequantize(none).shape == (0, 40)
+
+
+# -------------------------------------------------------------------------------------- adjust
+def lists(rng, rows, items, mean, low=-3, high=3):
+    n = rng.poisson(mean, rows)
+    n[rng.random(rows) < 0.2] = 0
+    ptr = np.concatenate(([0], np.cumsum(n))).astype(np.int64)
+    ids = rng.integers(low, max(items // 3, 1) + high, int(ptr[-1])).astype(np.int32)
+    return ptr, ids
+
+
+ADJUST = [(1, 1), (3, 31), (2, 64), (4, 1000), (5, 2048), (3, 2049), (2, 5003), (33, 300)]
+
+
+def adjust_case(rng, n, m, what):
+    kw, want = {}, {}
+    if 'history' in what or 'exclude' in what:
+        h = lists(rng, n, m, 40)
+        kw['history'], want['history'] = tuple(map(gpu, h)), h
+    if 'exclude' in what:
+        kw['exclude'] = want['exclude'] = True
+    if 'history' in what:
+        for name, v in (('repetition', 1.3), ('frequency', 0.25), ('presence', -0.5)):
+            if 'tensors' in what:
+                v = (v * rng.uniform(0.5, 2, n)).astype(np.float32)
+                kw[name], want[name] = gpu(v), v
+            else:
+                kw[name] = want[name] = v
+    if 'rows' in what:
+        r = rng.integers(-1, n + 2, n).astype(np.int32)
+        kw['history_rows'], want['history_rows'] = gpu(r), r
+    if 'bias' in what:
+        want['item_bias'] = rng.standard_normal(m).astype(np.float32)
+        kw['item_bias'] = gpu(want['item_bias'])
+        p, i = lists(rng, n, m, 9)
+        v = rng.standard_normal(i.size).astype(np.float32)
+        kw['row_bias'], want['row_bias'] = (gpu(p), gpu(i), gpu(v)), (p, i, v)
+    if 'mask' in what:
+        allowed = rng.random((4, m)) < 0.6
+        allowed[1] = False
+        words = rk.pack_mask(allowed)
+        r = rng.integers(-1, 5, n).astype(np.int32)
+        kw['mask'], want['mask'] = gpu(words), words
+        kw['mask_rows'], want['mask_rows'] = gpu(r), r
+    return kw, want
+
+
+@pytest.mark.parametrize('dtype', [F32, F64, F16, BF16])
+@pytest.mark.parametrize('what', ['', 'history', 'history tensors rows', 'exclude', 'exclude rows mask',
+                                  'bias', 'mask', 'history tensors bias mask'])
+@pytest.mark.parametrize('n,m', ADJUST)
+def test_adjust_matches_definition(n, m, what, dtype):
+    rng = np.random.default_rng(n * 10007 + m)
+    s = gpu(rng.standard_normal((n, m)) * 3).to(dtype)
+    kw, want = adjust_case(rng, n, m, what)
+    ref, mag = ro.adjust_scores(host(s), **want)
+    eps = half_step(F64 if dtype == F64 else F32)
+    tol = 8 * eps * mag + half_step(dtype) * np.where(np.isfinite(ref), np.abs(ref), 0)
+    tol += torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    inf = np.isinf(ref)
+
+    def check(got):
+        got = host(got)
+        assert (got[inf] == ref[inf]).all()
+        assert (np.abs(got[~inf] - ref[~inf]) <= tol[~inf]).all()
+    kept = s.clone()
+    check(rk.adjust_scores(s, **kw))
+    assert torch.equal(s, kept)
+    # strided in, strided out, nothing written between the rows
+    source, _ = strided(s)
+    out, flat = strided(torch.zeros_like(s), 4, 2)
+    check(rk.adjust_scores(source, out=out, **kw))
+    assert bool((flat[2:].view(n, m + 4)[:, m:] == 7).all()) and bool((flat[:2] == 7).all())
+    # in place, contiguous and strided
+    again = s.clone()
+    assert rk.adjust_scores(again, out=again, **kw) is again
+    check(again)
+    inner, flat = strided(s)
+    check(rk.adjust_scores(inner, out=inner, **kw))
+    assert bool((flat[1:].view(n, m + 3)[:, m:] == 7).all())
+
+
+def test_adjust_non_finite_scores():
+    """NaN and infinities stay where nothing takes them out, and go where the mask or the
+    exclusion does; the type's lowest value is an ordinary score."""
+    m = 40
+    for dtype in (F32, F16, BF16, F64):
+        low = torch.finfo(dtype).min
+        s = torch.zeros(2, m, dtype=dtype, device='cuda')
+        s[:, 0], s[:, 1], s[:, 2], s[:, 3] = NAN, INF, -INF, low
+        s[:, 10], s[:, 11], s[:, 12] = NAN, INF, -INF
+        allowed = np.ones((2, m), dtype=bool)
+        allowed[1, 10:13] = False
+        h = (gpu(np.array([0, 3, 6], dtype=np.int64)), gpu(np.array([0, 1, 2] * 2, dtype=np.int32)))
+        got = rk.adjust_scores(s, history=h, repetition=2.0, frequency=1.0, presence=1.0,
+                               mask=gpu(rk.pack_mask(allowed)))
+        assert bool(torch.isnan(got[:, 0]).all())
+        assert bool((got[:, 1] == INF).all()) and bool((got[:, 2] == -INF).all())
+        assert bool((got[:, 3] == low).all())
+        assert bool(torch.isnan(got[0, 10])) and float(got[0, 11]) == INF
+        assert bool((got[1, 10:13] == -INF).all())
+        out = rk.adjust_scores(s, history=h, exclude=True)
+        assert bool((out[:, :3] == -INF).all()) and bool(torch.isnan(out[:, 10]).all())
+
+
+def test_adjust_many_occurrences_and_long_lists():
+    """One item 100 000 times, lists longer than a workgroup's turn, the last of equal bias
+    entries, pointers that leave the list."""
+    m, n = 5000, 3
+    rng = np.random.default_rng(5)
+    ids = np.concatenate((np.full(100000, 17), rng.integers(0, m, 30000), [-1, m, 2 ** 31 - 1]))
+    ptr = np.array([0, 100000, ids.size, ids.size], dtype=np.int64)
+    h = (gpu(ptr), gpu(ids.astype(np.int32)))
+    s = torch.zeros(n, m, dtype=F32, device='cuda')
+    got = host(rk.adjust_scores(s, history=h, frequency=1.0))
+    for r in range(n):
+        part = ids[ptr[r]:ptr[r + 1]]
+        want = -np.bincount(part[(part >= 0) & (part < m)], minlength=m).astype(np.float64)
+        np.testing.assert_array_equal(got[r], want)
+    values = rng.standard_normal(ids.size).astype(np.float32)
+    got = host(rk.adjust_scores(s, row_bias=h + (gpu(values),)))
+    assert got[0, 17] == values[99999]
+    wide = (gpu(np.array([-5, 4, 2, 10 ** 12], dtype=np.int64)), h[1][:6].contiguous())
+    got = host(rk.adjust_scores(s, history=wide, frequency=1.0))
+    assert got[0, 17] == -4 and (got[1] == 0).all() and got[2, 17] == -4
+
+
+# ---------------------------------------------------------------------------------------- topk
+def check_topk(s, k, **kw):
+    items, best = rk.topk_rows(s, k, **kw)
+    raw = s.contiguous().cpu()
+    view = raw.view(torch.int16).numpy().view(np.float16) if s.dtype == BF16 else raw.numpy()
+    want = ro.topk_rows(view, k)
+    np.testing.assert_array_equal(items.cpu().numpy(), want)
+    picked = torch.gather(raw, 1, torch.from_numpy(want.astype(np.int64)))
+    assert best.dtype == s.dtype
+    np.testing.assert_array_equal(host(best), host(picked))
+
+
+TOPK = [(1, 1, 1), (3, 5, 5), (2, 64, 7), (2, 1024, 1024), (2, 4096, 10), (2, 4097, 1), (3, 4097, 1024),
+        (1, 50000, 1024), (5, 10000, 100), (1, 300000, 64), (2, 8191, 300), (40, 3000, 33),
+        (1, 1000003, 10), (300, 257, 20), (2, 20000, 512), (9, 26744, 10)]
+
+
+@pytest.mark.parametrize('dtype', [F32, F64, F16, BF16])
+@pytest.mark.parametrize('n,m,k', TOPK)
+def test_topk_matches_definition(n, m, k, dtype):
+    g = torch.Generator(device='cuda')
+    g.manual_seed(n + 7 * m + k)
+    s = torch.randn(n, m, generator=g, device='cuda').to(dtype)
+    check_topk(s, k)
+    check_topk(strided(s)[0], k)
+    # sorted rows: the best all in one place
+    check_topk(torch.sort(s, dim=1, descending=True).values.contiguous(), k)
+    check_topk(torch.sort(s, dim=1).values.contiguous(), k)
+
+
+@pytest.mark.parametrize('dtype', [F32, F64, F16, BF16])
+@pytest.mark.parametrize('m,k', [(50, 50), (4096, 1024), (9000, 10), (9000, 1000), (60000, 257)])
+def test_topk_ties_and_special_values(m, k, dtype):
+    """All scores equal, all -inf, a few different ones, -inf except for fewer than k, NaN of
+    both signs, both zeros, denormals."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(m + k)
+    rows = [torch.full((m,), 1.5), torch.full((m,), -INF), torch.zeros(m),
+            torch.randint(0, 3, (m,), generator=g, device='cuda').cpu().float(),
+            torch.full((m,), -INF), torch.randn(m), torch.randn(m) * 0]
+    rows[4][torch.randperm(m)[:max(1, k // 2)]] = 2.0
+    rows[5][torch.randperm(m)[:10]] = NAN
+    rows[5][torch.randperm(m)[:10]] = INF
+    s = torch.stack(rows).to(dtype)
+    s[5, m // 3] = -s[5, m // 3].abs()
+    s[5, m // 2] = torch.copysign(torch.tensor(NAN), torch.tensor(-1.0)).to(dtype)
+    s[6, 1::3] = -0.0
+    s[6, 2::3] = torch.finfo(dtype).smallest_normal / 2
+    check_topk(s.cuda(), k)
+
+
+def test_topk_batches():
+    s = torch.randn(50, 9000, device='cuda')
+    check_topk(s, 20, max_workspace_bytes=20000)
+    check_topk(strided(s)[0], 20, max_workspace_bytes=1)
+
+
+# ------------------------------------------------------------------------------- used together
+def chain(state, k):
+    t = rk.mx4_quantize(state['items'])
+    s = rk.mx4_scores(state['users'], t, rows=state['ids'])
+    s = rk.adjust_scores(s, history=state['history'], history_rows=state['ids'], exclude=True,
+                         item_bias=state['bias'], mask=state['mask'])
+    return rk.topk_rows(s, k) + (s,)
+
+
+def chain_state(rng, n=30, m=5000, width=50, sel=17):
+    allowed = rng.random(m) < 0.7
+    return {'items': gpu(rng.standard_normal((m, width)), F32),
+            'users': gpu(rng.standard_normal((n, width)), F32),
+            'ids': gpu(rng.integers(0, n, sel).astype(np.int32)),
+            'history': tuple(map(gpu, lists(rng, n, m, 60, 0, 0))),
+            'bias': gpu(rng.standard_normal(m).astype(np.float32)),
+            'mask': gpu(rk.pack_mask(allowed))}
+
+
+def test_catalogue_in_four_bits_to_lists():
+    """Quantise, score, adjust, select, against the same steps in 64 bits: every listed score is
+    its item's score, nothing that is taken out is listed, nothing better is missing."""
+    st = chain_state(np.random.default_rng(3))
+    items, best, _ = (host(t) for t in chain(st, 25))
+    codes, scales = ro.mx4_quantize(host(st['items']))
+    values = ro.mx4_values(codes, scales, 50)
+    ids = host(st['ids'])
+    users = host(st['users'])[ids]
+    ref, _ = ro.adjust_scores(users @ values.T, tuple(host(t) for t in st['history']), ids,
+                              exclude=True, item_bias=host(st['bias']), mask=host(st['mask']))
+    mag = np.abs(users) @ np.abs(values).T + np.abs(host(st['bias']))
+    tol = (3 * 50 + 2) * 2.0 ** -23 * mag
+    pick = lambda x: np.take_along_axis(x, items.astype(np.int64), axis=1)
+    assert np.isfinite(best).all()
+    assert (np.abs(best - pick(ref)) <= pick(tol)).all()
+    rest = ref.copy()
+    np.put_along_axis(rest, items.astype(np.int64), -np.inf, axis=1)
+    assert (rest.max(1) <= best[:, -1] + tol.max(1)).all()
+
+
+def test_chain_captured_and_replayed():
+    """The chain in a graph, replayed with other inputs in the same memory, with eager work between
+    the replays."""
+    rng = np.random.default_rng(4)
+    st = chain_state(rng)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        chain(st, 25)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain(st, 25)
+    for step in range(4):
+        st['items'].copy_(gpu(rng.standard_normal((5000, 50)), F32))
+        st['ids'].copy_(gpu(rng.integers(0, 30, 17).astype(np.int32)))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = chain(st, 25)
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    rng = np.random.default_rng(6)
+    states = [chain_state(rng) for _ in range(2)]
+    want = [chain(s, 25) for s in states]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in states]
+    for _ in range(5):
+        got = []
+        for s, stream in zip(states, streams):
+            with torch.cuda.stream(stream):
+                got.append(chain(s, 25))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize('rank,m', [(3, 40), (20, 700), (64, 2000), (100, 333)])
+@pytest.mark.parametrize('dtype', ['float32', 'float64'])
+def test_score_items_is_the_block_that_is_ranked(rank, m, dtype):
+    from alsmi import device as dev
+    device = dev.require_gpu()
+    rng = np.random.default_rng(rank)
+    U, V = rng.standard_normal((rank, 50)), rng.standard_normal((rank, m))
+    Ud, Vd = dev.factors_to_device(U, dtype, device), dev.factors_to_device(V, dtype, device)
+    users = rng.integers(0, 50, 70).astype(np.int32)
+    s = dev.score_items(rank, gpu(users), Ud, Vd)
+    Uq, Vq = dev.factors_to_host(Ud, rank), dev.factors_to_host(Vd, rank)
+    mag = np.abs(Uq[:, users]).T @ np.abs(Vq)
+    # fp32: the fp16 split keeps 2^-20 of each product, the sums add 3 * 128 roundings
+    tol = (2.0 ** -20 + 3 * 128 * 2.0 ** -24 if dtype == 'float32' else 130 * 2.0 ** -53) * mag
+    assert (np.abs(host(s) - Uq[:, users].T @ Vq) <= tol).all()
+    items, best = rk.topk_rows(s, 10)
+    want_items, want = dev.topk_items(rank, gpu(users), Ud, Vd, 10)
+    assert torch.equal(items, want_items) and torch.equal(best, want)
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'float64'])
+def test_recommend_with_exclusion_bias_mask_and_quantised_items(dtype, monkeypatch):
+    import pickle
+    from alsmi import ALS
+    import scipy.sparse as sps
+    rng = np.random.default_rng(11)
+    n, m, k = 60, 500, 12
+    R = sps.random(n, m, 0.08, format='csr', random_state=1, data_rvs=lambda s: rng.integers(1, 6, s))
+    R = sps.vstack([R, sps.csr_matrix((1, m))], format='csr')      # a user without ratings
+    rows, cols = R.nonzero()
+    als = ALS(8, random_state=0, max_iter=3, dtype=dtype).fit((rows, cols), R)
+    triplets = ALS(8, random_state=0, max_iter=3, dtype=dtype).fit(
+        (rows.astype(np.int32), cols.astype(np.int32)), np.asarray(R[rows, cols]).ravel(), shape=R.shape)
+    users = np.concatenate((rng.integers(0, n + 1, 30), [n, -1]))
+    bias = rng.standard_normal(m).astype(np.float32)
+    one, each = rng.random(m) < 0.5, rng.random((users.size, m)) < 0.3
+    each[3] = False
+    each[4, 7:] = False
+    dense = als.user_feats.T @ als.item_feats
+    codes, scales = ro.mx4_quantize(als.item_feats.T)
+    coarse = als.user_feats.T @ ro.mx4_values(codes, scales, 8).T
+    seen = R.toarray() != 0
+    for kw in (dict(exclude_seen=True), dict(item_bias=bias), dict(allowed=one), dict(allowed=each),
+               dict(exclude_seen=True, item_bias=bias, allowed=each), dict(catalogue='mx4'),
+               dict(exclude_seen=True, item_bias=bias, allowed=one, catalogue='mx4')):
+        want = (coarse if kw.get('catalogue') == 'mx4' else dense)[users].copy()
+        if 'item_bias' in kw:
+            want += bias
+        if kw.get('exclude_seen'):
+            want[seen[users]] = -np.inf
+        if 'allowed' in kw:
+            want[~np.broadcast_to(kw['allowed'], want.shape)] = -np.inf
+        tol = 1e-10 if dtype == 'float64' and 'catalogue' not in kw else 2e-5
+        for model, block in ((als, None), (triplets, None), (als, 7)):
+            if block:  # several blocks of users
+                monkeypatch.setattr('alsmi.als._BLOCK_SCORES', block * m)
+            items, scores = model.recommend(users, k, **kw)
+            monkeypatch.undo()
+            got = np.take_along_axis(want, items.astype(np.int64), axis=1)
+            out = np.isinf(scores)
+            assert (np.isinf(got) == out).all()
+            assert np.abs(scores[~out] - got[~out]).max() <= tol
+            rest = want.copy()
+            np.put_along_axis(rest, items.astype(np.int64), -np.inf, axis=1)
+            assert (rest.max(1) <= scores[:, -1] + tol).all()
+            assert all(np.unique(r).size == k for r in items)
+    # nothing on offer: the smallest ids, all at -inf
+    items, scores = als.recommend([0], 3, allowed=np.zeros(m, bool))
+    assert list(items[0]) == [0, 1, 2] and np.isinf(scores).all()
+    copy = pickle.loads(pickle.dumps(als))
+    a, b = copy.recommend(users, k, catalogue='mx4'), als.recommend(users, k, catalogue='mx4')
+    assert (a[0] == b[0]).all() and (a[1] == b[1]).all()
+    # a new rating is seen, and the changed user is scored with the new factors
+    best = int(als.recommend([0], 1, exclude_seen=True)[0][0, 0])
+    als.update_user(0, best, 5.0)
+    assert best not in als.recommend([0], k, exclude_seen=True)[0]
+    with pytest.raises(ValueError):
+        als.recommend([0], m + 1, exclude_seen=True)

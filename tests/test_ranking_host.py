@@ -1,0 +1,213 @@
+"""The ranking operators' refusals and host-side parts (no GPU): the functions of alsmi.ranking reject
+what does not fit before anything is launched, and so do the entry points of the C ABI."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from alsmi import _lib, ranking as rk
+from oracle import ranking_oracle as ro
+
+
+def table(n=4, width=40):
+    codes, scales = ro.mx4_quantize(np.random.default_rng(0).standard_normal((n, width)))
+    return rk.Mx4Table(torch.from_numpy(codes), torch.from_numpy(scales), width)
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def i64(*v):
+    return torch.tensor(v, dtype=torch.int64)
+
+
+def f32(*v):
+    return torch.tensor(v, dtype=torch.float32)
+
+
+X = torch.zeros(3, 8)
+HIST = (i64(0, 1, 1, 2), i32(0, 1))
+
+REFUSED = {
+    'quantize: 1-D': (lambda: rk.mx4_quantize(torch.zeros(8)), '2-D'),
+    'quantize: integers': (lambda: rk.mx4_quantize(torch.zeros(2, 8, dtype=torch.int32)), 'one of'),
+    'quantize: no columns': (lambda: rk.mx4_quantize(torch.zeros(2, 0)), 'columns'),
+    'quantize: columns': (lambda: rk.mx4_quantize(torch.zeros(8, 2).t()), 'unit stride'),
+    'quantize: expanded': (lambda: rk.mx4_quantize(torch.zeros(1, 8).expand(3, 8)), 'overlapping'),
+    'quantize: gradient': (lambda: rk.mx4_quantize(torch.zeros(2, 8, requires_grad=True)), 'gradient'),
+    'quantize: host': (lambda: rk.mx4_quantize(X), 'HIP device'),
+    'table: codes': (lambda: rk.Mx4Table(torch.zeros(2, 16, dtype=torch.uint8),
+                                         torch.zeros(2, 2, dtype=torch.uint8), 40), 'codes'),
+    'table: scales': (lambda: rk.Mx4Table(torch.zeros(2, 32, dtype=torch.uint8),
+                                          torch.zeros(2, 1, dtype=torch.uint8), 40), 'scales'),
+    'table: rows': (lambda: rk.Mx4Table(torch.zeros(2, 32, dtype=torch.uint8),
+                                        torch.zeros(3, 2, dtype=torch.uint8), 40), 'number of rows'),
+    'table: width': (lambda: rk.Mx4Table(torch.zeros(2, 0, dtype=torch.uint8),
+                                         torch.zeros(2, 0, dtype=torch.uint8), 0), 'width'),
+    'table: alignment': (lambda: rk.Mx4Table(torch.zeros(33, dtype=torch.uint8)[1:].view(2, 16),
+                                             torch.zeros(2, 1, dtype=torch.uint8), 32), 'aligned'),
+    'dequantize: no table': (lambda: rk.mx4_dequantize(X), 'Mx4Table'),
+    'dequantize: type': (lambda: rk.mx4_dequantize(table(), torch.int32), 'dtype'),
+    'dequantize: rows': (lambda: rk.mx4_dequantize(table(), rows=i64(0)), 'rows'),
+    'dequantize: out': (lambda: rk.mx4_dequantize(table(), out=torch.zeros(4, 41)), 'shape'),
+    'dequantize: host': (lambda: rk.mx4_dequantize(table()), 'HIP device'),
+    'scores: width': (lambda: rk.mx4_scores(torch.zeros(2, 39), table()), 'columns'),
+    'scores: fp64': (lambda: rk.mx4_scores(torch.zeros(2, 40, dtype=torch.float64), table()), 'one of'),
+    'scores: out type': (lambda: rk.mx4_scores(torch.zeros(2, 40), table(),
+                                               out_dtype=torch.float64), 'out_dtype'),
+    'scores: out shape': (lambda: rk.mx4_scores(torch.zeros(2, 40), table(),
+                                                out=torch.zeros(2, 5)), 'shape'),
+    'scores: rows of nothing': (lambda: rk.mx4_scores(torch.zeros(0, 40), table(), rows=i32(0)), 'empty'),
+    'scores: rows type': (lambda: rk.mx4_scores(torch.zeros(2, 40), table(), rows=i64(0)), 'rows'),
+    'scores: no table': (lambda: rk.mx4_scores(torch.zeros(2, 40), torch.zeros(4, 40)), 'Mx4Table'),
+    'scores: host': (lambda: rk.mx4_scores(torch.zeros(2, 40), table()), 'HIP device'),
+    'adjust: type': (lambda: rk.adjust_scores(X.to(torch.int32)), 'one of'),
+    'adjust: history type': (lambda: rk.adjust_scores(X, history=(i32(0, 0, 0, 0), i32(0))), 'pointers'),
+    'adjust: history ids': (lambda: rk.adjust_scores(X, history=(i64(0, 0, 0, 0), i64(0))), 'ids'),
+    'adjust: history shape': (lambda: rk.adjust_scores(X, history=HIST[0]), 'tuple'),
+    'adjust: lists': (lambda: rk.adjust_scores(X, history=(i64(0, 1), i32(0))), 'lists'),
+    'adjust: no pointers': (lambda: rk.adjust_scores(X, history=(i64(), i32()),
+                                                     history_rows=i32(0, 0, 0)), 'pointers'),
+    'adjust: history rows': (lambda: rk.adjust_scores(X, history=HIST, history_rows=i32(0)), 'history_rows'),
+    'adjust: rows without lists': (lambda: rk.adjust_scores(X, history_rows=i32(0, 0, 0)), 'need a history'),
+    'adjust: exclude nothing': (lambda: rk.adjust_scores(X, exclude=True), 'need a history'),
+    'adjust: penalty': (lambda: rk.adjust_scores(X, presence=1.0), 'needs a history'),
+    'adjust: excluded penalty': (lambda: rk.adjust_scores(X, history=HIST, exclude=True,
+                                                          frequency=1.0), 'needs a history'),
+    'adjust: repetition': (lambda: rk.adjust_scores(X, history=HIST, repetition=0.0), 'positive'),
+    'adjust: NaN': (lambda: rk.adjust_scores(X, history=HIST, presence=float('nan')), 'a number'),
+    'adjust: penalty size': (lambda: rk.adjust_scores(X, history=HIST, frequency=f32(1.0)), 'entries'),
+    'adjust: bias size': (lambda: rk.adjust_scores(X, item_bias=f32(1.0)), 'entries'),
+    'adjust: row bias lists': (lambda: rk.adjust_scores(X, row_bias=(i64(0, 1), i32(0), f32(1))), 'row_bias'),
+    'adjust: row bias values': (lambda: rk.adjust_scores(X, row_bias=(i64(0, 1, 1, 1), i32(0), f32(1, 2))),
+                                'entries'),
+    'adjust: mask words': (lambda: rk.adjust_scores(X, mask=torch.zeros(3, 2, dtype=torch.int32)), 'mask'),
+    'adjust: mask rows': (lambda: rk.adjust_scores(X, mask=torch.zeros(2, 1, dtype=torch.int32)), 'one row'),
+    'adjust: no masks': (lambda: rk.adjust_scores(X, mask=torch.zeros(0, 1, dtype=torch.int32),
+                                                  mask_rows=i32(0, 0, 0)), 'no rows'),
+    'adjust: rows without mask': (lambda: rk.adjust_scores(X, mask_rows=i32(0, 0, 0)), 'needs a mask'),
+    'adjust: out type': (lambda: rk.adjust_scores(X, out=X.to(torch.float16)), 'out'),
+    'adjust: out overlaps': (lambda: rk.adjust_scores(torch.zeros(40)[:24].view(3, 8),
+                                                      out=X), 'HIP device'),
+    'adjust: host': (lambda: rk.adjust_scores(X), 'HIP device'),
+    'topk: k = 0': (lambda: rk.topk_rows(X, 0), 'k must'),
+    'topk: k': (lambda: rk.topk_rows(X, 9), 'k must'),
+    'topk: k > 1024': (lambda: rk.topk_rows(torch.zeros(1, 2000), 1025), 'k must'),
+    'topk: type': (lambda: rk.topk_rows(X.to(torch.int64), 1), 'one of'),
+    'topk: host': (lambda: rk.topk_rows(X, 1), 'HIP device'),
+}
+
+
+@pytest.mark.parametrize('name', sorted(REFUSED))
+def test_refused(name):
+    call, match = REFUSED[name]
+    with pytest.raises(ValueError, match=match):
+        call()
+
+
+def test_overlapping_output_is_refused():
+    base = torch.zeros(64)
+    with pytest.raises(ValueError, match='overlap'):
+        rk.adjust_scores(base[:24].view(3, 8), out=base[8:32].view(3, 8))
+    t = table()
+    with pytest.raises(ValueError, match='overlap'):
+        a = base[:40].view(1, 40)
+        rk.mx4_scores(a, t, out=base[:4].view(1, 4))
+
+
+def test_pack_mask():
+    rng = np.random.default_rng(1)
+    for n, m in ((1, 1), (3, 31), (2, 32), (4, 33), (2, 100)):
+        allowed = rng.random((n, m)) < 0.5
+        words = rk.pack_mask(allowed)
+        assert words.dtype == np.int32 and words.shape == (n, (m + 31) // 32)
+        bit = np.arange(m)
+        assert (((words[:, bit // 32] >> (bit % 32)) & 1).astype(bool) == allowed).all()
+        # nothing set behind the last item
+        last = words[:, -1].view(np.uint32) >> np.uint32((m - 1) % 32)
+        assert (last <= 1).all()
+
+
+def test_c_entry_points_refuse():
+    """Status -1 and a message naming the call, for every argument that the kernels rely on."""
+    lib = _lib.load()
+    buf = (ctypes.c_double * 64)()
+    p = ctypes.cast(buf, ctypes.c_void_p)
+    odd = ctypes.c_void_p(p.value + 1)
+
+    def refused(name, *args):
+        assert getattr(lib, name)(*args) == -1
+        assert name.encode() in lib.alsmi_last_error()
+
+    q = 'alsmi_mx4_quantize'
+    refused(q, 4, 1, 8, p, 8, p, p, None)
+    refused(q, 0, -1, 8, p, 8, p, p, None)
+    refused(q, 0, 1, 0, p, 8, p, p, None)
+    refused(q, 0, 1, (1 << 20) + 1, p, 8, p, p, None)
+    refused(q, 0, 2, 8, p, 7, p, p, None)
+    refused(q, 0, 1, 8, None, 8, p, p, None)
+    refused(q, 0, 1, 8, p, 8, odd, p, None)
+    assert lib.alsmi_mx4_quantize(0, 0, 8, None, 8, None, None, None) == 0
+    d = 'alsmi_mx4_dequantize'
+    refused(d, 4, 1, None, 1, 8, p, p, p, 8, None)
+    refused(d, 0, 2, None, 1, 8, p, p, p, 8, None)
+    refused(d, 0, 2, None, 2, 8, p, p, p, 7, None)
+    refused(d, 0, 1, None, 1, 0, p, p, p, 8, None)
+    refused(d, 0, 1, None, 1, 8, odd, p, p, 8, None)
+    refused(d, 0, 1, None, 1, 8, p, p, None, 8, None)
+    s = 'alsmi_mx4_scores'
+    refused(s, 1, 1, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None)
+    refused(s, 0, 1, None, 1, p, 8, None, 1, 8, p, p, 1, p, 1, None)
+    refused(s, 0, 2, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None)
+    refused(s, 0, 1, p, 0, p, 8, None, 1, 8, p, p, 0, p, 1, None)
+    refused(s, 0, 2, None, 2, p, 7, None, 1, 8, p, p, 0, p, 1, None)
+    refused(s, 0, 2, None, 2, p, 8, None, 2, 8, p, p, 0, p, 1, None)
+    refused(s, 4, 1, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None)
+    refused(s, 4, 1, None, 1, odd, 8, p, 1, 8, p, p, 0, p, 1, None)
+    refused(s, 0, 1, None, 1, p, 8, None, 1, 8, odd, p, 0, p, 1, None)
+    assert lib.alsmi_mx4_scores(0, 0, None, 0, None, 8, None, 5, 8, None, None, 0, None, 5, None) == 0
+
+    def adjust(dtype=0, scores=p, out=p, **fields):
+        a = _lib.Adjust(n_rows=2, n_items=8, ld_scores=8, ld_out=8, repetition_value=1.0)
+        for name, value in fields.items():
+            setattr(a, name, value)
+        return lib.alsmi_adjust_scores(dtype, ctypes.byref(a), scores, out, None)
+
+    for bad in (dict(dtype=4), dict(scores=None), dict(out=None), dict(n_rows=-1), dict(ld_out=7),
+                dict(ld_scores=7), dict(history_ptr=p, n_history=1, n_history_rows=2),
+                dict(history_ptr=p, n_history=1, history_ids=p, n_history_rows=1),
+                dict(history_ptr=p, n_history=-1, history_ids=p, n_history_rows=2),
+                dict(bias_ptr=p, n_bias=1, bias_ids=p), dict(bias_ptr=p, n_bias=1, bias_values=p),
+                dict(mask=p, n_masks=0)):
+        assert adjust(**bad) == -1, bad
+        assert b'alsmi_adjust_scores' in lib.alsmi_last_error()
+    assert lib.alsmi_adjust_scores(0, None, p, p, None) == -1
+    assert adjust(n_rows=0) == 0
+    t = 'alsmi_topk_rows'
+    refused(t, 4, 1, 8, p, 8, 1, p, p, p, None)
+    refused(t, 0, 1, 8, p, 8, 0, p, p, p, None)
+    refused(t, 0, 1, 8, p, 8, 9, p, p, p, None)
+    refused(t, 0, 2, 8, p, 7, 1, p, p, p, None)
+    refused(t, 0, 1, 8, None, 8, 1, p, p, p, None)
+    refused(t, 0, 1, 8, p, 8, 1, p, p, ctypes.c_void_p(p.value + 8 if p.value % 16 == 0 else p.value),
+            None)
+    assert lib.alsmi_topk_rows_workspace_bytes(9, 1, 8, 1) == 0
+    assert lib.alsmi_topk_rows_workspace_bytes(0, 1, 8, 1) > 0
+    refused('alsmi_score_items', 2, 4, 1, p, p, p, 1, p, p, None)
+    refused('alsmi_score_items', 0, 129, 1, p, p, p, 1, p, p, None)
+    refused('alsmi_score_items', 0, 4, 1, None, p, p, 1, p, p, None)
+
+
+def test_recommend_refuses():
+    from alsmi import ALS
+    als = ALS(rank=3)
+    als.user_feats, als.item_feats = np.ones((3, 4)), np.ones((3, 5))
+    for kw, error in ((dict(catalogue='mx3'), ValueError), (dict(item_bias=np.zeros(4)), ValueError),
+                      (dict(allowed=np.ones(4)), ValueError), (dict(exclude_seen=True), ValueError),
+                      (dict(allowed=np.ones((3, 5))), ValueError)):
+        with pytest.raises(error):
+            als.recommend([0, 1], k=2, **kw)
+    with pytest.raises(IndexError):
+        als.recommend([4], k=2, exclude_seen=True)
