@@ -22,6 +22,9 @@ from . import _lib
 _CODES = {torch.float32: _lib.F32, torch.float64: _lib.F64, torch.float16: _lib.F16,
           torch.bfloat16: _lib.BF16}
 _FLOATS = tuple(_CODES)
+# the current stream's handle without a Stream object around it (a microsecond of a small call)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _NARROW = (torch.float32, torch.float16, torch.bfloat16)
 BLOCK = 32
 MAX_K = 1024
@@ -39,11 +42,14 @@ def _matrix(name, t, dtypes):
         raise ValueError('%s requires a gradient, which this operator does not give; detach it'
                          % name)
     n, m = t.shape
-    if m > 1 and t.stride(1) != 1:
+    row, step = t.stride()
+    if m > 1 and step != 1:
         raise ValueError('%s must have unit stride inside a row' % name)
-    if n > 1 and t.stride(0) < m:
-        raise ValueError('%s must not have overlapping rows' % name)
-    return max(t.stride(0), m) if n > 1 else m
+    if n > 1:
+        if row < m:
+            raise ValueError('%s must not have overlapping rows' % name)
+        return row
+    return m
 
 
 def _vector(name, t, dtype, size=None):
@@ -56,18 +62,14 @@ def _vector(name, t, dtype, size=None):
         raise ValueError('%s must have %d entries, got %d' % (name, size, t.numel()))
 
 
-def _device(**tensors):
-    """The HIP device all the given tensors are on."""
-    device = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError('%s must be on a HIP device; there is no CPU fallback' % name)
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError('%s is on %s, not on %s' % (name, t.device, device))
+def _device(t, *others):
+    """The HIP device that `t` and the other tensors (or None) are on."""
+    if not t.is_cuda:
+        raise ValueError('tensors must be on a HIP device; there is no CPU fallback')
+    device = t.device
+    for o in others:
+        if o is not None and o.device != device:
+            raise ValueError('tensors on %s and on %s in one call' % (device, o.device))
     return device
 
 
@@ -78,11 +80,14 @@ def _p(t):
 def _call(device, name, *args):
     """Enqueue an entry point on the current stream of `device`."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+            status = fn(*args, _raw_stream(index))
+    if status != 0:
+        _lib.check(status, name)
 
 
 def _overlap(a, b):
@@ -129,6 +134,13 @@ class Mx4Table(object):
             raise ValueError('codes must be aligned to 4 bytes')
         self.codes, self.scales, self.width = codes, scales, width
 
+    @classmethod
+    def _of(cls, codes, scales, width):
+        """A table of parts known to fit each other."""
+        self = cls.__new__(cls)
+        self.codes, self.scales, self.width = codes, scales, width
+        return self
+
     @property
     def shape(self):
         return (self.codes.shape[0], self.width)
@@ -155,13 +167,13 @@ def mx4_quantize(x):
     n, width = x.shape
     if not 1 <= width <= MAX_WIDTH:
         raise ValueError('x must have between 1 and %d columns, got %d' % (MAX_WIDTH, width))
-    device = _device(x=x)
+    device = _device(x)
     blocks = (width + BLOCK - 1) // BLOCK
     codes = torch.empty((n, blocks * 16), dtype=torch.uint8, device=device)
     scales = torch.empty((n, blocks), dtype=torch.uint8, device=device)
     _call(device, 'alsmi_mx4_quantize', _CODES[x.dtype], n, width, _p(x), ld, _p(codes),
           _p(scales))
-    return Mx4Table(codes, scales, width)
+    return Mx4Table._of(codes, scales, width)
 
 
 def mx4_dequantize(table, dtype=torch.float32, rows=None, out=None):
@@ -175,7 +187,7 @@ def mx4_dequantize(table, dtype=torch.float32, rows=None, out=None):
         _vector('rows', rows, torch.int32)
     n = len(table) if rows is None else rows.numel()
     out, ld = _result('out', out, (n, table.width), dtype, table.device, table.codes, table.scales)
-    device = _device(table=table.codes, scales=table.scales, rows=rows, out=out)
+    device = _device(table.codes, table.scales, rows, out)
     _call(device, 'alsmi_mx4_dequantize', _CODES[dtype], n, _p(rows), len(table), table.width,
           _p(table.codes), _p(table.scales), _p(out), ld)
     return out
@@ -209,8 +221,7 @@ def mx4_scores(a, table, rows=None, out_dtype=None, out=None):
     if m and a.shape[0] == 0:
         raise ValueError('rows of an empty a')
     out, ldo = _result('out', out, (m, len(table)), out_dtype, table.device, data, table.codes)
-    device = _device(a=data, a_scales=a_scales, table=table.codes, scales=table.scales, rows=rows,
-                     out=out)
+    device = _device(table.codes, table.scales, data, a_scales, rows, out)
     _call(device, 'alsmi_mx4_scores', code, m, _p(rows), a.shape[0], _p(data), ld, _p(a_scales),
           len(table), table.width, _p(table.codes), _p(table.scales), _CODES[out_dtype], _p(out),
           ldo)
@@ -335,7 +346,7 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
         out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores.device, scores)
     else:
         args.ld_out = ld
-    device = _device(scores=scores, out=out, **kept)
+    device = _device(scores, out, *kept.values())
     for name, t in kept.items():
         setattr(args, name, _p(t))
     _call(device, 'alsmi_adjust_scores', _CODES[scores.dtype], ctypes.byref(args), _p(scores),
@@ -352,7 +363,7 @@ def topk_rows(scores, k, max_workspace_bytes=1 << 30):
     k = int(k)
     if not 1 <= k <= min(MAX_K, m):
         raise ValueError('k must be between 1 and min(%d, number of items), got %r' % (MAX_K, k))
-    device = _device(scores=scores)
+    device = _device(scores)
     code = _CODES[scores.dtype]
     items = torch.empty((n, k), dtype=torch.int32, device=device)
     best = torch.empty((n, k), dtype=scores.dtype, device=device)

@@ -8,6 +8,8 @@
 #include "alsmi_common.h"
 #include "elem.h"
 
+#include <type_traits>
+
 namespace alsmi {
 
 constexpr int MX4_BLOCK = 32;
@@ -160,6 +162,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t n_sel,
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -249,31 +252,44 @@ struct Rows {
 struct ScoreStore {
     void *out;
     int64_t ld, n_sel, n_items;
-    int type;  // ALSMI_F32 / F16 / BF16
-    // four consecutive items of one output row
-    __device__ __forceinline__ void put(int64_t row, int64_t item, f32x4 v) const {
-        if (row >= n_sel || item >= n_items) return;
-        const int64_t at = row * ld + item;
-        const int n = n_items - item < 4 ? (int)(n_items - item) : 4;
-        if (type == ALSMI_F32) store_n<float>(static_cast<float *>(out) + at, v, n);
-        else if (type == ALSMI_BF16) store_n<__bf16>(static_cast<__bf16 *>(out) + at, v, n);
-        else store_n<_Float16>(static_cast<_Float16 *>(out) + at, v, n);
-    }
-    template <typename T>
-    static __device__ __forceinline__ void store_n(T *p, f32x4 v, int n) {
-        typedef T vec_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-        if (n == 4) {
-            *reinterpret_cast<vec_t *>(p) = __builtin_convertvector(v, vec_t);
-        } else {
-            for (int i = 0; i < n; ++i) p[i] = (T)v[i];
-        }
-    }
 };
+// A lane's part of one output row: the NT tiles' results v[n] for lane group g, 4 NT consecutive
+// items from `item` on.  (The NT tiles of a wave share out 16 NT items so that this is so: row i of
+// tile n is item (i / 4) 4 NT + 4 n + i % 4; one long store instead of NT short ones.)
+template <int NT>
+__device__ __forceinline__ int item_of(int n, int i) {
+    return (i >> 2) * 4 * NT + 4 * n + (i & 3);
+}
+template <typename TO, int NT>
+__device__ __forceinline__ void put_row(TO *row, int64_t item, int64_t n_items, const f32x4 (&v)[NT]) {
+    static_assert(NT % 2 == 0, "eight items per store");
+    typedef TO vec_t __attribute__((ext_vector_type(8), aligned(sizeof(TO))));
+    if (!row) return;
+    if (item + 4 * NT <= n_items) {
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+            vec_t w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (TO)v[n][i], w[4 + i] = (TO)v[n + 1][i];
+            *reinterpret_cast<vec_t *>(row + item + 4 * n) = w;
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (item + 4 * n + i < n_items) row[item + 4 * n + i] = (TO)v[n][i];
+    }
+}
+template <typename TO>
+__device__ __forceinline__ TO *out_row(const ScoreStore &o, int64_t row) {
+    return row < o.n_sel ? static_cast<TO *>(o.out) + row * o.ld : nullptr;
+}
 
 // Rows of at most four blocks (rank <= 128): UT tiles of 16 activation rows stay in registers,
 // split once, and the wave walks `tpw` tiles of 16 items.  Bound by the table's bytes for a few
 // rows, by the write of the scores for many.
-template <typename T, int NBL, int UT>
+template <typename T, typename TO, int NBL, int UT, int NT>
 __global__ __launch_bounds__(256) void mx4_scores_narrow_kernel(Rows rows, const T *__restrict__ a,
                                                                 int width,
                                                                 const uint8_t *__restrict__ codes,
@@ -281,23 +297,43 @@ __global__ __launch_bounds__(256) void mx4_scores_narrow_kernel(Rows rows, const
                                                                 int nb, ScoreStore o, int groups,
                                                                 int tpw) {
     constexpr int NP = Parts<T>::N;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int g = lane >> 4, q = lane & 15;
     const unsigned chunk = blockIdx.x / (unsigned)groups;
     const int64_t row_base = (int64_t)(blockIdx.x - chunk * groups) * (16 * UT);
     const int64_t n_tiles = (o.n_items + 15) / 16;
-    const int64_t t0 = ((int64_t)chunk * 4 + (threadIdx.x >> 6)) * tpw;
+    const int64_t t0 = ((int64_t)chunk * 4 + wave) * tpw;
     const int64_t t1 = t0 + tpw < n_tiles ? t0 + tpw : n_tiles;
-    if (t0 >= t1) return;
     const int blk = (g * NBL) >> 2;  // this lane's block
-    bf16x8 af[UT][NBL][NP];
+    // NT neighbouring tiles per turn: a lane's stores of one output row lie side by side.  The codes
+    // of the next turn are on their way during the products of this one.
+    unsigned c[NT][NBL];
+    unsigned sb[NT];
+    auto fetch = [&](int64_t tile) {
 #pragma unroll
-    for (int t = 0; t < UT; ++t) {
-        int64_t i = row_base + 16 * t + q;
-        i = i < rows.n_sel ? i : rows.n_sel - 1;  // (rows past the end are not stored)
-        const int64_t r = rows.of(i);
+        for (int n = 0; n < NT; ++n) {
+            int64_t item = 16 * tile + item_of<NT>(n, q);
+            item = item < o.n_items ? item : o.n_items - 1;
+            sb[n] = 127u;
 #pragma unroll
-        for (int j = 0; j < NBL; ++j) {
+            for (int j = 0; j < NBL; ++j) c[n][j] = 0;
+            if (blk < nb) {
+                load_codes<NBL>(c[n], codes + item * (16 * (int64_t)nb) + g * NBL * 4);
+                sb[n] = scales[item * nb + blk];
+            }
+        }
+    };
+    if (t0 < t1) fetch(t0);
+    // the four waves split a quarter of the activations each and hand them round through LDS
+    __shared__ bf16x8 shared_a[UT * NBL][NP][64];
+#pragma unroll
+    for (int f = 0; f < UT * NBL; f += 4) {
+        const int part = f + wave;
+        if (UT * NBL >= 4 || part < UT * NBL) {
+            const int t = part / NBL, j = part - t * NBL;
+            int64_t i = row_base + 16 * t + q;
+            i = i < rows.n_sel ? i : rows.n_sel - 1;  // (rows past the end are not stored)
+            const int64_t r = rows.of(i);
             const int k = (g * NBL + j) * 8;
             float x[8];
             load8<T>(x, a + (r < 0 ? 0 : r) * rows.ld + k, width - k);
@@ -305,42 +341,80 @@ __global__ __launch_bounds__(256) void mx4_scores_narrow_kernel(Rows rows, const
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = __builtin_nanf("");
             }
-            split8<NP>(x, af[t][j]);
+            bf16x8 h[NP];
+            split8<NP>(x, h);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) shared_a[part][p][lane] = h[p];
         }
     }
-    for (int64_t tile = t0; tile < t1; ++tile) {
-        int64_t item = 16 * tile + q;
-        item = item < o.n_items ? item : o.n_items - 1;
-        unsigned c[NBL];
-        float s = 1.0f;
+    __syncthreads();
+    if (t0 >= t1) return;
+    bf16x8 af[UT][NBL][NP];
 #pragma unroll
-        for (int j = 0; j < NBL; ++j) c[j] = 0;
-        if (blk < nb) {
-            load_codes<NBL>(c, codes + item * (16 * (int64_t)nb) + g * NBL * 4);
-            s = scale_value(scales[item * nb + blk]);
-        }
-        f32x4 acc[UT];
+    for (int t = 0; t < UT; ++t)
 #pragma unroll
-        for (int t = 0; t < UT; ++t) acc[t] = f32x4{0, 0, 0, 0};
+        for (int j = 0; j < NBL; ++j)
 #pragma unroll
-        for (int j = 0; j < NBL; ++j) {
-            const bf16x8 b = codes_to_bf16(c[j], s);
+            for (int p = 0; p < NP; ++p) af[t][j][p] = shared_a[t * NBL + j][p][lane];
+    TO *dst[UT];
+#pragma unroll
+    for (int t = 0; t < UT; ++t) dst[t] = out_row<TO>(o, row_base + 16 * t + q);
+    for (int64_t tile = t0; tile < t1; tile += NT) {
+        bf16x8 b[NT][NBL];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < NBL; ++j) b[n][j] = codes_to_bf16(c[n][j], scale_value(sb[n]));
+        if (tile + NT < t1) fetch(tile + NT);
+        f32x4 acc[UT][NT];
+#pragma unroll
+        for (int t = 0; t < UT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < NBL; ++j)
 #pragma unroll
             for (int p = NP - 1; p >= 0; --p)  // small parts first
 #pragma unroll
                 for (int t = 0; t < UT; ++t)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, af[t][j][p], acc[t], 0, 0, 0);
-        }
 #pragma unroll
-        for (int t = 0; t < UT; ++t) o.put(row_base + 16 * t + q, 16 * tile + 4 * g, acc[t]);
+                    for (int n = 0; n < NT; ++n)
+                        acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[n][j], af[t][j][p],
+                                                                            acc[t][n], 0, 0, 0);
+#pragma unroll
+        for (int t = 0; t < UT; ++t)
+            put_row<TO, NT>(dst[t], 16 * tile + 4 * NT * g, o.n_items, acc[t]);
     }
+}
+
+// Sums the KW waves' tiles into wave 0's, in wave order; whether this wave holds the result.
+template <int MT, int NT, int KW>
+__device__ __forceinline__ bool join_waves(f32x4 (&acc)[MT][NT], int wave, int lane) {
+    if constexpr (KW > 1) {
+        __shared__ f32x4 part[KW - 1][MT * NT][64];
+        if (wave > 0) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) part[wave - 1][t * NT + n][lane] = acc[t][n];
+        }
+        __syncthreads();
+        if (wave > 0) return false;
+#pragma unroll
+        for (int w = 0; w < KW - 1; ++w)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[t][n] += part[w][t * NT + n][lane];
+    }
+    return true;
 }
 
 // Rows of any width: a wave forms MT x NT tiles (16 activation rows x 16 items each) in steps of
 // four blocks.  KW = 1: the four waves of a workgroup take neighbouring items; KW = 4: they share
 // one tile group and take a quarter of the steps each, joined in wave order through LDS, where
 // there are too few tiles to fill the chip.
-template <typename T, int MT, int NT, int KW>
+template <typename T, typename TO, int MT, int NT, int KW>
 __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T *__restrict__ a,
                                                               int width,
                                                               const uint8_t *__restrict__ codes,
@@ -372,7 +446,7 @@ __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T
     int64_t it[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int64_t i = item_base + 16 * n + q;
+        const int64_t i = item_base + item_of<NT>(n, q);
         it[n] = i < o.n_items ? i : o.n_items - 1;
     }
     f32x4 acc[MT][NT];
@@ -417,36 +491,101 @@ __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T
             }
         }
     }
-    if constexpr (KW > 1) {
-        __shared__ f32x4 part[KW - 1][MT * NT][64];
-        if (wave > 0) {
+    if (!join_waves<MT, NT, KW>(acc, wave, lane)) return;
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+    for (int t = 0; t < MT; ++t) {
+        if (no_row[t]) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) part[wave - 1][t * NT + n][lane] = acc[t][n];
+            for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{} + __builtin_nanf("");
         }
-        __syncthreads();
-        if (wave > 0) return;
-#pragma unroll
-        for (int w = 0; w < KW - 1; ++w)
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) acc[t][n] += part[w][t * NT + n][lane];
+        put_row<TO, NT>(out_row<TO>(o, row_base + 16 * t + q), item_base + 4 * NT * g, o.n_items, acc[t]);
     }
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            f32x4 v = acc[t][n];
-            if (no_row[t]) v = f32x4{} + __builtin_nanf("");
-            o.put(row_base + 16 * t + q, item_base + 16 * n + 4 * g, v);
-        }
 }
 
 // Both sides in 4 bits: v_mfma_scale_f32_16x16x128_f8f6f4 takes 32 codes per lane (one block) and
 // its scale byte, four blocks per instruction.
-template <int MT, int NT>
+__device__ __forceinline__ i32x8 as_operand(u32x4 w) {
+    return i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+}
+// Block `blk` of a row, or zeros with scale 1 behind the row's end.
+__device__ __forceinline__ void load_block(const uint8_t *__restrict__ c, const uint8_t *__restrict__ s,
+                                           int64_t row, int blk, int nb, u32x4 &w, int &e) {
+    typedef unsigned vec_t __attribute__((ext_vector_type(4), aligned(4)));
+    w = u32x4{0, 0, 0, 0};
+    e = 127;
+    if (blk < nb) {
+        w = *reinterpret_cast<const vec_t *>(c + (row * nb + blk) * 16);
+        e = s[row * nb + blk];
+    }
+}
+
+// Rows of at most 4 NS blocks: the activations stay in registers and the wave walks the items, as in
+// mx4_scores_narrow_kernel.
+template <typename TO, int NS, int UT, int NT>
+__global__ __launch_bounds__(256) void mx4_scores_both_narrow_kernel(
+    Rows rows, const uint8_t *__restrict__ acodes, const uint8_t *__restrict__ ascales,
+    const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int nb, ScoreStore o,
+    int groups, int tpw) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = lane >> 4, q = lane & 15;
+    const unsigned chunk = blockIdx.x / (unsigned)groups;
+    const int64_t row_base = (int64_t)(blockIdx.x - chunk * groups) * (16 * UT);
+    const int64_t n_tiles = (o.n_items + 15) / 16;
+    const int64_t t0 = ((int64_t)chunk * 4 + wave) * tpw;
+    const int64_t t1 = t0 + tpw < n_tiles ? t0 + tpw : n_tiles;
+    if (t0 >= t1) return;
+    u32x4 c[NT][NS];
+    int e[NT][NS];
+    auto fetch = [&](int64_t tile) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            int64_t item = 16 * tile + item_of<NT>(n, q);
+            item = item < o.n_items ? item : o.n_items - 1;
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+                load_block(codes, scales, item, 4 * s + g, nb, c[n][s], e[n][s]);
+        }
+    };
+    fetch(t0);
+    u32x4 aw[UT][NS];
+    int ae[UT][NS];
+    TO *dst[UT];
+#pragma unroll
+    for (int t = 0; t < UT; ++t) {
+        const int64_t i = row_base + 16 * t + q;
+        const int64_t r = rows.of(i < rows.n_sel ? i : rows.n_sel - 1);
+        dst[t] = out_row<TO>(o, i);
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            load_block(acodes, ascales, r < 0 ? 0 : r, 4 * s + g, nb, aw[t][s], ae[t][s]);
+            if (r < 0) ae[t][s] = 255;  // no such row: NaN
+        }
+    }
+    for (int64_t tile = t0; tile < t1; tile += NT) {
+        f32x4 acc[UT][NT];
+#pragma unroll
+        for (int t = 0; t < UT; ++t)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int t = 0; t < UT; ++t)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    acc[t][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                        as_operand(c[n][s]), as_operand(aw[t][s]), acc[t][n], 4, 4, 0, e[n][s], 0,
+                        ae[t][s]);
+        if (tile + NT < t1) fetch(tile + NT);
+#pragma unroll
+        for (int t = 0; t < UT; ++t)
+            put_row<TO, NT>(dst[t], 16 * tile + 4 * NT * g, o.n_items, acc[t]);
+    }
+}
+
+// Any width, straight from memory: the form for a few rows and for products too small to tile.  KW as
+// in mx4_scores_wide_kernel.
+template <typename TO, int MT, int NT, int KW>
 __global__ __launch_bounds__(256) void mx4_scores_both_kernel(Rows rows,
                                                               const uint8_t *__restrict__ acodes,
                                                               const uint8_t *__restrict__ ascales,
@@ -457,8 +596,8 @@ __global__ __launch_bounds__(256) void mx4_scores_both_kernel(Rows rows,
     const int g = lane >> 4, q = lane & 15;
     const unsigned chunk = blockIdx.x / (unsigned)groups;
     const int64_t row_base = (int64_t)(blockIdx.x - chunk * groups) * (16 * MT);
-    const int64_t item_base = ((int64_t)chunk * 4 + wave) * (16 * NT);
-    if (item_base >= o.n_items) return;
+    const int64_t item_base = (KW == 1 ? (int64_t)chunk * 4 + wave : (int64_t)chunk) * (16 * NT);
+    if (item_base >= o.n_items) return;  // (with KW > 1 no workgroup has only some such waves)
     int64_t ai[MT], it[NT];
     bool no_row[MT];
 #pragma unroll
@@ -467,50 +606,230 @@ __global__ __launch_bounds__(256) void mx4_scores_both_kernel(Rows rows,
         i = i < rows.n_sel ? i : rows.n_sel - 1;
         const int64_t r = rows.of(i);
         no_row[t] = r < 0;
-        ai[t] = (r < 0 ? 0 : r) * nb;
+        ai[t] = r < 0 ? 0 : r;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int64_t i = item_base + 16 * n + q;
-        it[n] = (i < o.n_items ? i : o.n_items - 1) * nb;
+        const int64_t i = item_base + item_of<NT>(n, q);
+        it[n] = i < o.n_items ? i : o.n_items - 1;
     }
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0, 0, 0, 0};
-    for (int blk = g; blk - g < nb; blk += 4) {
-        const bool in = blk < nb;
-        i32x8 af[MT], bf[NT];
+    const int steps = (nb + 3) / 4, per = (steps + KW - 1) / KW;
+    const int s0 = KW == 1 ? 0 : wave * per, s1 = s0 + per < steps ? s0 + per : steps;
+    for (int s = s0; s < s1; ++s) {
+        const int blk = 4 * s + g;
+        u32x4 af[MT], bf[NT];
         int as[MT], bs[NT];
-        auto fetch = [&](const uint8_t *c, const uint8_t *s, int64_t at, i32x8 &f, int &e) {
-            unsigned w[4] = {0, 0, 0, 0};
-            e = 127;
-            if (in) {
-                load_codes<4>(w, c + (at + blk) * 16);
-                e = s[at + blk];
-            }
-            f = i32x8{(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-        };
 #pragma unroll
-        for (int t = 0; t < MT; ++t) fetch(acodes, ascales, ai[t], af[t], as[t]);
+        for (int t = 0; t < MT; ++t) load_block(acodes, ascales, ai[t], blk, nb, af[t], as[t]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) fetch(codes, scales, it[n], bf[n], bs[n]);
+        for (int n = 0; n < NT; ++n) load_block(codes, scales, it[n], blk, nb, bf[n], bs[n]);
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
                 acc[t][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                    bf[n], af[t], acc[t][n], 4, 4, 0, bs[n], 0, as[t]);
+                    as_operand(bf[n]), as_operand(af[t]), acc[t][n], 4, 4, 0, bs[n], 0, as[t]);
     }
+    if (!join_waves<MT, NT, KW>(acc, wave, lane)) return;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        if (no_row[t]) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{} + __builtin_nanf("");
+        }
+        put_row<TO, NT>(out_row<TO>(o, row_base + 16 * t + q), item_base + 4 * NT * g, o.n_items, acc[t]);
+    }
+}
+
+// The same for large products, tiled through LDS: a workgroup of WM x WN waves forms BM rows x BN
+// items in steps of eight blocks (128 bytes a row), two steps a turn, each wave MT x NT tiles of
+// 16 x 16.
+//  - Codes go from memory straight into LDS (16 bytes per lane), into two buffers: the next step's are on
+//    their way during this step's products.  The chunks of a row lie permuted, so the 16 rows
+//    that a matrix operand reads at once spread over all banks.
+//  - Lane group g takes blocks 2g and 2g + 1 of a step (the contraction index may be dealt out in
+//    any way both sides share): one word brings their scales for both steps of the turn, and the
+//    instruction picks the byte.  Scales go through registers, 16 of a row at a time, one turn ahead.
+//  - A turn has no branch in it: otherwise the compiler moves products behind the next barrier and
+//    keeps all their operands.  The blocks of a row behind the last whole turn are read from memory.
+//  - An operand is needed every MT products; the reads are spread between them by hand.
+// Workgroups are dealt to the eight XCDs in contiguous ranges, so that neighbours in a cache
+// share their operands.
+template <typename TO, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
+    Rows rows, const uint8_t *__restrict__ acodes, const uint8_t *__restrict__ ascales,
+    const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int nb, ScoreStore o,
+    int row_tiles) {
+    constexpr int THREADS = 64 * WM * WN;
+    constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
+    static_assert(BM + BN == THREADS, "one row of scales per thread");
+    constexpr int LA = BM * 8 / THREADS, LB = BN * 8 / THREADS;  // 16-byte loads per thread and step
+    // rows of the activations, then of the items; two arrays and not one of two halves: only for
+    // different arrays does the compiler see that a read of one need not wait for the loads into
+    // the other
+    __shared__ u32x4 sc0[(BM + BN) * 8], sc1[(BM + BN) * 8];
+    __shared__ u32x4 ss[2][BM + BN];  // word g of a row: the scales for lane group g in a turn
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // (in a scalar register)
+    const int g = lane >> 4, q = lane & 15;
+    // contiguous ranges of tiles per XCD (workgroups are dealt out to them in turn)
+    const unsigned total = gridDim.x, xcd = blockIdx.x & 7u, nth = blockIdx.x >> 3;
+    const unsigned per = total >> 3, extra = total & 7u;
+    const unsigned tile = xcd * per + (xcd < extra ? xcd : extra) + nth;
+    const int64_t row_base = (int64_t)(tile % (unsigned)row_tiles) * BM;
+    const int64_t item_base = (int64_t)(tile / (unsigned)row_tiles) * BN;
+    auto a_row = [&](int i) {  // table row of the tile's row i (some row where there is none)
+        int64_t r = row_base + i;
+        r = rows.of(r < rows.n_sel ? r : rows.n_sel - 1);
+        return r < 0 ? 0 : r;
+    };
+    auto b_row = [&](int i) {
+        const int64_t r = item_base + i;
+        return r < o.n_items ? r : o.n_items - 1;
+    };
+    // slot s of a buffer: row s / 8, chunk (s % 8) ^ swizzle of the row; a thread's slots are THREADS
+    // apart, THREADS / 8 rows, which leaves the activations' swizzle as it is and turns the third
+    // bit of the items' over every time
+    auto a_swz = [](unsigned row) { return row >> 1 & 7u; };
+    auto b_swz = [](unsigned row) { return (row >> 1 & 1u) | (row / (4u * NT) & 3u) << 1; };
+    static_assert(THREADS / 8 == 8 * NT, "rows between a thread's slots");
+    const unsigned ca = (tid & 7) ^ a_swz(tid >> 3), cb = (tid & 7) ^ b_swz(tid >> 3);
+    unsigned src[LA + LB];  // first block of the row (the host makes sure that 32 bits do)
+#pragma unroll
+    for (int i = 0; i < LA + LB; ++i) {
+        const int row = (i < LA ? i : i - LA) * (THREADS / 8) + (tid >> 3);
+        src[i] = (unsigned)(i < LA ? a_row(row) : b_row(row)) * (unsigned)nb;
+    }
+    auto load_step = [&](unsigned step, u32x4 *to) __attribute__((always_inline)) {
+        // (one step is loaded past the last turn, and not used: any block of the row will do)
+        auto held = [&](unsigned k) { return k < (unsigned)nb ? k : (unsigned)nb - 1u; };
+        const unsigned ka = held(8u * step + ca), kb0 = held(8u * step + cb),
+                       kb1 = held(8u * step + (cb ^ 4u));
+#pragma unroll
+        for (int i = 0; i < LA + LB; ++i) {
+            const unsigned at = src[i] + (i < LA ? ka : (i - LA) & 1 ? kb1 : kb0);
+            const uint8_t *p = (i < LA ? acodes : codes) + ((uint64_t)at << 4);
+            // (the destination is the wave's: lane l writes the l-th 16 bytes behind it)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void *)p,
+                (__attribute__((address_space(3))) void *)&to[i * THREADS + wave * 64], 16, 0, 0);
+        }
+    };
+    const uint8_t *scale_row = tid < BM ? ascales + a_row(tid) * nb : scales + b_row(tid - BM) * nb;
+    typedef unsigned unaligned_t __attribute__((ext_vector_type(4), aligned(1)));
+    f32x4 acc[MT][NT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            f32x4 v = acc[t][n];
-            if (no_row[t]) v = f32x4{} + __builtin_nanf("");
-            o.put(row_base + 16 * t + q, item_base + 16 * n + 4 * g, v);
+        for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0, 0, 0, 0};
+    const int wm = wave % WM, wn = wave / WM;
+    // rows in the buffers
+    const int ar = wm * MT * 16 + q;
+    const int br = wn * NT * 16 + item_of<NT>(0, q);
+    const int sa = a_swz(ar), sb = b_swz(br);  // (the same for all of the wave's tiles)
+    // the products of one step; SECOND: of the second step of a turn
+    auto products = [&](auto second, const u32x4 *buf, const int (&as)[MT], const int (&bs)[NT])
+                        __attribute__((always_inline)) {
+        constexpr int S = 2 * decltype(second)::value;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            i32x8 af[MT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                af[t] = as_operand(buf[(ar + 16 * t) * 8 + ((2 * g + h) ^ sa)]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const i32x8 bf = as_operand(buf[(BM + br + 4 * n) * 8 + ((2 * g + h) ^ sb)]);
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    acc[t][n] = h == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                             bf, af[t], acc[t][n], 4, 4, S, bs[n], S, as[t])
+                                       : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                                             bf, af[t], acc[t][n], 4, 4, S + 1, bs[n], S + 1, as[t]);
+            }
         }
+    };
+    // order of the above: first the reads of the scales, the first half's activations and two
+    // items' codes; then one read of the item operand two turns ahead before every MT products, the
+    // second half's activations in the last two turns of the first
+    auto spread = [&](auto extra) __attribute__((always_inline)) {
+        constexpr int DS_READ = 0x100, MFMA = 0x8;
+        __builtin_amdgcn_sched_group_barrier(DS_READ, decltype(extra)::value + MT + 2, 0);
+#pragma unroll
+        for (int n = 0; n < 2 * NT; ++n) {
+            __builtin_amdgcn_sched_group_barrier(MFMA, MT, 0);
+            if (n == NT - 2 || n == NT - 1) __builtin_amdgcn_sched_group_barrier(DS_READ, MT / 2 + 1, 0);
+            else if (n < 2 * NT - 2) __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int turns = nb / 16;
+    if (turns > 0) {
+        u32x4 sr = *reinterpret_cast<const unaligned_t *>(scale_row);
+        load_step(0, sc0);
+        for (int turn = 0; turn < turns; ++turn) {
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(1): this wave's codes of this step are in LDS
+            // 16 scales, eight of either step -> word g: blocks 2g, 2g + 1 of the first, then the second
+            u32x4 word;
+            word[0] = __builtin_amdgcn_perm(sr[2], sr[0], 0x05040100u);
+            word[1] = __builtin_amdgcn_perm(sr[2], sr[0], 0x07060302u);
+            word[2] = __builtin_amdgcn_perm(sr[3], sr[1], 0x05040100u);
+            word[3] = __builtin_amdgcn_perm(sr[3], sr[1], 0x07060302u);
+            ss[turn & 1][tid] = word;
+            __syncthreads();  // everyone's are, and the other buffer is free
+            load_step(2 * turn + 1, sc1);
+            sr = *reinterpret_cast<const unaligned_t *>(scale_row + (turn + 1 < turns ? 16 * turn + 16 : 0));
+            __builtin_amdgcn_sched_barrier(0);
+            const int *sw = reinterpret_cast<const int *>(ss[turn & 1]) + g;
+            int as[MT], bs[NT];
+#pragma unroll
+            for (int t = 0; t < MT; ++t) as[t] = sw[(ar + 16 * t) * 4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) bs[n] = sw[(BM + br + 4 * n) * 4];
+            products(std::integral_constant<int, 0>{}, sc0, as, bs);
+            spread(std::integral_constant<int, MT + NT>{});
+            __builtin_amdgcn_s_waitcnt(0x0f70);
+            __syncthreads();
+            load_step(2 * turn + 2, sc0);
+            __builtin_amdgcn_sched_barrier(0);
+            products(std::integral_constant<int, 1>{}, sc1, as, bs);
+            spread(std::integral_constant<int, 0>{});
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // (the step loaded for nothing)
+    }
+#pragma unroll 1
+    for (int blk = 16 * turns + g; blk - g < nb; blk += 4) {
+        u32x4 af[MT], bf;
+        int as[MT], bs;
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            load_block(acodes, ascales, a_row(ar + 16 * t), blk, nb, af[t], as[t]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            load_block(codes, scales, b_row(br + 4 * n), blk, nb, bf, bs);
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[t][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                    as_operand(bf), as_operand(af[t]), acc[t][n], 4, 4, 0, bs, 0, as[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int64_t row = row_base + ar + 16 * t;
+        TO *dst = out_row<TO>(o, row);
+        if (!dst) continue;
+        if (rows.of(row) < 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{} + __builtin_nanf("");
+        }
+        put_row<TO, NT>(dst, item_base + wn * NT * 16 + g * 4 * NT, o.n_items, acc[t]);
+    }
 }
 
 // ---- launches ------------------------------------------------------------------------------------
@@ -526,69 +845,129 @@ static RowGrid row_grid(int64_t n_rows, int nb) {
     return r;
 }
 
-template <typename T, int NBL, int UT>
+template <typename T, typename TO, int NBL, int UT, int NT>
 static int launch_narrow(const Rows &rows, const void *a, int width, const uint8_t *codes,
                          const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
     const int64_t groups = (rows.n_sel + 16 * UT - 1) / (16 * UT);
     const int64_t n_tiles = (o.n_items + 15) / 16;
-    // long walks once there is enough work for 8192 waves
-    int64_t tpw = n_tiles * groups / 8192;
-    tpw = tpw < 1 ? 1 : (tpw > 32 ? 32 : tpw);
+    // one turn per wave until there are TARGET waves (what the registers let run at once), then
+    // longer walks
+    constexpr int TARGET = UT == 1 ? 4096 : 2048;
+    int64_t turns = n_tiles * groups / (TARGET * NT);
+    turns = turns < 1 ? 1 : (turns > 16 ? 16 : turns);
+    const int64_t tpw = turns * NT;
     const int64_t blocks = (n_tiles + 4 * tpw - 1) / (4 * tpw) * groups;
     ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
-    hipLaunchKernelGGL((mx4_scores_narrow_kernel<T, NBL, UT>), dim3((unsigned)blocks), dim3(256), 0, st,
-                       rows, static_cast<const T *>(a), width, codes, scales, nb, o, (int)groups,
+    hipLaunchKernelGGL((mx4_scores_narrow_kernel<T, TO, NBL, UT, NT>), dim3((unsigned)blocks), dim3(256), 0,
+                       st, rows, static_cast<const T *>(a), width, codes, scales, nb, o, (int)groups,
                        (int)tpw);
     ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
 }
 
-template <typename T, int MT, int NT, int KW>
+template <typename T, typename TO, int MT, int NT, int KW>
 static int launch_wide(const Rows &rows, const void *a, int width, const uint8_t *codes,
                        const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
     const int64_t groups = (rows.n_sel + 16 * MT - 1) / (16 * MT);
     const int64_t per = 16 * NT * (KW == 1 ? 4 : 1);
     const int64_t blocks = (o.n_items + per - 1) / per * groups;
     ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
-    hipLaunchKernelGGL((mx4_scores_wide_kernel<T, MT, NT, KW>), dim3((unsigned)blocks), dim3(256), 0,
+    hipLaunchKernelGGL((mx4_scores_wide_kernel<T, TO, MT, NT, KW>), dim3((unsigned)blocks), dim3(256), 0,
                        st, rows, static_cast<const T *>(a), width, codes, scales, nb, o, (int)groups);
     ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
 }
 
-template <int MT, int NT>
+template <typename TO, int NS, int UT, int NT>
+static int launch_both_narrow(const Rows &rows, const void *a, const uint8_t *a_scales,
+                              const uint8_t *codes, const uint8_t *scales, int nb, const ScoreStore &o,
+                              hipStream_t st) {
+    const int64_t groups = (rows.n_sel + 16 * UT - 1) / (16 * UT);
+    const int64_t n_tiles = (o.n_items + 15) / 16;
+    int64_t turns = n_tiles * groups / (4096 * NT);  // as in launch_narrow
+    turns = turns < 1 ? 1 : (turns > 16 ? 16 : turns);
+    const int64_t tpw = turns * NT;
+    const int64_t blocks = (n_tiles + 4 * tpw - 1) / (4 * tpw) * groups;
+    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
+    hipLaunchKernelGGL((mx4_scores_both_narrow_kernel<TO, NS, UT, NT>), dim3((unsigned)blocks), dim3(256),
+                       0, st, rows, static_cast<const uint8_t *>(a), a_scales, codes, scales, nb, o,
+                       (int)groups, (int)tpw);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
+template <typename TO, int MT, int NT, int KW>
 static int launch_both(const Rows &rows, const void *a, const uint8_t *a_scales, const uint8_t *codes,
                        const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
     const int64_t groups = (rows.n_sel + 16 * MT - 1) / (16 * MT);
-    const int64_t per = 64 * NT;
+    const int64_t per = 16 * NT * (KW == 1 ? 4 : 1);
     const int64_t blocks = (o.n_items + per - 1) / per * groups;
     ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
-    hipLaunchKernelGGL((mx4_scores_both_kernel<MT, NT>), dim3((unsigned)blocks), dim3(256), 0, st, rows,
+    hipLaunchKernelGGL((mx4_scores_both_kernel<TO, MT, NT, KW>), dim3((unsigned)blocks), dim3(256), 0, st, rows,
                        static_cast<const uint8_t *>(a), a_scales, codes, scales, nb, o, (int)groups);
     ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
 }
 
-template <typename T>
+template <typename TO, int WM, int WN, int MT, int NT>
+static int launch_tiled(const Rows &rows, const void *a, const uint8_t *a_scales, const uint8_t *codes,
+                        const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
+    constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
+    const int64_t row_tiles = (rows.n_sel + BM - 1) / BM;
+    const int64_t blocks = (o.n_items + BN - 1) / BN * row_tiles;
+    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
+    hipLaunchKernelGGL((mx4_scores_tiled_kernel<TO, WM, WN, MT, NT>), dim3((unsigned)blocks),
+                       dim3(64 * WM * WN), 0, st, rows, static_cast<const uint8_t *>(a), a_scales, codes,
+                       scales, nb, o, (int)row_tiles);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
+template <typename TO>
+static int run_both(const Rows &rows, const void *a, const uint8_t *a_scales, const uint8_t *codes,
+                    const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
+    const bool one = rows.n_sel <= 16;
+    if (nb <= 4)
+        return one ? launch_both_narrow<TO, 1, 1, 2>(rows, a, a_scales, codes, scales, nb, o, st)
+                   : launch_both_narrow<TO, 1, 4, 2>(rows, a, a_scales, codes, scales, nb, o, st);
+    if (nb <= 8)
+        return one ? launch_both_narrow<TO, 2, 1, 2>(rows, a, a_scales, codes, scales, nb, o, st)
+                   : launch_both_narrow<TO, 2, 4, 2>(rows, a, a_scales, codes, scales, nb, o, st);
+    const int64_t tiles = (rows.n_sel + 15) / 16 * ((o.n_items + 15) / 16);
+    if (one)
+        return tiles < 32768 ? launch_both<TO, 1, 2, 4>(rows, a, a_scales, codes, scales, nb, o, st)
+                             : launch_both<TO, 1, 4, 1>(rows, a, a_scales, codes, scales, nb, o, st);
+    // (the tiled form counts blocks in 32 bits and loads 16 bytes at a time)
+    const bool aligned = (uintptr_t)a % 16 == 0 && (uintptr_t)codes % 16 == 0 &&
+                         rows.n_rows * nb < (int64_t)1 << 32 && o.n_items * nb < (int64_t)1 << 32;
+    const int64_t t256 = (rows.n_sel + 255) / 256 * ((o.n_items + 255) / 256);
+    if (aligned && nb >= 16 && t256 >= 192)
+        return launch_tiled<TO, 4, 2, 4, 8>(rows, a, a_scales, codes, scales, nb, o, st);
+    if (aligned && nb >= 16 && rows.n_sel > 64)
+        return launch_tiled<TO, 2, 2, 4, 4>(rows, a, a_scales, codes, scales, nb, o, st);
+    return launch_both<TO, 4, 4, 1>(rows, a, a_scales, codes, scales, nb, o, st);
+}
+
+template <typename T, typename TO>
 static int run_scores(const Rows &rows, const void *a, int width, const uint8_t *codes,
                       const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
     const bool one = rows.n_sel <= 16;
     if (nb == 1)
-        return one ? launch_narrow<T, 1, 1>(rows, a, width, codes, scales, nb, o, st)
-                   : launch_narrow<T, 1, 4>(rows, a, width, codes, scales, nb, o, st);
+        return one ? launch_narrow<T, TO, 1, 1, 2>(rows, a, width, codes, scales, nb, o, st)
+                   : launch_narrow<T, TO, 1, 4, 2>(rows, a, width, codes, scales, nb, o, st);
     if (nb == 2)
-        return one ? launch_narrow<T, 2, 1>(rows, a, width, codes, scales, nb, o, st)
-                   : launch_narrow<T, 2, 4>(rows, a, width, codes, scales, nb, o, st);
+        return one ? launch_narrow<T, TO, 2, 1, 2>(rows, a, width, codes, scales, nb, o, st)
+                   : launch_narrow<T, TO, 2, 4, 2>(rows, a, width, codes, scales, nb, o, st);
     // (three parts of four tiles at four blocks would need 192 registers)
     if (nb <= 4)
-        return one ? launch_narrow<T, 4, 1>(rows, a, width, codes, scales, nb, o, st)
-                   : launch_narrow<T, 4, 2>(rows, a, width, codes, scales, nb, o, st);
+        return one ? launch_narrow<T, TO, 4, 1, 2>(rows, a, width, codes, scales, nb, o, st)
+                   : launch_narrow<T, TO, 4, 2, 2>(rows, a, width, codes, scales, nb, o, st);
     const int64_t tiles = (rows.n_sel + 15) / 16 * ((o.n_items + 15) / 16);
     if (one)
-        return tiles < 32768 ? launch_wide<T, 1, 2, 4>(rows, a, width, codes, scales, nb, o, st)
-                             : launch_wide<T, 1, 4, 1>(rows, a, width, codes, scales, nb, o, st);
-    return tiles < 16384 ? launch_wide<T, 2, 2, 4>(rows, a, width, codes, scales, nb, o, st)
-                         : launch_wide<T, 4, 4, 1>(rows, a, width, codes, scales, nb, o, st);
+        return tiles < 32768 ? launch_wide<T, TO, 1, 2, 4>(rows, a, width, codes, scales, nb, o, st)
+                             : launch_wide<T, TO, 1, 4, 1>(rows, a, width, codes, scales, nb, o, st);
+    return tiles < 16384 ? launch_wide<T, TO, 2, 2, 4>(rows, a, width, codes, scales, nb, o, st)
+                         : launch_wide<T, TO, 4, 4, 1>(rows, a, width, codes, scales, nb, o, st);
 }
 
 }  // namespace alsmi
@@ -685,12 +1064,21 @@ int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_ro
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
     const Rows r = {n_sel, n_rows, lda, rows};
-    const ScoreStore o = {out, ldo, n_sel, n_items, out_dtype};
-    if (dtype == ALSMI_F32) return run_scores<float>(r, a, (int)width, codes, scales, nb, o, st);
-    if (dtype == ALSMI_F16) return run_scores<_Float16>(r, a, (int)width, codes, scales, nb, o, st);
-    if (dtype == ALSMI_BF16) return run_scores<__bf16>(r, a, (int)width, codes, scales, nb, o, st);
-    return n_sel <= 16 ? launch_both<1, 4>(r, a, a_scales, codes, scales, nb, o, st)
-                       : launch_both<4, 4>(r, a, a_scales, codes, scales, nb, o, st);
+    const ScoreStore o = {out, ldo, n_sel, n_items};
+#define ALSMI_CASE(TO)                                                                               \
+    do {                                                                                             \
+        if (dtype == ALSMI_F32)                                                                      \
+            return run_scores<float, TO>(r, a, (int)width, codes, scales, nb, o, st);                \
+        if (dtype == ALSMI_F16)                                                                      \
+            return run_scores<_Float16, TO>(r, a, (int)width, codes, scales, nb, o, st);             \
+        if (dtype == ALSMI_BF16)                                                                     \
+            return run_scores<__bf16, TO>(r, a, (int)width, codes, scales, nb, o, st);               \
+        return run_both<TO>(r, a, a_scales, codes, scales, nb, o, st);                              \
+    } while (0)
+    if (out_dtype == ALSMI_F32) ALSMI_CASE(float);
+    else if (out_dtype == ALSMI_BF16) ALSMI_CASE(__bf16);
+    else ALSMI_CASE(_Float16);
+#undef ALSMI_CASE
 }
 
 }  // extern "C"
