@@ -1,46 +1,86 @@
 // The k largest scores of every row of a score block, best first, ties to the lowest index.
 //
 // Scores are ranked through the order-preserving integer image of their bits joined with the
-// complement of their index: (image << 32) | ~index.  These keys are all different, so "the k-th
+// complement of their index: (image << 32) | ~index, 48, 64 or 96 bits.  These keys are all different, so "the k-th
 // largest" is one element however many scores are equal (rows that a mask left mostly at -inf, 16-bit
-// scores), and comparing keys is the whole tie rule.
-// A row is cut into tiles of 4096; a workgroup holds its tile's keys in registers, finds the tile's
-// k-th largest key by a radix descent over LDS histograms and keeps the k keys at or above it.  The
-// kept keys of all tiles are the next, k / 4096 times shorter, row; the last level sorts.
+// scores), comparing keys is the whole tie rule, and any set of candidates can be merged in any
+// order.  0 is below every key.
+//
+// k <= 64: a wave keeps its k best, sorted, one per lane, and streams over its part of the row: a key at
+//   or below the k-th best is dropped by one comparison, the few others wait in LDS until 64 of them
+//   are sorted and merged into the list at once.  Four waves per workgroup, as many workgroups per row
+//   as fill the chip; a second launch merges their lists.
+// k > 64: a workgroup holds a tile of 8192 keys in registers, finds the tile's k-th largest by a radix
+//   descent over LDS histograms (2048 bins a digit) and keeps the k keys at or above it; the kept
+//   keys of all tiles are the next, 8192 / k times shorter, row.  The last level takes up to 16384 keys
+//   in one workgroup and sorts.
 #include "alsmi_common.h"
 #include "elem.h"
 
+#include <type_traits>
+
 namespace alsmi {
 
-constexpr int TR_THREADS = 256;
-constexpr int TR_E = 16;                       // keys per thread
-constexpr int TR_TILE = TR_THREADS * TR_E;     // 4096
 constexpr int TR_MAX_K = 1024;
+constexpr int TR_LIST = 64;         // the longest list one wave keeps
+constexpr int TR_CHUNK = 1024;      // keys a wave looks at per turn, 16 per lane
+constexpr int TR_PART = 4 * TR_CHUNK;
+constexpr int TR_THREADS = 512;     // k > 64: threads and keys per workgroup
+constexpr int TR_TILE = 8192;
+constexpr int TR_LAST = 16384;      // and of the last level's 1024 threads
 
 typedef unsigned __int128 u128;
 
 template <typename T>
-struct RowKey {  // 16- and 32-bit scores through their fp32 image
+struct RowKey {  // fp32: 32 bits of image, 32 of index
     typedef unsigned long long type;
+    typedef unsigned image_t;
     static constexpr int BITS = 64;
-    static __device__ __forceinline__ type make(T s, unsigned index) {
-        const unsigned b = __builtin_bit_cast(unsigned, (float)s);
-        const unsigned image = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-        return ((type)image << 32) | (unsigned)~index;
+    static __device__ __forceinline__ image_t image(T s) {
+        const unsigned b = __builtin_bit_cast(unsigned, s);
+        return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
     }
     static __device__ __forceinline__ T score(type k) {
         const unsigned i = (unsigned)(k >> 32);
-        return (T)__builtin_bit_cast(float, (i & 0x80000000u) ? (i & 0x7fffffffu) : ~i);
+        return __builtin_bit_cast(T, (i & 0x80000000u) ? (i & 0x7fffffffu) : ~i);
     }
+};
+struct RowKey16 {  // fp16, bf16: 16 bits of image
+    typedef unsigned long long type;
+    typedef unsigned image_t;
+    static constexpr int BITS = 48;
+    static __device__ __forceinline__ image_t image(unsigned short b) {
+        return (b ^ ((unsigned)((int)(short)b >> 31) | 0x8000u)) & 0xffffu;
+    }
+    static __device__ __forceinline__ unsigned short bits(type k) {
+        const unsigned i = (unsigned)(k >> 32);
+        return (unsigned short)((i & 0x8000u) ? (i & 0x7fffu) : ~i);
+    }
+};
+template <>
+struct RowKey<_Float16> : RowKey16 {
+    static __device__ __forceinline__ image_t image(_Float16 s) {
+        return RowKey16::image(__builtin_bit_cast(unsigned short, s));
+    }
+    static __device__ __forceinline__ _Float16 score(type k) {
+        return __builtin_bit_cast(_Float16, bits(k));
+    }
+};
+template <>
+struct RowKey<__bf16> : RowKey16 {
+    static __device__ __forceinline__ image_t image(__bf16 s) {
+        return RowKey16::image(__builtin_bit_cast(unsigned short, s));
+    }
+    static __device__ __forceinline__ __bf16 score(type k) { return __builtin_bit_cast(__bf16, bits(k)); }
 };
 template <>
 struct RowKey<double> {
     typedef u128 type;
+    typedef unsigned long long image_t;
     static constexpr int BITS = 96;
-    static __device__ __forceinline__ type make(double s, unsigned index) {
+    static __device__ __forceinline__ image_t image(double s) {
         const unsigned long long b = __builtin_bit_cast(unsigned long long, s);
-        const unsigned long long image = (b >> 63) ? ~b : (b | 0x8000000000000000ull);
-        return ((type)image << 32) | (unsigned)~index;
+        return b ^ ((unsigned long long)((long long)b >> 63) | 0x8000000000000000ull);
     }
     static __device__ __forceinline__ double score(type k) {
         const unsigned long long i = (unsigned long long)(k >> 32);
@@ -48,158 +88,479 @@ struct RowKey<double> {
     }
 };
 
-// One tile: keys of `n` elements (scores, or keys left by the level before) starting at `first`.
-// SORT: the only tile of its row; its k best are sorted and written out.
-template <typename T, bool FROM_KEYS, bool SORT>
-__global__ __launch_bounds__(TR_THREADS) void topk_rows_kernel(
-    const T *__restrict__ scores, int64_t lds, const typename RowKey<T>::type *__restrict__ in,
-    int64_t n, int k, unsigned tiles, typename RowKey<T>::type *__restrict__ kept,
-    int32_t *__restrict__ items_out, T *__restrict__ scores_out) {
+// Where a launch reads: a row of scores, or the keys that the level before kept of it.
+template <typename T, bool FROM_KEYS>
+struct KeySource {
     typedef typename RowKey<T>::type key_t;
-    __shared__ unsigned hist[256];
+    typedef typename std::conditional<FROM_KEYS, key_t, T>::type raw_t;
+    const raw_t *data;
+    int64_t ld;  // row stride
+    int64_t n;
+    // N elements of a row from `at` on; those at and behind `end` are not read
+    template <int N>
+    static __device__ __forceinline__ void load(raw_t (&v)[N], const raw_t *row, int64_t at, int64_t end) {
+        if constexpr (sizeof(raw_t) == 16) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = at + i < end ? row[at + i] : (raw_t)0;
+        } else {
+            typedef raw_t vec_t __attribute__((ext_vector_type(N), aligned(sizeof(raw_t))));
+            if (at + N <= end) {
+                const vec_t w = *reinterpret_cast<const vec_t *>(row + at);
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = w[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[i] = at + i < end ? row[at + i] : (raw_t)0;
+            }
+        }
+    }
+    typedef typename RowKey<T>::image_t image_t;
+    static __device__ __forceinline__ image_t image(raw_t v) {
+        if constexpr (FROM_KEYS) return (image_t)(v >> 32);
+        else return RowKey<T>::image(v);
+    }
+    // the key of element `at`; 0 at and behind `end`
+    static __device__ __forceinline__ key_t key(raw_t v, int64_t at, int64_t end) {
+        if constexpr (FROM_KEYS) return v;
+        else return at < end ? ((key_t)RowKey<T>::image(v) << 32) | (unsigned)~(unsigned)at : (key_t)0;
+    }
+};
+
+// The value of lane (lane ^ MASK).  All masks the sorts use are vector instructions (a shuffle through
+// LDS takes some ten times as long): permutations of 4 lanes, mirrors of 8 and 16, a rotation of 16
+// by 8, and the swaps of rows of 16 and halves of 32.
+template <int MASK>
+__device__ __forceinline__ unsigned lane_xor(unsigned x, int lane) {
+    auto dpp = [](unsigned v, auto ctrl) {
+        return (unsigned)__builtin_amdgcn_mov_dpp((int)v, decltype(ctrl)::value, 0xf, 0xf, true);
+    };
+    if constexpr (MASK == 1) return dpp(x, std::integral_constant<int, 0xb1>{});
+    else if constexpr (MASK == 2) return dpp(x, std::integral_constant<int, 0x4e>{});
+    else if constexpr (MASK == 3) return dpp(x, std::integral_constant<int, 0x1b>{});
+    else if constexpr (MASK == 7) return dpp(x, std::integral_constant<int, 0x141>{});
+    else if constexpr (MASK == 15) return dpp(x, std::integral_constant<int, 0x140>{});
+    else if constexpr (MASK == 8) return dpp(x, std::integral_constant<int, 0x128>{});
+    else if constexpr (MASK == 4) return lane_xor<3>(lane_xor<7>(x, lane), lane);
+    else if constexpr (MASK == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return (lane & 16) ? r[0] : r[1];
+    } else if constexpr (MASK == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return (lane & 32) ? r[0] : r[1];
+    } else {
+        static_assert(MASK == 31 || MASK == 63, "mask of no sort");
+        return lane_xor<MASK == 63 ? 31 : 15>(lane_xor<MASK == 63 ? 32 : 16>(x, lane), lane);
+    }
+}
+template <int MASK>
+__device__ __forceinline__ unsigned long long key_xor(unsigned long long k, int lane) {
+    return ((unsigned long long)lane_xor<MASK>((unsigned)(k >> 32), lane) << 32) |
+           lane_xor<MASK>((unsigned)k, lane);
+}
+template <int MASK>
+__device__ __forceinline__ u128 key_xor(u128 k, int lane) {  // (96 bits)
+    return ((u128)lane_xor<MASK>((unsigned)(k >> 64), lane) << 64) |
+           key_xor<MASK>((unsigned long long)k, lane);
+}
+__device__ __forceinline__ unsigned long long lane_key(unsigned long long k, int lane) {
+    return ((unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32) |
+           (unsigned)__builtin_amdgcn_readlane((int)k, lane);
+}
+__device__ __forceinline__ u128 lane_key(u128 k, int lane) {
+    return ((u128)lane_key((unsigned long long)(k >> 64), lane) << 64) |
+           lane_key((unsigned long long)k, lane);
+}
+
+// One step of a sort, largest first: of lanes l and l ^ MASK the one without MASK's top bit keeps the
+// larger key.
+template <int MASK, typename K>
+__device__ __forceinline__ K sort_step(K k, int lane) {
+    constexpr int TOP = MASK >= 32 ? 32 : MASK >= 16 ? 16 : MASK >= 8 ? 8 : MASK >= 4 ? 4 : MASK >= 2 ? 2 : 1;
+    const K o = key_xor<MASK>(k, lane);
+    return (o > k) != ((lane & TOP) != 0) ? o : k;
+}
+// A bitonic sequence of the 64 lanes put in order; all of them sorted.  (A sorted run meets the mirror
+// image of the next one, so every run is sorted the same way.)
+template <typename K>
+__device__ __forceinline__ K wave_merge(K k, int lane) {
+    k = sort_step<32>(k, lane);
+    k = sort_step<16>(k, lane);
+    k = sort_step<8>(k, lane);
+    k = sort_step<4>(k, lane);
+    k = sort_step<2>(k, lane);
+    return sort_step<1>(k, lane);
+}
+template <typename K>
+__device__ __forceinline__ K wave_sort(K k, int lane) {
+    k = sort_step<1>(k, lane);
+    k = sort_step<3>(k, lane);
+    k = sort_step<1>(k, lane);
+    k = sort_step<7>(k, lane);
+    k = sort_step<2>(k, lane);
+    k = sort_step<1>(k, lane);
+    k = sort_step<15>(k, lane);
+    k = sort_step<4>(k, lane);
+    k = sort_step<2>(k, lane);
+    k = sort_step<1>(k, lane);
+    k = sort_step<31>(k, lane);
+    k = sort_step<8>(k, lane);
+    k = sort_step<4>(k, lane);
+    k = sort_step<2>(k, lane);
+    k = sort_step<1>(k, lane);
+    k = sort_step<63>(k, lane);
+    k = sort_step<16>(k, lane);
+    k = sort_step<8>(k, lane);
+    k = sort_step<4>(k, lane);
+    k = sort_step<2>(k, lane);
+    return sort_step<1>(k, lane);
+}
+// the best 64 of two sorted lists, sorted
+template <typename K>
+__device__ __forceinline__ K wave_join(K list, K other, int lane) {
+    const K back = key_xor<63>(other, lane);
+    return wave_merge(back > list ? back : list, lane);
+}
+
+template <typename T, bool FROM_KEYS>
+__global__ __launch_bounds__(256) void topk_list_kernel(KeySource<T, FROM_KEYS> src, int k,
+                                                        unsigned parts, int64_t part_len,
+                                                        typename RowKey<T>::type *__restrict__ kept,
+                                                        int32_t *__restrict__ items_out,
+                                                        T *__restrict__ scores_out) {
+    typedef typename RowKey<T>::type key_t;
+    // elements per load (16 bytes), loads per chunk
+    constexpr int VEC = FROM_KEYS ? 16 / (int)sizeof(key_t) : 16 / (int)sizeof(T);
+    constexpr int LOADS = 16 / VEC;
+    __shared__ key_t waiting_sh[4][TR_LIST + TR_CHUNK];
+    __shared__ key_t bounds[4][TR_LIST], lists[4][TR_LIST];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned r32 = blockIdx.x / parts;
+    const int64_t row = r32;
+    const unsigned part = blockIdx.x - r32 * parts;
+    const int64_t first = (int64_t)part * part_len;
+    const int64_t end = first + part_len < src.n ? first + part_len : src.n;
+    volatile key_t *waiting = waiting_sh[wave];  // (one wave's reads and writes of LDS keep their order)
+    key_t list = 0;      // the wave's best so far, best in lane 0
+    key_t floor_key = 0; // keys at or below it are out
+    int n_waiting = 0;
+    auto flush = [&]() {
+        const int m = n_waiting < TR_LIST ? n_waiting : TR_LIST;
+        n_waiting -= m;
+        key_t v = 0;
+        if (lane < m) v = waiting[n_waiting + lane];
+        list = wave_join(list, wave_sort(v, lane), lane);
+        const key_t kth = lane_key(list, k - 1);
+        floor_key = kth > floor_key ? kth : floor_key;
+    };
+    typedef KeySource<T, FROM_KEYS> source;
+    const typename source::raw_t *data = src.data + row * src.ld;
+    typename source::raw_t raw[LOADS][VEC];
+    auto fetch = [&](int64_t at) {
+        if (at + TR_CHUNK <= end) {  // (the whole wave alike: plain loads, all in flight together)
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j)
+                source::load(raw[j], data + at + (j * 64 + lane) * VEC, 0, VEC);
+        } else {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) source::load(raw[j], data, at + (j * 64 + lane) * VEC, end);
+        }
+    };
+    const int64_t start = first + wave * TR_CHUNK;
+    fetch(start);
+    {
+        // a first bound: the k-th largest of the 256 lanes' largest of the waves' first chunks
+        key_t top = 0;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const key_t x = source::key(raw[j][i], start + (j * 64 + lane) * VEC + i, end);
+                top = x > top ? x : top;
+            }
+        top = wave_sort(top, lane);
+        bounds[wave][lane] = top;
+        __syncthreads();
+#pragma unroll 1
+        for (int w = 1; w < 4; ++w) top = wave_join(top, (key_t)bounds[(wave + w) & 3][lane], lane);
+        const key_t kth = lane_key(top, k - 1);
+        floor_key = kth ? kth - 1 : 0;
+    }
+    for (int64_t at = start; at < end; at += 4 * TR_CHUNK) {
+        typename source::raw_t now[LOADS][VEC];
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) now[j][i] = raw[j][i];
+        fetch(at + 4 * TR_CHUNK);  // (on its way while this chunk is looked at)
+        auto key_at = [&](int j, int i) {
+            return source::key(now[j][i], at + (j * 64 + lane) * VEC + i, end);
+        };
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            // most loads hold nothing: one look at the largest score of a lane, whole keys only then
+            // (elements behind the end count as whatever they are read as, and are no hits)
+            typename source::image_t top = source::image(now[j][0]);
+#pragma unroll
+            for (int i = 1; i < VEC; ++i) {
+                const typename source::image_t x = source::image(now[j][i]);
+                top = x > top ? x : top;
+            }
+            if (__ballot(top >= (typename source::image_t)(floor_key >> 32)) == 0) continue;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const key_t x = key_at(j, i);
+                const bool hit = x > floor_key;
+                const unsigned long long m = __ballot(hit);
+                if (m == 0) continue;
+                if (hit) waiting[n_waiting + __popcll(m & ((1ull << lane) - 1ull))] = x;
+                n_waiting += __popcll(m);
+            }
+        }
+        // (in one place: unrolled into every load this was 60 KB of code, and fetching it the
+        // largest part of a small launch)
+        const bool last = at + 4 * TR_CHUNK >= end;
+        while (n_waiting >= TR_LIST || (last && n_waiting > 0)) flush();
+    }
+    lists[wave][lane] = list;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll 1
+    for (int w = 1; w < 4; ++w) list = wave_join(list, (key_t)lists[w][lane], lane);
+    if (lane >= k) return;
+    if (parts > 1) {
+        kept[(row * parts + part) * k + lane] = list;
+    } else {
+        items_out[row * k + lane] = (int32_t)~(unsigned)list;
+        scores_out[row * k + lane] = RowKey<T>::score(list);
+    }
+}
+
+// ---- k > 64 --------------------------------------------------------------------------------------
+// The smallest of the k largest keys of a workgroup (THREADS x E keys in registers, all different but
+// for zeros), by digits of at most 11 bits from the top, image first, then the `index_bits` bits
+// in which indices differ (the bits between are ones in every key); 1 if there are no k keys but
+// zeros.
+template <typename K, int BITS, int THREADS, int E>
+__device__ __forceinline__ K kth_key(const K (&key)[E], int k, int index_bits) {
+    constexpr int DIGIT = 11, BINS = 1 << DIGIT, PER = BINS / THREADS, WAVES = THREADS / 64;
+    __shared__ unsigned hist[BINS];
+    __shared__ unsigned wave_sum[WAVES];
+    __shared__ unsigned bin_sh, above_sh, in_bin_sh;
+    const int tid = threadIdx.x, lane = tid & 63;
+    K prefix = 0;
+    unsigned want = k;
+    for (int high = BITS, low; high > 0; high = low == 32 ? index_bits : low) {
+        // bits [low, high) of the key
+        low = high - DIGIT > 32 ? high - DIGIT : high > 32 ? 32 : high > DIGIT ? high - DIGIT : 0;
+        if (high == index_bits) prefix |= (K)(0xffffffffull >> index_bits << index_bits);
+        const unsigned mask = (1u << (high - low)) - 1u;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) hist[i * THREADS + tid] = 0;
+        __syncthreads();
+        if (tid == 0) bin_sh = BINS;  // no bin yet
+        const K upper = high >= BITS ? (K)0 : ~(K)0 << high;  // (a key of zeros fits no image)
+        // scores share their leading bits: a thread adds up a run of equal digits first
+        int run_bin = -1;
+        unsigned run = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            if ((key[j] & upper) != prefix) continue;
+            const int b = (int)((unsigned)(key[j] >> low) & mask);
+            if (b != run_bin) {
+                if (run) atomicAdd(&hist[run_bin], run);
+                run_bin = b;
+                run = 0;
+            }
+            ++run;
+        }
+        if (run) atomicAdd(&hist[run_bin], run);
+        __syncthreads();
+        // thread t: bins BINS-1 - PER t downwards; keys above them = the sums of the threads before
+        unsigned h[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sum += h[i] = hist[BINS - 1 - PER * tid - i];
+        unsigned upto = sum;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const unsigned o = __shfl_up(upto, off);
+            if (lane >= off) upto += o;
+        }
+        if (lane == 63) wave_sum[tid >> 6] = upto;
+        __syncthreads();
+        unsigned above = upto - sum;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+            if (w < (tid >> 6)) above += wave_sum[w];
+        if (above < want && above + sum >= want) {
+            int i = 0;
+#pragma unroll
+            for (int s = 0; s < PER - 1; ++s)
+                if (i == s && above + h[s] < want) above += h[s], i = s + 1;
+            bin_sh = BINS - 1 - PER * tid - i;
+            above_sh = above;
+            in_bin_sh = h[0];
+#pragma unroll
+            for (int s = 1; s < PER; ++s)
+                if (i == s) in_bin_sh = h[s];
+        }
+        __syncthreads();
+        if (bin_sh == BINS) return 1;  // there are fewer than k keys but zeros
+        prefix |= (K)bin_sh << low;
+        want -= above_sh;
+        if (in_bin_sh == want) break;  // the whole bin is in
+    }
+    return prefix ? prefix : (K)1;
+}
+
+// One tile of a row; SORT: the only tile of its row, whose k best are sorted and written out.
+template <typename T, bool FROM_KEYS, bool SORT, int THREADS, int E>
+__global__ __launch_bounds__(THREADS) void topk_tile_kernel(KeySource<T, FROM_KEYS> src, int k,
+                                                            int index_bits, unsigned tiles,
+                                                            typename RowKey<T>::type *__restrict__ kept,
+                                                            int32_t *__restrict__ items_out,
+                                                            T *__restrict__ scores_out) {
+    typedef typename RowKey<T>::type key_t;
+    constexpr int VEC = FROM_KEYS ? 16 / (int)sizeof(key_t) : 16 / (int)sizeof(T);
+    static_assert(!SORT || THREADS == TR_MAX_K, "one key per thread to sort");
     __shared__ key_t sel[SORT ? TR_MAX_K : 1];
-    __shared__ int bin_sh, above_sh, in_bin_sh, n_kept;
-    const int tid = threadIdx.x;
+    __shared__ int n_kept;
+    const int tid = threadIdx.x, lane = tid & 63;
     const unsigned r32 = blockIdx.x / tiles;
     const int64_t row = r32;
     const unsigned tile = blockIdx.x - r32 * tiles;
-    const int64_t first = (int64_t)tile * TR_TILE;
-    const int64_t left = n - first;
-    const int count = left < TR_TILE ? (int)left : TR_TILE;
-    key_t key[TR_E];
+    const int64_t first = (int64_t)tile * (THREADS * E);
+    key_t key[E];
 #pragma unroll
-    for (int j = 0; j < TR_E; ++j) {
-        const int i = j * TR_THREADS + tid;
-        key[j] = 0;  // below every key: ~index is never 0
-        if (i < count) {
-            if constexpr (FROM_KEYS) key[j] = in[row * n + first + i];
-            else key[j] = RowKey<T>::make(scores[row * lds + first + i], (unsigned)(first + i));
-        }
-    }
-    // radix descent: `floor` = the smallest key kept
-    key_t floor_key = 1;
-    if (count > k) {
-        key_t prefix = 0;
-        int want = k;
-        for (int shift = RowKey<T>::BITS - 8; shift >= 0; shift -= 8) {
-            hist[tid] = 0;
-            __syncthreads();
-            const key_t high = shift + 8 >= RowKey<T>::BITS ? (key_t)0 : ~(key_t)0 << (shift + 8);
-            int run_bin = -1;
-            unsigned run = 0;
+    for (int j = 0; j < E; j += VEC) {
+        typedef KeySource<T, FROM_KEYS> source;
+        typename source::raw_t raw[VEC];
+        const int64_t at = first + j * THREADS + tid * VEC;
+        source::load(raw, src.data + row * src.ld, at, src.n);
 #pragma unroll
-            for (int j = 0; j < TR_E; ++j) {
-                if ((key[j] & high) != prefix) continue;
-                const int b = (int)(key[j] >> shift) & 255;
-                if (b != run_bin) {
-                    if (run) atomicAdd(&hist[run_bin], run);
-                    run_bin = b;
-                    run = 0;
-                }
-                ++run;
-            }
-            if (run) atomicAdd(&hist[run_bin], run);
-            __syncthreads();
-            if (tid < 64) {
-                // lane l holds bins 255 - 4l .. 252 - 4l; running count from the top
-                unsigned h[4], sum = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum += h[i] = hist[255 - 4 * tid - i];
-                unsigned upto = sum;
-#pragma unroll
-                for (int off = 1; off < 64; off <<= 1) {
-                    const unsigned o = __shfl_up(upto, off);
-                    if (tid >= off) upto += o;
-                }
-                unsigned above = upto - sum;
-                if (above < (unsigned)want && upto >= (unsigned)want) {
-                    int i = 0;
-                    while (above + h[i] < (unsigned)want) above += h[i++];
-                    bin_sh = 255 - 4 * tid - i;
-                    above_sh = (int)above;
-                    in_bin_sh = (int)h[i];
-                }
-            }
-            __syncthreads();
-            prefix |= (key_t)bin_sh << shift;
-            want -= above_sh;
-            if (in_bin_sh == want) break;  // the whole bin is kept
-        }
-        floor_key = prefix;
+        for (int i = 0; i < VEC; ++i) key[j + i] = source::key(raw[i], at + i, src.n);
     }
     if (tid == 0) n_kept = 0;
+    key_t floor_key = 1;
+    if (src.n - first > k) floor_key = kth_key<key_t, RowKey<T>::BITS, THREADS, E>(key, k, index_bits);
     __syncthreads();
     key_t *dst = SORT ? sel : kept + (row * tiles + tile) * k;
 #pragma unroll
-    for (int j = 0; j < TR_E; ++j)
-        if (key[j] != 0 && key[j] >= floor_key) dst[atomicAdd(&n_kept, 1)] = key[j];
+    for (int j = 0; j < E; ++j) {
+        const bool in = key[j] >= floor_key;
+        const unsigned long long m = __ballot(in);
+        if (m == 0) continue;
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&n_kept, (int)__popcll(m));
+        base = __builtin_amdgcn_readfirstlane(base);
+        if (in) dst[base + __popcll(m & ((1ull << lane) - 1ull))] = key[j];
+    }
     __syncthreads();
     const int have = n_kept;
     if constexpr (!SORT) {
-        for (int i = have + tid; i < k; i += TR_THREADS) dst[i] = 0;
+        for (int i = have + tid; i < k; i += THREADS) dst[i] = 0;
     } else {
-        int np2 = 1;
-        while (np2 < k) np2 <<= 1;
-        for (int i = have + tid; i < np2; i += TR_THREADS) sel[i] = 0;
-        __syncthreads();
-        for (int size = 2; size <= np2; size <<= 1)
-            for (int stride = size >> 1; stride > 0; stride >>= 1) {
-                for (int i = tid; i < np2 / 2; i += TR_THREADS) {
-                    const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
-                    const key_t a = sel[lo], b = sel[hi];
-                    if ((a > b) != ((lo & size) == 0)) {
-                        sel[lo] = b;
-                        sel[hi] = a;
-                    }
-                }
+        // one key per thread: sorted by wave, then runs of 64, 128, ... meet the mirror image of the next
+        // run; steps within a wave go through the lanes, the others through LDS
+        key_t mine = wave_sort(tid < have ? sel[tid] : (key_t)0, lane);
+        for (int size = 128; size < 2 * k; size <<= 1) {  // (runs behind the k-th key hold zeros)
+            int mask = size - 1;
+            for (int top = size >> 1; top >= 64; top >>= 1) {
                 __syncthreads();
+                sel[tid] = mine;
+                __syncthreads();
+                const key_t o = sel[tid ^ mask];
+                mine = (o > mine) != ((tid & top) != 0) ? o : mine;
+                mask = top >> 1;
             }
-        for (int i = tid; i < k; i += TR_THREADS) {
-            items_out[row * k + i] = (int32_t)~(unsigned)sel[i];
-            scores_out[row * k + i] = RowKey<T>::score(sel[i]);
+            mine = wave_merge(mine, lane);
+        }
+        if (tid < k) {
+            items_out[row * k + tid] = (int32_t)~(unsigned)mine;
+            scores_out[row * k + tid] = RowKey<T>::score(mine);
         }
     }
 }
 
-static int64_t topk_tiles(int64_t n) { return (n + TR_TILE - 1) / TR_TILE; }
+// ---- launches ------------------------------------------------------------------------------------
+// k <= 64: workgroups per row, so that the launch has about 1024, at least 4096 keys each.
+static int64_t list_parts(int64_t n_rows, int64_t n_items, int64_t &part_len) {
+    const int64_t most = (n_items + TR_PART - 1) / TR_PART;
+    int64_t parts = 1024 / n_rows;
+    parts = parts < 1 ? 1 : (parts > most ? most : parts);
+    part_len = ((n_items + parts - 1) / parts + TR_PART - 1) / TR_PART * TR_PART;
+    return (n_items + part_len - 1) / part_len;
+}
+static int64_t tiles_of(int64_t n) { return (n + TR_TILE - 1) / TR_TILE; }
 
 template <typename T>
-static int run_topk_rows(int64_t n_rows, int64_t n_items, const void *scores, int64_t lds, int k,
-                         int32_t *items_out, void *scores_out, void *workspace, hipStream_t st) {
+static int run_lists(int64_t n_rows, const KeySource<T, false> &src, int k, int32_t *items_out,
+                     T *scores_out, typename RowKey<T>::type *kept, hipStream_t st) {
+    int64_t part_len = 0;
+    const int64_t parts = list_parts(n_rows, src.n, part_len);
+    hipLaunchKernelGGL((topk_list_kernel<T, false>), dim3((unsigned)(parts * n_rows)), dim3(256), 0, st,
+                       src, k, (unsigned)parts, part_len, kept, items_out, scores_out);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    if (parts == 1) return ALSMI_OK;
+    const int64_t n = parts * k;
+    const KeySource<T, true> left = {kept, n, n};
+    hipLaunchKernelGGL((topk_list_kernel<T, true>), dim3((unsigned)n_rows), dim3(256), 0, st, left, k, 1u,
+                       (n + TR_PART - 1) / TR_PART * TR_PART, (typename RowKey<T>::type *)nullptr,
+                       items_out, scores_out);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
+template <typename T>
+static int run_tiles(int64_t n_rows, const KeySource<T, false> &src, int k, int32_t *items_out,
+                     T *scores_out, typename RowKey<T>::type *kept, hipStream_t st) {
     typedef typename RowKey<T>::type key_t;
-    const T *s = static_cast<const T *>(scores);
-    T *so = static_cast<T *>(scores_out);
-    // keys of the first level, then levels alternate between the two halves of the workspace
-    int64_t n = n_items, tiles = topk_tiles(n);
-    key_t *a = static_cast<key_t *>(workspace), *b = a + n_rows * tiles * k;
-    const dim3 block(TR_THREADS);
-    auto grid = [&](int64_t t) { return dim3((unsigned)(t * n_rows)); };
-    ALSMI_REQUIRE(tiles * n_rows <= INT32_MAX, "alsmi_topk_rows: too many rows x items");
-    if (tiles == 1) {
-        hipLaunchKernelGGL((topk_rows_kernel<T, false, true>), grid(1), block, 0, st, s, lds,
-                           (const key_t *)nullptr, n, k, 1u, (key_t *)nullptr, items_out, so);
+    const dim3 last_grid((unsigned)n_rows), last_block(TR_MAX_K);
+    int index_bits = 1;
+    while (index_bits < 31 && (src.n - 1) >> index_bits) ++index_bits;
+    if (src.n <= TR_LAST) {
+        hipLaunchKernelGGL((topk_tile_kernel<T, false, true, TR_MAX_K, TR_LAST / TR_MAX_K>), last_grid,
+                           last_block, 0, st, src, k, index_bits, 1u, (key_t *)nullptr, items_out, scores_out);
         ALSMI_HIP_CHECK(hipGetLastError());
         return ALSMI_OK;
     }
-    hipLaunchKernelGGL((topk_rows_kernel<T, false, false>), grid(tiles), block, 0, st, s, lds,
-                       (const key_t *)nullptr, n, k, (unsigned)tiles, a, (int32_t *)nullptr,
-                       (T *)nullptr);
+    int64_t tiles = tiles_of(src.n);
+    ALSMI_REQUIRE(tiles * n_rows <= INT32_MAX, "alsmi_topk_rows: too many rows x items");
+    hipLaunchKernelGGL((topk_tile_kernel<T, false, false, TR_THREADS, TR_TILE / TR_THREADS>),
+                       dim3((unsigned)(tiles * n_rows)), dim3(TR_THREADS), 0, st, src, k, index_bits,
+                       (unsigned)tiles, kept, (int32_t *)nullptr, (T *)nullptr);
     ALSMI_HIP_CHECK(hipGetLastError());
-    for (;;) {
-        n = tiles * k;
-        tiles = topk_tiles(n);
-        if (tiles == 1) break;
-        hipLaunchKernelGGL((topk_rows_kernel<T, true, false>), grid(tiles), block, 0, st, s, lds, a, n,
-                           k, (unsigned)tiles, b, (int32_t *)nullptr, (T *)nullptr);
+    // the levels alternate between the two parts of the workspace
+    key_t *from = kept, *to = kept + n_rows * tiles * k;
+    int64_t n = tiles * k;
+    while (n > TR_LAST) {
+        tiles = tiles_of(n);
+        const KeySource<T, true> left = {from, n, n};
+        hipLaunchKernelGGL((topk_tile_kernel<T, true, false, TR_THREADS, TR_TILE / TR_THREADS>),
+                           dim3((unsigned)(tiles * n_rows)), dim3(TR_THREADS), 0, st, left, k, index_bits,
+                           (unsigned)tiles, to, (int32_t *)nullptr, (T *)nullptr);
         ALSMI_HIP_CHECK(hipGetLastError());
-        key_t *t = a;
-        a = b;
-        b = t;
+        key_t *t = from;
+        from = to;
+        to = t;
+        n = tiles * k;
     }
-    hipLaunchKernelGGL((topk_rows_kernel<T, true, true>), grid(1), block, 0, st, s, lds, a, n, k, 1u,
-                       (key_t *)nullptr, items_out, so);
+    const KeySource<T, true> left = {from, n, n};
+    hipLaunchKernelGGL((topk_tile_kernel<T, true, true, TR_MAX_K, TR_LAST / TR_MAX_K>), last_grid,
+                       last_block, 0, st, left, k, index_bits, 1u, (key_t *)nullptr, items_out, scores_out);
     ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
+}
+
+template <typename T>
+static int run_topk_rows(int64_t n_rows, int64_t n_items, const void *scores, int64_t ld, int k,
+                         int32_t *items_out, void *scores_out, void *workspace, hipStream_t st) {
+    typedef typename RowKey<T>::type key_t;
+    const KeySource<T, false> src = {static_cast<const T *>(scores), ld, n_items};
+    T *so = static_cast<T *>(scores_out);
+    key_t *kept = static_cast<key_t *>(workspace);
+    return k <= TR_LIST ? run_lists<T>(n_rows, src, k, items_out, so, kept, st)
+                        : run_tiles<T>(n_rows, src, k, items_out, so, kept, st);
 }
 
 }  // namespace alsmi
@@ -210,11 +571,16 @@ size_t alsmi_topk_rows_workspace_bytes(int dtype, int64_t n_rows, int64_t n_item
     using namespace alsmi;
     if (dtype < ALSMI_F32 || dtype > ALSMI_BF16 || n_rows < 0 || n_items < 0 || k < 1 || k > TR_MAX_K)
         return 0;
-    const int64_t t1 = topk_tiles(n_items);
-    if (t1 <= 1) return 16;
-    const int64_t t2 = topk_tiles(t1 * k);
-    return (size_t)n_rows * (size_t)k * (size_t)(t1 + (t2 > 1 ? t2 : 0)) * (dtype == ALSMI_F64 ? 16 : 8) +
-           16;
+    if (n_rows == 0 || n_items == 0) return 16;
+    int64_t keys = 0;
+    if (k <= TR_LIST) {
+        int64_t part_len = 0;
+        keys = list_parts(n_rows, n_items, part_len) * k;
+    } else if (n_items > TR_LAST) {
+        const int64_t n = tiles_of(n_items) * k;
+        keys = n + (n > TR_LAST ? tiles_of(n) * k : 0);
+    }
+    return (size_t)n_rows * (size_t)keys * (dtype == ALSMI_F64 ? 16 : 8) + 16;
 }
 
 int alsmi_topk_rows(int dtype, int64_t n_rows, int64_t n_items, const void *scores, int64_t ld_scores,
