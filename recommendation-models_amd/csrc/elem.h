@@ -17,14 +17,17 @@ struct Elem<double> {
     typedef double wide;
 };
 
-// N consecutive elements from p, widened; those at or behind `valid` are zero and not read.
-template <typename T, int N>
+// N consecutive elements from p, widened; those at or behind `valid` are zero and not read.  STREAM: past
+// the caches (data that is larger than they are anyway).
+template <typename T, int N, bool STREAM = false>
 __device__ __forceinline__ void load_n(typename Elem<T>::wide (&v)[N], const T *__restrict__ p,
                                        int64_t valid) {
     typedef typename Elem<T>::wide W;
     typedef T vec_t __attribute__((ext_vector_type(N), aligned(sizeof(T))));
     if (valid >= N) {
-        const vec_t x = *reinterpret_cast<const vec_t *>(p);
+        vec_t x;
+        if constexpr (STREAM) x = __builtin_nontemporal_load(reinterpret_cast<const vec_t *>(p));
+        else x = *reinterpret_cast<const vec_t *>(p);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = (W)x[i];
     } else {
@@ -39,7 +42,7 @@ __device__ __forceinline__ void load8(typename Elem<T>::wide (&v)[8], const T *_
 }
 
 // The first `valid` of N elements to p, rounded to nearest.
-template <typename T, int N>
+template <typename T, int N, bool STREAM = false>
 __device__ __forceinline__ void store_n(T *__restrict__ p, const typename Elem<T>::wide (&v)[N],
                                         int64_t valid) {
     typedef T vec_t __attribute__((ext_vector_type(N), aligned(sizeof(T))));
@@ -47,7 +50,8 @@ __device__ __forceinline__ void store_n(T *__restrict__ p, const typename Elem<T
         vec_t x;
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = (T)v[i];
-        *reinterpret_cast<vec_t *>(p) = x;
+        if constexpr (STREAM) __builtin_nontemporal_store(x, reinterpret_cast<vec_t *>(p));
+        else *reinterpret_cast<vec_t *>(p) = x;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)

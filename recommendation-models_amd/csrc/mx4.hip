@@ -41,23 +41,27 @@ __device__ __forceinline__ unsigned long long abs_bits(double x) {
     return __builtin_bit_cast(unsigned long long, x) & 0x7fffffffffffffffull;
 }
 
-// Eight elements to eight codes, element 0 in the lowest four bits.
-__device__ __forceinline__ unsigned to_codes(const float (&x)[8], unsigned byte) {
+// E (4 or 8) elements to as many codes, element 0 in the lowest four bits.
+template <int E>
+__device__ __forceinline__ unsigned to_codes(const float (&x)[E], unsigned byte) {
     const float s = scale_value(byte);
     unsigned c = 0;  // (x / s rounded to nearest even and saturated by the instruction)
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], s, 0);
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], s, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], s, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], s, 3);
+    if constexpr (E == 8) {
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], s, 2);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], s, 3);
+    }
     return byte == 255u ? 0u : c;
 }
 // fp64 elements are compared with the midpoints in fp64: a first rounding to fp32 could carry a
 // value onto a midpoint.
-__device__ __forceinline__ unsigned to_codes(const double (&x)[8], unsigned byte) {
+template <int E>
+__device__ __forceinline__ unsigned to_codes(const double (&x)[E], unsigned byte) {
     if (byte == 255u) return 0u;
     unsigned c = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < E; ++i) {
         const double v = ldexp(fabs(x[i]), 127 - (int)byte);
         unsigned m = (v > 0.25) + (v >= 0.75) + (v > 1.25) + (v >= 1.75) + (v > 2.5) + (v >= 3.5) +
                      (v > 5.0);
@@ -67,85 +71,143 @@ __device__ __forceinline__ unsigned to_codes(const double (&x)[8], unsigned byte
     return c;
 }
 
-// A lane takes eight consecutive elements, four neighbouring lanes a block: 32 bytes of fp32 per
-// lane in, four bytes out.  `upr` = lanes per row (4 per block); a workgroup takes `rpb` whole rows, or
-// 256 lanes' worth of one row (blockIdx.y) where a row is longer than that.  Bound by HBM.
+// Elements of T per lane: 16 bytes a load, so that a wave's loads are contiguous.
 template <typename T>
+constexpr int mx4_lane() {
+    return sizeof(T) == 2 ? 8 : 4;
+}
+// How a workgroup covers rows: `upr` lanes' worth (units) a row, TURNS * 256 units per workgroup, as whole
+// rows (`rpb` of them) or as part blockIdx.y of one row.
+constexpr int MX4_TURNS = 4;
+struct RowGrid {
+    unsigned upr, rpb, inverse;  // inverse: 2^32 / upr rounded up
+    dim3 grid;
+};
+static RowGrid row_grid(int64_t n_rows, int nb, int per_lane) {
+    RowGrid r;
+    constexpr unsigned UNITS = 256 * MX4_TURNS;
+    r.upr = (unsigned)nb * (MX4_BLOCK / per_lane);
+    r.rpb = r.upr < UNITS ? UNITS / r.upr : 1;
+    r.inverse = (unsigned)((((uint64_t)1 << 32) + r.upr - 1) / r.upr);
+    r.grid = dim3((unsigned)((n_rows + r.rpb - 1) / r.rpb), (r.upr + UNITS - 1) / UNITS);
+    return r;
+}
+// Row and unit of a thread in a turn; false where there is none.  (x < 1024: the product is exact.)
+__device__ __forceinline__ bool row_unit(const unsigned upr, const unsigned rpb, const unsigned inverse,
+                                         int turn, int64_t n_rows, int64_t &row, unsigned &sub) {
+    const unsigned x = turn * 256 + threadIdx.x;
+    const unsigned rl = rpb > 1 ? __umulhi(x, inverse) : 0u;
+    sub = x - rl * upr + blockIdx.y * (256 * MX4_TURNS);
+    row = (int64_t)blockIdx.x * rpb + rl;
+    return rl < rpb && row < n_rows && sub < upr;
+}
+
+// Tables larger than the last-level cache go past it: written through it, the lines of one call
+// are still being written back during the next (1 M x 128 fp32: reading back 90 us either way, but
+// quantising after it 139 us, 101 past the cache).  Smaller ones are left in it for their reader.
+constexpr int64_t MX4_STREAM_BYTES = (int64_t)256 << 20;
+
+// A lane takes 16 bytes of elements, 4 or 8 neighbouring lanes a block.  Bound by HBM.
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(int64_t n_rows, int width,
                                                            const T *__restrict__ x, int64_t ldx,
                                                            uint8_t *__restrict__ codes,
-                                                           uint8_t *__restrict__ scales, int upr,
-                                                           int rpb) {
+                                                           uint8_t *__restrict__ scales, unsigned upr,
+                                                           unsigned rpb, unsigned inverse) {
     typedef typename Elem<T>::wide W;
-    const unsigned rl = threadIdx.x / (unsigned)upr;  // (0 where upr >= 256)
-    if (rl >= (unsigned)rpb) return;                  // whole groups of four lanes leave together
-    const int64_t row = (int64_t)blockIdx.x * rpb + rl;
-    const int sub = (int)(threadIdx.x - rl * upr) + (int)blockIdx.y * 256;
-    if (row >= n_rows || sub >= upr) return;
-    W v[8];
-    load8<T>(v, x + row * ldx + (int64_t)sub * 8, width - sub * 8);
-    auto m = abs_bits(v[0]);
+    constexpr int E = mx4_lane<T>(), LANES = MX4_BLOCK / E;
+    typedef typename std::conditional<E == 8, unsigned, unsigned short>::type code_t;
+    W v[MX4_TURNS][E];
+    int64_t row[MX4_TURNS];
+    unsigned sub[MX4_TURNS];
+    bool in[MX4_TURNS];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
-        const auto b = abs_bits(v[i]);
-        m = b > m ? b : m;
+    for (int t = 0; t < MX4_TURNS; ++t) {
+        in[t] = row_unit(upr, rpb, inverse, t, n_rows, row[t], sub[t]);
+        load_n<T, E, STREAM>(v[t], x + (in[t] ? row[t] * ldx + (int64_t)sub[t] * E : 0),
+                     in[t] ? width - (int)sub[t] * E : 0);
     }
 #pragma unroll
-    for (int off = 1; off < 4; off <<= 1) {
-        const auto b = __shfl_xor(m, off);
-        m = b > m ? b : m;
+    for (int t = 0; t < MX4_TURNS; ++t) {
+        auto m = abs_bits(v[t][0]);
+#pragma unroll
+        for (int i = 1; i < E; ++i) {
+            const auto b = abs_bits(v[t][i]);
+            m = b > m ? b : m;
+        }
+#pragma unroll
+        for (int off = 1; off < LANES; off <<= 1) {
+            const auto b = __shfl_xor(m, off);
+            m = b > m ? b : m;
+        }
+        const unsigned byte = scale_byte(m);
+        const unsigned c = to_codes(v[t], byte);
+        if (!in[t]) continue;  // (a block's lanes are all in or all out)
+        const int64_t at = row[t] * upr + sub[t];
+        reinterpret_cast<code_t *>(codes)[at] = (code_t)c;
+        if (sub[t] % LANES == 0) scales[at / LANES] = (uint8_t)byte;
     }
-    const unsigned byte = scale_byte(m);
-    const int64_t at = row * upr + sub;
-    reinterpret_cast<unsigned *>(codes)[at] = to_codes(v, byte);
-    if ((sub & 3) == 0) scales[at >> 2] = (uint8_t)byte;
 }
 
 // ---- reading back --------------------------------------------------------------------------------
-__device__ __forceinline__ void from_codes(unsigned c, unsigned byte, float (&v)[8]) {
+template <int E>
+__device__ __forceinline__ void from_codes(unsigned c, unsigned byte, float (&v)[E]) {
     typedef float f2 __attribute__((ext_vector_type(2)));
     const float s = scale_value(byte);
     const f2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 0);
     const f2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 1);
-    const f2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
-    const f2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
     v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
-    v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
+    if constexpr (E == 8) {
+        const f2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 2);
+        const f2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, 3);
+        v[4] = d[0], v[5] = d[1], v[6] = e[0], v[7] = e[1];
+    }
 }
 // (fp64: 6 x 2^127 is past fp32's range, so the scale is applied in fp64)
-__device__ __forceinline__ void from_codes(unsigned c, unsigned byte, double (&v)[8]) {
-    float f[8];
+template <int E>
+__device__ __forceinline__ void from_codes(unsigned c, unsigned byte, double (&v)[E]) {
+    float f[E];
     from_codes(c, byte == 255u ? 255u : 127u, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = ldexp((double)f[i], (int)byte - 127);
+    for (int i = 0; i < E; ++i) v[i] = ldexp((double)f[i], (int)byte - 127);
 }
 
 // Row i of the output is row rows[i] of the table (row i where rows is null), NaN where there is
 // no such row.  Lanes as in mx4_quantize_kernel.
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t n_sel,
                                                              const int32_t *__restrict__ rows,
                                                              int64_t n_rows, int width,
                                                              const uint8_t *__restrict__ codes,
                                                              const uint8_t *__restrict__ scales,
                                                              T *__restrict__ out, int64_t ldo,
-                                                             int upr, int rpb) {
+                                                             unsigned upr, unsigned rpb,
+                                                             unsigned inverse) {
     typedef typename Elem<T>::wide W;
-    const unsigned rl = threadIdx.x / (unsigned)upr;
-    if (rl >= (unsigned)rpb) return;
-    const int64_t i = (int64_t)blockIdx.x * rpb + rl;
-    const int sub = (int)(threadIdx.x - rl * upr) + (int)blockIdx.y * 256;
-    if (i >= n_sel || sub >= upr) return;
-    const int64_t row = rows ? (int64_t)rows[i] : i;
-    unsigned c = 0, byte = 255u;
-    if (row >= 0 && row < n_rows) {
+    constexpr int E = mx4_lane<T>(), LANES = MX4_BLOCK / E;
+    typedef typename std::conditional<E == 8, unsigned, unsigned short>::type code_t;
+    unsigned c[MX4_TURNS], byte[MX4_TURNS];
+#pragma unroll
+    for (int t = 0; t < MX4_TURNS; ++t) {
+        int64_t i;
+        unsigned sub;
+        c[t] = 0, byte[t] = 255u;
+        if (!row_unit(upr, rpb, inverse, t, n_sel, i, sub)) continue;
+        const int64_t row = rows ? (int64_t)rows[i] : i;
+        if (row < 0 || row >= n_rows) continue;
         const int64_t at = row * upr + sub;
-        c = reinterpret_cast<const unsigned *>(codes)[at];
-        byte = scales[at >> 2];
+        c[t] = reinterpret_cast<const code_t *>(codes)[at];
+        byte[t] = scales[at / LANES];
     }
-    W v[8];
-    from_codes(c, byte, v);
-    store8<T>(out + i * ldo + (int64_t)sub * 8, v, width - sub * 8);
+#pragma unroll
+    for (int t = 0; t < MX4_TURNS; ++t) {
+        int64_t i;
+        unsigned sub;
+        if (!row_unit(upr, rpb, inverse, t, n_sel, i, sub)) continue;
+        W v[E];
+        from_codes(c[t], byte[t], v);
+        store_n<T, E, STREAM>(out + i * ldo + (int64_t)sub * E, v, width - (int)sub * E);
+    }
 }
 
 // ---- scores: out[i, j] = sum_k a[i, k] table[j, k] -----------------------------------------------
@@ -833,18 +895,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
 }
 
 // ---- launches ------------------------------------------------------------------------------------
-struct RowGrid {
-    int upr, rpb;
-    dim3 grid;
-};
-static RowGrid row_grid(int64_t n_rows, int nb) {
-    RowGrid r;
-    r.upr = 4 * nb;
-    r.rpb = r.upr < 256 ? 256 / r.upr : 1;
-    r.grid = dim3((unsigned)((n_rows + r.rpb - 1) / r.rpb), (unsigned)((r.upr + 255) / 256));
-    return r;
-}
-
 template <typename T, typename TO, int NBL, int UT, int NT>
 static int launch_narrow(const Rows &rows, const void *a, int width, const uint8_t *codes,
                          const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
@@ -989,10 +1039,15 @@ int alsmi_mx4_quantize(int dtype, int64_t n_rows, int64_t width, const void *x, 
     ALSMI_REQUIRE((uintptr_t)codes % 4 == 0, "alsmi_mx4_quantize: codes must be aligned to 4 bytes");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
-    const RowGrid rg = row_grid(n_rows, nb);
 #define ALSMI_CASE(T)                                                                                \
-    hipLaunchKernelGGL((mx4_quantize_kernel<T>), rg.grid, dim3(256), 0, st, n_rows, (int)width,      \
-                       static_cast<const T *>(x), ldx, codes, scales, rg.upr, rg.rpb)
+    do {                                                                                             \
+        const RowGrid rg = row_grid(n_rows, nb, mx4_lane<T>());                                      \
+        auto kernel = n_rows * width * (int64_t)sizeof(T) > MX4_STREAM_BYTES                         \
+                          ? mx4_quantize_kernel<T, true>                                             \
+                          : mx4_quantize_kernel<T, false>;                                           \
+        hipLaunchKernelGGL(kernel, rg.grid, dim3(256), 0, st, n_rows, (int)width,                    \
+                           static_cast<const T *>(x), ldx, codes, scales, rg.upr, rg.rpb, rg.inverse); \
+    } while (0)
     if (dtype == ALSMI_F32) ALSMI_CASE(float);
     else if (dtype == ALSMI_F64) ALSMI_CASE(double);
     else if (dtype == ALSMI_F16) ALSMI_CASE(_Float16);
@@ -1022,10 +1077,16 @@ int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t 
     ALSMI_REQUIRE((uintptr_t)codes % 4 == 0, "alsmi_mx4_dequantize: codes must be aligned to 4 bytes");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
-    const RowGrid rg = row_grid(n_sel, nb);
 #define ALSMI_CASE(T)                                                                                 \
-    hipLaunchKernelGGL((mx4_dequantize_kernel<T>), rg.grid, dim3(256), 0, st, n_sel, rows, n_rows,    \
-                       (int)width, codes, scales, static_cast<T *>(out), ldo, rg.upr, rg.rpb)
+    do {                                                                                              \
+        const RowGrid rg = row_grid(n_sel, nb, mx4_lane<T>());                                        \
+        auto kernel = n_sel * width * (int64_t)sizeof(T) > MX4_STREAM_BYTES                           \
+                          ? mx4_dequantize_kernel<T, true>                                            \
+                          : mx4_dequantize_kernel<T, false>;                                          \
+        hipLaunchKernelGGL(kernel, rg.grid, dim3(256), 0, st, n_sel, rows, n_rows,                    \
+                           (int)width, codes, scales, static_cast<T *>(out), ldo, rg.upr, rg.rpb,     \
+                           rg.inverse);                                                               \
+    } while (0)
     if (dtype == ALSMI_F32) ALSMI_CASE(float);
     else if (dtype == ALSMI_F64) ALSMI_CASE(double);
     else if (dtype == ALSMI_F16) ALSMI_CASE(_Float16);
