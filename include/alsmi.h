@@ -223,10 +223,11 @@ int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_ro
 
 /* Penalties, exclusion, biases and masks of score rows.  For row r and item i, with c = the
  * occurrences of i in the row's history:
- *   c > 0:  x = -inf if `exclude`, else x = s > 0 ? s / repetition : s * repetition and
- *           x -= frequency * c + presence;      c == 0: x = s
+ *   c > 0:  x = s > 0 ? s / repetition : s * repetition, then x -= frequency * c + presence
+ *   c == 0: x = s
  *   x += item_bias[i];  x += the value of the last entry of i in the row's bias list
- *   x = -inf where the row's mask has no bit i (bit i % 32 of word i / 32 set: i is on offer)
+ *   x = -inf where the row's mask has no bit i (bit i % 32 of word i / 32 set: i is on offer), or
+ *   where c > 0 if `exclude`
  * worked in fp32 (fp64 for ALSMI_F64), rounded once.  `out` may be `scores` itself.
  * Any pointer may be NULL: no history / bias list / item bias / mask.  repetition, frequency and
  * presence are [n_rows] fp32 arrays, or NULL for the *_value fields.  The history of row r is list

@@ -276,11 +276,10 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
 
     For row r and item i, with c the number of times i occurs in the row's history:
 
-        c > 0:  x = -inf                                      with `exclude`, else
-                x = s / repetition if s > 0 else s * repetition, then
+        c > 0:  x = s / repetition if s > 0 else s * repetition, then
                 x -= frequency * c + presence
         x += item_bias[i];  x += the last value given for i in the row's `row_bias`
-        x = -inf where the row's mask has no bit i
+        x = -inf where the row's mask has no bit i, or where c > 0 with `exclude`
 
     worked in float32 (float64 for float64 scores) and rounded once.
 
