@@ -215,11 +215,13 @@ int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t 
  * out_dtype (ALSMI_F32, F16 or BF16).  `a` has n_rows rows of `width` elements of dtype ALSMI_F32,
  * F16 or BF16 (every product exact, fp32 sums), or with ALSMI_MX4 is a table's codes and a_scales
  * its scales (a_scales is ignored otherwise).  rows as in alsmi_mx4_dequantize: a row of NaN where
- * there is no such row. */
+ * there is no such row.  workspace: alsmi_mx4_scores_workspace_bytes() bytes, aligned to 16 (large
+ * products of float activations split them there first); may be NULL where that is 0. */
+size_t alsmi_mx4_scores_workspace_bytes(int dtype, int64_t n_sel, int64_t n_items, int64_t width);
 int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, const void *a,
                      int64_t ld_a, const uint8_t *a_scales, int64_t n_items, int64_t width,
                      const uint8_t *codes, const uint8_t *scales, int out_dtype, void *out,
-                     int64_t ld_out, void *stream);
+                     int64_t ld_out, void *workspace, void *stream);
 
 /* Penalties, exclusion, biases and masks of score rows.  For row r and item i, with c = the
  * occurrences of i in the row's history:

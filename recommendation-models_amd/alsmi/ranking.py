@@ -222,9 +222,11 @@ def mx4_scores(a, table, rows=None, out_dtype=None, out=None):
         raise ValueError('rows of an empty a')
     out, ldo = _result('out', out, (m, len(table)), out_dtype, table.device, data, table.codes)
     device = _device(table.codes, table.scales, data, a_scales, rows, out)
-    _call(device, 'alsmi_mx4_scores', code, m, _p(rows), a.shape[0], _p(data), ld, _p(a_scales),
-          len(table), table.width, _p(table.codes), _p(table.scales), _CODES[out_dtype], _p(out),
-          ldo)
+    n, width = table.shape
+    size = _lib.load().alsmi_mx4_scores_workspace_bytes(code, m, n, width)
+    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _call(device, 'alsmi_mx4_scores', code, m, _p(rows), a.shape[0], _p(data), ld, _p(a_scales), n,
+          width, _p(table.codes), _p(table.scales), _CODES[out_dtype], _p(out), ldo, _p(ws))
     return out
 
 

@@ -564,6 +564,169 @@ __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T
     }
 }
 
+// ---- large products of float activations ---------------------------------------------------------
+// A first kernel splits the activations into their bf16 parts, rows picked and padded to whole turns
+// (planes[p][row][steps * 64]); a second one forms 128 rows x 128 items per workgroup through LDS,
+// four waves of 64 x 64, in steps of 64 elements, two steps a turn.  Parts and codes go from
+// memory straight into LDS, into two buffers; the codes become bf16 in registers, once per wave
+// and step for all parts of 64 rows.  Each part costs one matrix instruction: fp32 activations run at a
+// third of the bf16 rate.
+constexpr int WT_ROWS = 128, WT_ITEMS = 128;
+
+template <typename T>
+__global__ __launch_bounds__(256) void mx4_split_kernel(Rows rows, const T *__restrict__ a, int width,
+                                                        int units, u32x4 *__restrict__ planes) {
+    constexpr int NP = Parts<T>::N;
+    const int64_t i = blockIdx.x;  // one row per workgroup and turn, eight elements per thread
+    const int64_t r = rows.of(i);
+    for (int u = threadIdx.x; u < units; u += 256) {
+        float x[8];
+        load8<T>(x, a + (r < 0 ? 0 : r) * rows.ld + (int64_t)u * 8, width - u * 8);
+        if (r < 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __builtin_nanf("");
+        }
+        bf16x8 h[NP];
+        split8<NP>(x, h);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+            planes[((int64_t)p * rows.n_sel + i) * units + u] = __builtin_bit_cast(u32x4, h[p]);
+    }
+}
+
+template <typename TO, int NP>
+__global__ __launch_bounds__(256, 2) void mx4_scores_split_kernel(const u32x4 *__restrict__ planes,
+                                                                  const uint8_t *__restrict__ codes,
+                                                                  const uint8_t *__restrict__ scales,
+                                                                  int nb, ScoreStore o, int row_tiles) {
+    constexpr int MT = 4, NT = 4;
+    // rows of the parts (eight chunks of eight elements each, permuted as in mx4_scores_tiled_kernel)
+    // and of the items (two blocks each); separate arrays: see there
+    __shared__ u32x4 sa0[NP * WT_ROWS * 8], sa1[NP * WT_ROWS * 8];
+    __shared__ u32x4 sb0[WT_ITEMS * 2], sb1[WT_ITEMS * 2];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, q = lane & 15;
+    const unsigned total = gridDim.x, xcd = blockIdx.x & 7u, nth = blockIdx.x >> 3;
+    const unsigned per = total >> 3, extra = total & 7u;
+    const unsigned tile = xcd * per + (xcd < extra ? xcd : extra) + nth;
+    const int64_t row_base = (int64_t)(tile % (unsigned)row_tiles) * WT_ROWS;
+    const int64_t item_base = (int64_t)(tile / (unsigned)row_tiles) * WT_ITEMS;
+    const int turns = (nb + 3) / 4;
+    const int64_t units = (int64_t)turns * 16;  // chunks of a row of the planes
+    auto b_row = [&](int i) {
+        const int64_t r = item_base + i;
+        return r < o.n_items ? r : o.n_items - 1;
+    };
+    // A thread's slots in a part's rows: row 32 i + tid / 8, chunk (tid % 8) ^ (row / 2 % 8), the same
+    // for every i; its slot of the items: place tid / 2, block tid % 2.  The item at a place: the 16
+    // items that a matrix operand reads at once lie side by side.
+    const int chunk = (tid & 7) ^ (tid >> 4 & 7);
+    const u32x4 *asrc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = row_base + i * 32 + (tid >> 3);
+        asrc[i] = planes + (r < o.n_sel ? r : o.n_sel - 1) * units + chunk;
+    }
+    const int64_t plane = o.n_sel * units;
+    const int place = tid >> 1;
+    const int64_t bsrc =
+        b_row((place & 3) | (place >> 4 & 3) << 2 | (place >> 2 & 3) << 4 | (place & 64)) * nb;
+    auto load_step = [&](unsigned step, u32x4 *to_a, u32x4 *to_b) __attribute__((always_inline)) {
+        // (one step is loaded past the last turn, and not used)
+        const unsigned s = step < 2u * turns ? step : 0u;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void *)(asrc[i] + p * plane + s * 8u),
+                    (__attribute__((address_space(3))) void *)&to_a[(p * 4 + i) * 256 + wave * 64], 16, 0,
+                    0);
+        // (a block behind the row's end meets zeros of the activations: any codes will do)
+        const unsigned k = 2u * s + (tid & 1);
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void *)(codes +
+                                                             (bsrc + (k < (unsigned)nb ? k : nb - 1)) * 16),
+            (__attribute__((address_space(3))) void *)&to_b[wave * 64], 16, 0, 0);
+    };
+    const int wm = wave & 1, wn = wave >> 1;
+    const int ar = wm * 64 + q, sa = ar >> 1 & 7;
+    const uint8_t *srow[NT];  // the scales of this lane's items
+#pragma unroll
+    for (int n = 0; n < NT; ++n) srow[n] = scales + b_row(wn * 64 + item_of<NT>(n, q)) * nb;
+    unsigned sw[NT];
+    auto load_scales = [&](int turn) {  // the turn's four scales; 1 behind the row's end
+        typedef unsigned word_t __attribute__((aligned(1)));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (4 * turn + 4 <= nb) {
+                sw[n] = *reinterpret_cast<const word_t *>(srow[n] + 4 * turn);
+            } else {
+                sw[n] = 0x7f7f7f7fu;
+                for (int i = 0; 4 * turn + i < nb; ++i)
+                    sw[n] = (sw[n] & ~(255u << (8 * i))) | (unsigned)srow[n][4 * turn + i] << (8 * i);
+            }
+        }
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{0, 0, 0, 0};
+    auto products = [&](int step, const u32x4 *a, const u32x4 *b, const unsigned (&w)[NT])
+                        __attribute__((always_inline)) {
+        const u32x2 *codes_of = reinterpret_cast<const u32x2 *>(b) + (wn * 64 + q) * 4 + g;
+        u32x2 c[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) c[n] = codes_of[n * 16 * 4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            bf16x8 bf[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                bf[n] = codes_to_bf16(c[n][j], scale_value(w[n] >> (16 * step + 8 * (g >> 1)) & 255u));
+#pragma unroll
+            for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const bf16x8 af = __builtin_bit_cast(
+                        bf16x8, a[(p * WT_ROWS + ar + 16 * t) * 8 + ((2 * g + j) ^ sa)]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        acc[t][n] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[n], af, acc[t][n], 0, 0, 0);
+                }
+        }
+    };
+    load_scales(0);
+    load_step(0, sa0, sb0);
+    for (int turn = 0; turn < turns; ++turn) {
+        unsigned w[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) w[n] = sw[n];
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's part of the step is in LDS
+        __syncthreads();                     // everyone's is, and the other buffer is free
+        load_step(2 * turn + 1, sa1, sb1);
+        if (turn + 1 < turns) load_scales(turn + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        products(0, sa0, sb0, w);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __syncthreads();
+        load_step(2 * turn + 2, sa0, sb0);
+        __builtin_amdgcn_sched_barrier(0);
+        products(1, sa1, sb1, w);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // (the step loaded for nothing)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+        put_row<TO, NT>(out_row<TO>(o, row_base + ar + 16 * t), item_base + wn * 64 + 4 * NT * g, o.n_items,
+                        acc[t]);
+}
+
 // Both sides in 4 bits: v_mfma_scale_f32_16x16x128_f8f6f4 takes 32 codes per lane (one block) and
 // its scale byte, four blocks per instruction.
 __device__ __forceinline__ i32x8 as_operand(u32x4 w) {
@@ -998,9 +1161,38 @@ static int run_both(const Rows &rows, const void *a, const uint8_t *a_scales, co
     return launch_both<TO, 4, 4, 1>(rows, a, a_scales, codes, scales, nb, o, st);
 }
 
+// Whether a float product is split first: enough whole tiles, and rows long enough for a few turns.
+static bool splits(int64_t n_sel, int64_t n_items, int nb) {
+    const int64_t tiles = (n_sel + WT_ROWS - 1) / WT_ROWS * ((n_items + WT_ITEMS - 1) / WT_ITEMS);
+    return n_sel > 64 && nb > 4 && tiles >= 128;
+}
+static int64_t split_bytes(int64_t n_sel, int nb, int parts) {
+    return n_sel * ((nb + 3) / 4) * 256 * parts;
+}
+
+template <typename T, typename TO>
+static int launch_split(const Rows &rows, const void *a, int width, const uint8_t *codes,
+                        const uint8_t *scales, int nb, const ScoreStore &o, void *workspace,
+                        hipStream_t st) {
+    u32x4 *planes = static_cast<u32x4 *>(workspace);
+    const int64_t row_tiles = (rows.n_sel + WT_ROWS - 1) / WT_ROWS;
+    const int64_t blocks = (o.n_items + WT_ITEMS - 1) / WT_ITEMS * row_tiles;
+    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
+    hipLaunchKernelGGL((mx4_split_kernel<T>), dim3((unsigned)rows.n_sel), dim3(256), 0, st, rows,
+                       static_cast<const T *>(a), width, (nb + 3) / 4 * 16, planes);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL((mx4_scores_split_kernel<TO, Parts<T>::N>), dim3((unsigned)blocks), dim3(256), 0, st,
+                       planes, codes, scales, nb, o, (int)row_tiles);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    return ALSMI_OK;
+}
+
 template <typename T, typename TO>
 static int run_scores(const Rows &rows, const void *a, int width, const uint8_t *codes,
-                      const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
+                      const uint8_t *scales, int nb, const ScoreStore &o, void *workspace,
+                      hipStream_t st) {
+    if (splits(rows.n_sel, o.n_items, nb) && (uintptr_t)codes % 16 == 0)
+        return launch_split<T, TO>(rows, a, width, codes, scales, nb, o, workspace, st);
     const bool one = rows.n_sel <= 16;
     if (nb == 1)
         return one ? launch_narrow<T, TO, 1, 1, 2>(rows, a, width, codes, scales, nb, o, st)
@@ -1096,10 +1288,18 @@ int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t 
     return ALSMI_OK;
 }
 
+size_t alsmi_mx4_scores_workspace_bytes(int dtype, int64_t n_sel, int64_t n_items, int64_t width) {
+    using namespace alsmi;
+    if (n_sel < 0 || n_items < 0 || width < 1 || width > MX4_MAX_WIDTH) return 0;
+    const int parts = dtype == ALSMI_F32 ? 3 : dtype == ALSMI_F16 ? 2 : dtype == ALSMI_BF16 ? 1 : 0;
+    const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
+    return splits(n_sel, n_items, nb) ? (size_t)split_bytes(n_sel, nb, parts) : 0;
+}
+
 int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, const void *a,
                      int64_t lda, const uint8_t *a_scales, int64_t n_items, int64_t width,
                      const uint8_t *codes, const uint8_t *scales, int out_dtype, void *out,
-                     int64_t ldo, void *stream) {
+                     int64_t ldo, void *workspace, void *stream) {
     using namespace alsmi;
     ALSMI_REQUIRE(dtype == ALSMI_F32 || dtype == ALSMI_F16 || dtype == ALSMI_BF16 || dtype == ALSMI_MX4,
                   "alsmi_mx4_scores: bad dtype %d", dtype);
@@ -1124,16 +1324,19 @@ int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_ro
                   "alsmi_mx4_scores: codes must be aligned to 4 bytes");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
+    ALSMI_REQUIRE(alsmi_mx4_scores_workspace_bytes(dtype, n_sel, n_items, width) == 0 ||
+                      (workspace && (uintptr_t)workspace % 16 == 0),
+                  "alsmi_mx4_scores: needs a workspace aligned to 16 bytes");
     const Rows r = {n_sel, n_rows, lda, rows};
     const ScoreStore o = {out, ldo, n_sel, n_items};
 #define ALSMI_CASE(TO)                                                                               \
     do {                                                                                             \
         if (dtype == ALSMI_F32)                                                                      \
-            return run_scores<float, TO>(r, a, (int)width, codes, scales, nb, o, st);                \
+            return run_scores<float, TO>(r, a, (int)width, codes, scales, nb, o, workspace, st);     \
         if (dtype == ALSMI_F16)                                                                      \
-            return run_scores<_Float16, TO>(r, a, (int)width, codes, scales, nb, o, st);             \
+            return run_scores<_Float16, TO>(r, a, (int)width, codes, scales, nb, o, workspace, st);             \
         if (dtype == ALSMI_BF16)                                                                     \
-            return run_scores<__bf16, TO>(r, a, (int)width, codes, scales, nb, o, st);               \
+            return run_scores<__bf16, TO>(r, a, (int)width, codes, scales, nb, o, workspace, st);               \
         return run_both<TO>(r, a, a_scales, codes, scales, nb, o, st);                              \
     } while (0)
     if (out_dtype == ALSMI_F32) ALSMI_CASE(float);

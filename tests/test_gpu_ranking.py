@@ -178,10 +178,11 @@ def test_scores_match_definition(m, n, width, kind):
     assert bool((flat[3:].view(m + 3, n + 5)[:, n:] == 7).all()) and bool((flat[:3] == 7).all())
 
 
-@pytest.mark.parametrize('kind', ['f32', 'bf16', 'mx4'])
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'f16', 'mx4'])
 @pytest.mark.parametrize('m,n,width', [(1, 300001, 64), (3, 540000, 130), (20, 140000, 132),
                                        (1, 70001, 200), (257, 9001, 128), (2048, 2049, 192),
-                                       (513, 2000, 2080)])
+                                       (513, 2000, 2080), (300, 6001, 300), (1000, 2100, 1100),
+                                       (129, 8300, 135), (4000, 3333, 520), (70, 16385, 512)])
 def test_scores_large(m, n, width, kind):
     """Sizes that take the long-walk and one-step forms; a strip of items against the definition,
     the rest against another order of the same items."""
@@ -189,15 +190,49 @@ def test_scores_large(m, n, width, kind):
     g.manual_seed(m + n)
     table = rk.mx4_quantize(torch.randn(n, width, generator=g, device='cuda'))
     a = torch.randn(m, width, generator=g, device='cuda')
-    at = rk.mx4_quantize(a) if kind == 'mx4' else a.to({'f32': F32, 'bf16': BF16}[kind])
+    at = rk.mx4_quantize(a) if kind == 'mx4' else a.to({'f32': F32, 'bf16': BF16, 'f16': F16}[kind])
     av = host(rk.mx4_dequantize(at)) if kind == 'mx4' else host(at)
     got = rk.mx4_scores(at, table, out_dtype=F32)
+    half = rk.mx4_scores(at, table, out_dtype=BF16)
+    assert torch.equal(half, got.to(BF16))  # rounded once, from the same sums
     strip = torch.cat((torch.arange(0, min(n, 64)), torch.arange(n // 2, n // 2 + 40) % n,
                        torch.arange(max(0, n - 70), n))).cuda()
     values = ro.mx4_values(table.codes[strip].cpu().numpy(), table.scales[strip].cpu().numpy(), width)
     check_scores(host(got[:, strip]), av, values, F32)
     back = rk.Mx4Table(table.codes.flip(0).contiguous(), table.scales.flip(0).contiguous(), width)
     assert torch.equal(rk.mx4_scores(at, back, out_dtype=F32).flip(1), got)
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'f16', 'mx4'])
+@pytest.mark.parametrize('m,n,width', [(200, 9001, 300), (300, 70000, 544), (17, 40000, 700)])
+def test_scores_of_picked_rows_large(m, n, width, kind):
+    """Rows by id, some missing, out of strided activations into a strided output, at sizes of the
+    tiled forms; blocks that are no number reach their items alone."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(m)
+    table = rk.mx4_quantize(torch.randn(n, width, generator=g, device='cuda'))
+    table.scales[5, -1] = 255
+    table.scales[n - 1, 0] = 255
+    a = torch.randn(3 * m, width, generator=g, device='cuda')
+    at = rk.mx4_quantize(a) if kind == 'mx4' else strided(
+        a.to({'f32': F32, 'bf16': BF16, 'f16': F16}[kind]), 1, 1)[0]
+    ids = torch.randint(0, 3 * m, (m,), generator=g, device='cuda').to(torch.int32)
+    ids[3], ids[m - 1] = -1, 3 * m
+    out, flat = strided(torch.zeros(m, n, device='cuda'), 3, 1)
+    rk.mx4_scores(at, table, rows=ids, out=out)
+    assert bool((flat[1:].view(m, n + 3)[:, n:] == 7).all())
+    none = torch.zeros(m, dtype=torch.bool, device='cuda')
+    none[3] = none[m - 1] = True
+    nan = torch.isnan(out)
+    want = torch.zeros_like(nan)
+    want[none] = True
+    want[:, 5] = want[:, n - 1] = True
+    assert torch.equal(nan, want)
+    values = rk.mx4_dequantize(at) if kind == 'mx4' else at.float()
+    picked = values[ids.long().clamp(0, 3 * m - 1)]
+    cols = torch.randint(6, n - 1, (50,), generator=g, device='cuda')
+    check_scores(host(out[~none][:, cols]), host(picked[~none]),
+                 host(rk.mx4_dequantize(table, rows=cols.to(torch.int32))), F32)
 
 
 @pytest.mark.parametrize('kind', ['f32', 'bf16', 'f16', 'mx4'])

@@ -158,16 +158,20 @@ def test_c_entry_points_refuse():
     refused(d, 0, 1, None, 1, 8, odd, p, p, 8, None)
     refused(d, 0, 1, None, 1, 8, p, p, None, 8, None)
     s = 'alsmi_mx4_scores'
-    refused(s, 1, 1, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None)
-    refused(s, 0, 1, None, 1, p, 8, None, 1, 8, p, p, 1, p, 1, None)
-    refused(s, 0, 2, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None)
-    refused(s, 0, 1, p, 0, p, 8, None, 1, 8, p, p, 0, p, 1, None)
-    refused(s, 0, 2, None, 2, p, 7, None, 1, 8, p, p, 0, p, 1, None)
-    refused(s, 0, 2, None, 2, p, 8, None, 2, 8, p, p, 0, p, 1, None)
-    refused(s, 4, 1, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None)
-    refused(s, 4, 1, None, 1, odd, 8, p, 1, 8, p, p, 0, p, 1, None)
-    refused(s, 0, 1, None, 1, p, 8, None, 1, 8, odd, p, 0, p, 1, None)
-    assert lib.alsmi_mx4_scores(0, 0, None, 0, None, 8, None, 5, 8, None, None, 0, None, 5, None) == 0
+    refused(s, 1, 1, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None, None)
+    refused(s, 0, 1, None, 1, p, 8, None, 1, 8, p, p, 1, p, 1, None, None)
+    refused(s, 0, 2, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None, None)
+    refused(s, 0, 1, p, 0, p, 8, None, 1, 8, p, p, 0, p, 1, None, None)
+    refused(s, 0, 2, None, 2, p, 7, None, 1, 8, p, p, 0, p, 1, None, None)
+    refused(s, 0, 2, None, 2, p, 8, None, 2, 8, p, p, 0, p, 1, None, None)
+    refused(s, 4, 1, None, 1, p, 8, None, 1, 8, p, p, 0, p, 1, None, None)
+    refused(s, 4, 1, None, 1, odd, 8, p, 1, 8, p, p, 0, p, 1, None, None)
+    refused(s, 0, 1, None, 1, p, 8, None, 1, 8, odd, p, 0, p, 1, None, None)
+    assert lib.alsmi_mx4_scores_workspace_bytes(0, 16, 1000, 64) == 0
+    need = lib.alsmi_mx4_scores_workspace_bytes(0, 128, 16384, 640)
+    assert need == 128 * 640 * 2 * 3
+    refused(s, 0, 128, None, 128, p, 640, None, 16384, 640, p, p, 0, p, 16384, None, None)
+    assert lib.alsmi_mx4_scores(0, 0, None, 0, None, 8, None, 5, 8, None, None, 0, None, 5, None, None) == 0
 
     def adjust(dtype=0, scores=p, out=p, **fields):
         a = _lib.Adjust(n_rows=2, n_items=8, ld_scores=8, ld_out=8, repetition_value=1.0)
