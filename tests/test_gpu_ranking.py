@@ -182,7 +182,8 @@ def test_scores_match_definition(m, n, width, kind):
 @pytest.mark.parametrize('m,n,width', [(1, 300001, 64), (3, 540000, 130), (20, 140000, 132),
                                        (1, 70001, 200), (257, 9001, 128), (2048, 2049, 192),
                                        (513, 2000, 2080), (300, 6001, 300), (1000, 2100, 1100),
-                                       (129, 8300, 135), (4000, 3333, 520), (70, 16385, 512)])
+                                       (129, 8300, 135), (4000, 3333, 520), (70, 16385, 512),
+                                       (40, 30001, 256), (90, 9000, 250)])
 def test_scores_large(m, n, width, kind):
     """Sizes that take the long-walk and one-step forms; a strip of items against the definition,
     the rest against another order of the same items."""
