@@ -337,29 +337,42 @@ __global__ __launch_bounds__(256) void topk_list_kernel(KeySource<T, FROM_KEYS> 
 }
 
 // ---- k > 64 --------------------------------------------------------------------------------------
-// The smallest of the k largest keys of a workgroup (THREADS x E keys in registers, all different but
-// for zeros), by digits of at most 11 bits from the top, image first, then the `index_bits` bits
-// in which indices differ (the bits between are ones in every key); 1 if there are no k keys but
-// zeros.
-template <typename K, int BITS, int THREADS, int E>
-__device__ __forceinline__ K kth_key(const K (&key)[E], int k, int index_bits) {
-    constexpr int DIGIT = 11, BINS = 1 << DIGIT, PER = BINS / THREADS, WAVES = THREADS / 64;
-    __shared__ unsigned hist[BINS];
-    __shared__ unsigned wave_sum[WAVES];
-    __shared__ unsigned bin_sh, above_sh, in_bin_sh;
+// Sum over lanes 0 .. lane.
+__device__ __forceinline__ unsigned wave_prefix(unsigned x) {
+    auto add = [&](auto ctrl, auto rows) {
+        x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value,
+                                                   0xf, false);
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // from 1 lane below,
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});  // 2, 4, 8 inside a row
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row ends to rows 1, 3
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // the lower half's end
+    return x;
+}
+
+// The smallest of the k largest keys of a workgroup (THREADS x E keys of at most `bits` bits in
+// registers, all different but for zeros), by digits of 11 bits from the top; 1 if there are no k
+// keys but zeros.  A pass costs its atomics and two barriers: every wave reads the whole histogram
+// and finds the digit by itself (one wave, or sums by thread and prefix sums over the workgroup,
+// with more barriers, took longer), and the other of two histograms is cleared meanwhile.
+template <typename K, int THREADS, int E>
+__device__ __forceinline__ K kth_key(const K (&key)[E], int k, int bits) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    constexpr int DIGIT = 11, BINS = 1 << DIGIT, LANE_BINS = BINS / 64;
+    __shared__ u32x4 hist4[2][BINS / 4];
     const int tid = threadIdx.x, lane = tid & 63;
     K prefix = 0;
     unsigned want = k;
-    for (int high = BITS, low; high > 0; high = low == 32 ? index_bits : low) {
-        // bits [low, high) of the key
-        low = high - DIGIT > 32 ? high - DIGIT : high > 32 ? 32 : high > DIGIT ? high - DIGIT : 0;
-        if (high == index_bits) prefix |= (K)(0xffffffffull >> index_bits << index_bits);
+    for (int i = tid; i < BINS / 4; i += THREADS) hist4[0][i] = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    int turn = 0;
+    for (int high = bits; high > 0; high -= DIGIT, turn ^= 1) {  // bits [low, high) of the keys
+        unsigned *hist = reinterpret_cast<unsigned *>(hist4[turn]);
+        const int low = high > DIGIT ? high - DIGIT : 0;
         const unsigned mask = (1u << (high - low)) - 1u;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) hist[i * THREADS + tid] = 0;
-        __syncthreads();
-        if (tid == 0) bin_sh = BINS;  // no bin yet
-        const K upper = high >= BITS ? (K)0 : ~(K)0 << high;  // (a key of zeros fits no image)
+        const K upper = ~(K)0 << high;
         // scores share their leading bits: a thread adds up a run of equal digits first
         int run_bin = -1;
         unsigned run = 0;
@@ -375,40 +388,33 @@ __device__ __forceinline__ K kth_key(const K (&key)[E], int k, int index_bits) {
             ++run;
         }
         if (run) atomicAdd(&hist[run_bin], run);
+        for (int i = tid; i < BINS / 4; i += THREADS) hist4[turn ^ 1][i] = u32x4{0, 0, 0, 0};
         __syncthreads();
-        // thread t: bins BINS-1 - PER t downwards; keys above them = the sums of the threads before
-        unsigned h[PER], sum = 0;
+        // lane l: the 32 bins below BINS - 32 l (its reads start at another place than its neighbours',
+        // or all lanes would meet in the same banks)
+        unsigned sum = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) sum += h[i] = hist[BINS - 1 - PER * tid - i];
-        unsigned upto = sum;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const unsigned o = __shfl_up(upto, off);
-            if (lane >= off) upto += o;
+        for (int i = 0; i < LANE_BINS / 4; ++i) {
+            const u32x4 h = hist4[turn][(63 - lane) * (LANE_BINS / 4) + ((i + lane) & (LANE_BINS / 4 - 1))];
+            sum += h[0] + h[1] + h[2] + h[3];
         }
-        if (lane == 63) wave_sum[tid >> 6] = upto;
-        __syncthreads();
-        unsigned above = upto - sum;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w)
-            if (w < (tid >> 6)) above += wave_sum[w];
-        if (above < want && above + sum >= want) {
-            int i = 0;
-#pragma unroll
-            for (int s = 0; s < PER - 1; ++s)
-                if (i == s && above + h[s] < want) above += h[s], i = s + 1;
-            bin_sh = BINS - 1 - PER * tid - i;
-            above_sh = above;
-            in_bin_sh = h[0];
-#pragma unroll
-            for (int s = 1; s < PER; ++s)
-                if (i == s) in_bin_sh = h[s];
-        }
-        __syncthreads();
-        if (bin_sh == BINS) return 1;  // there are fewer than k keys but zeros
-        prefix |= (K)bin_sh << low;
-        want -= above_sh;
-        if (in_bin_sh == want) break;  // the whole bin is in
+        unsigned upto = wave_prefix(sum);
+        unsigned long long found = __ballot(upto >= want);
+        if (found == 0) return 1;  // there are fewer than k keys but zeros
+        const int owner = __builtin_ctzll(found);
+        unsigned above = (unsigned)__builtin_amdgcn_readlane((int)(upto - sum), owner);
+        // and the bin among the owner's
+        const int top = BINS - LANE_BINS * owner - 1;
+        const unsigned h = lane < LANE_BINS ? hist[top - lane] : 0u;
+        upto = above + wave_prefix(h);
+        found = __ballot(upto >= want);
+        const int at = __builtin_ctzll(found);
+        above = (unsigned)__builtin_amdgcn_readlane((int)(upto - h), at);
+        const unsigned in_bin = (unsigned)__builtin_amdgcn_readlane((int)h, at);
+        prefix |= (K)(unsigned)(top - at) << low;
+        want -= above;
+        if (in_bin == want) break;  // the whole bin is in
+        __syncthreads();            // (the other histogram is clear, this one read)
     }
     return prefix ? prefix : (K)1;
 }
@@ -442,19 +448,30 @@ __global__ __launch_bounds__(THREADS) void topk_tile_kernel(KeySource<T, FROM_KE
     }
     if (tid == 0) n_kept = 0;
     key_t floor_key = 1;
-    if (src.n - first > k) floor_key = kth_key<key_t, RowKey<T>::BITS, THREADS, E>(key, k, index_bits);
+    if (src.n - first > k) {
+        // without the bits between image and index, which are ones in every key
+        const unsigned index_mask = 0xffffffffu >> (32 - index_bits);
+        auto without = [&](key_t x) { return ((x >> 32) << index_bits) | ((unsigned)x & index_mask); };
+        key_t dense[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j) dense[j] = without(key[j]);
+        const key_t kth =
+            kth_key<key_t, THREADS, E>(dense, k, RowKey<T>::BITS - 32 + index_bits);
+        floor_key = kth == 1 ? kth : ((kth >> index_bits) << 32) | (unsigned)~index_mask |
+                                         ((unsigned)kth & index_mask);
+    }
     __syncthreads();
     key_t *dst = SORT ? sel : kept + (row * tiles + tile) * k;
+    unsigned mine_kept = 0;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        const bool in = key[j] >= floor_key;
-        const unsigned long long m = __ballot(in);
-        if (m == 0) continue;
-        int base = 0;
-        if (lane == 0) base = atomicAdd(&n_kept, (int)__popcll(m));
-        base = __builtin_amdgcn_readfirstlane(base);
-        if (in) dst[base + __popcll(m & ((1ull << lane) - 1ull))] = key[j];
-    }
+    for (int j = 0; j < E; ++j) mine_kept += key[j] >= floor_key;
+    const unsigned upto = wave_prefix(mine_kept);
+    int place = 0;
+    if (lane == 63) place = atomicAdd(&n_kept, (int)upto);
+    place = __builtin_amdgcn_readlane(place, 63) + (int)(upto - mine_kept);
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (key[j] >= floor_key) dst[place++] = key[j];
     __syncthreads();
     const int have = n_kept;
     if constexpr (!SORT) {
