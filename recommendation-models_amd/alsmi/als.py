@@ -440,7 +440,7 @@ class ALS(BaseEstimator):
             held = getattr(self, '_mx4', None)  # quantised once for these item factors
             if held is None or held[0] is not V:
                 held = self._mx4 = (V, ranking.mx4_quantize(V[:, :self.rank]))
-            table, users32 = held[1], U[:, :self.rank].to(torch.float32)
+            table = held[1]
         n = int(d_users.numel())
         items = torch.empty((n, k), dtype=torch.int32, device=device)
         best = torch.empty((n, k), dtype=torch.float32 if catalogue == 'mx4' else U.dtype,
@@ -453,7 +453,11 @@ class ALS(BaseEstimator):
             hi = min(n, lo + block)
             part = d_users[lo:hi]
             if catalogue == 'mx4':
-                s = ranking.mx4_scores(users32, table, rows=part)
+                if U.dtype == torch.float32:
+                    s = ranking.mx4_scores(U[:, :self.rank], table, rows=part)
+                else:
+                    s = ranking.mx4_scores(U.index_select(0, part)[:, :self.rank].to(torch.float32),
+                                           table)
             else:
                 s = dev.score_items(self.rank, part, U, V)
             kw = {}

@@ -339,21 +339,24 @@ def topk_items(rank, users, row_table, col_table, k, max_workspace_bytes=1 << 30
 def score_items(rank, users, row_table, col_table, out=None):
     """The dense score block [n, n_items] of `users` (int32 device tensor) that ``topk_items``
     ranks: <row_table[users[p]], col_table[i]>, for callers that change the scores before they
-    select (src/als.py:347-364 for a block of users)."""
+    select (src/als.py:347-364 for a block of users).  `users` must be rows of `row_table`: the
+    ids are not looked at."""
     device = row_table.device
     n_sel, n_items = int(users.numel()), int(col_table.shape[0])
-    if users.dtype != torch.int32:
-        raise ValueError('users must be an int32 device tensor')
-    if row_table.dtype != col_table.dtype:
-        raise ValueError('factor tables must share a dtype')
+    if users.dtype != torch.int32 or users.device != device or not users.is_contiguous():
+        raise ValueError('users must be a contiguous int32 tensor on the device of the tables')
+    if row_table.dtype != col_table.dtype or col_table.device != device:
+        raise ValueError('factor tables must share a dtype and a device')
     np_dtype = np.float32 if row_table.dtype == torch.float32 else np.float64
     if out is None:
         out = torch.empty((n_sel, n_items), dtype=row_table.dtype, device=device)
     elif out.dtype != row_table.dtype or tuple(out.shape) != (n_sel, n_items) or \
-            not out.is_contiguous():
-        raise ValueError('out must be contiguous [%d x %d] %s' % (n_sel, n_items, row_table.dtype))
+            out.device != device or not out.is_contiguous():
+        raise ValueError('out must be contiguous [%d x %d] %s on the device of the tables'
+                         % (n_sel, n_items, row_table.dtype))
     ws = torch.empty(4, dtype=torch.int32, device=device)
-    _lib.check(_lib.load().alsmi_score_items(
-        _lib.dtype_code(np_dtype), int(rank), n_sel, _ptr(users), _ptr(row_table), _ptr(col_table),
-        n_items, _ptr(out), _ptr(ws), _stream()), 'alsmi_score_items')
+    with torch.cuda.device(device):
+        _lib.check(_lib.load().alsmi_score_items(
+            _lib.dtype_code(np_dtype), int(rank), n_sel, _ptr(users), _ptr(row_table),
+            _ptr(col_table), n_items, _ptr(out), _ptr(ws), _stream()), 'alsmi_score_items')
     return out

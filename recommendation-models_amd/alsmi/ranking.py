@@ -90,14 +90,17 @@ def _call(device, name, *args):
         _lib.check(status, name)
 
 
+def _span(t):
+    """First and last byte address of a tensor with no negative strides."""
+    size = sum((n - 1) * step for n, step in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + size * t.element_size()
+
+
 def _overlap(a, b):
-    """Whether the memory spans of two 2-D tensors meet."""
-    def span(t):
-        size = ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size()
-        return t.data_ptr(), t.data_ptr() + size
+    """Whether the memory spans of two tensors meet."""
     if a.numel() == 0 or b.numel() == 0:
         return False
-    (a0, a1), (b0, b1) = span(a), span(b)
+    (a0, a1), (b0, b1) = _span(a), _span(b)
     return a0 < b1 and b0 < a1
 
 
@@ -108,7 +111,7 @@ def _result(name, out, shape, dtype, device, *sources):
     ld = _matrix(name, out, (dtype,))
     if tuple(out.shape) != tuple(shape):
         raise ValueError('%s must have shape %s, got %s' % (name, tuple(shape), tuple(out.shape)))
-    if any(_overlap(out, s) for s in sources):
+    if any(s is not None and _overlap(out, s) for s in sources):
         raise ValueError('%s must not overlap the operands' % name)
     return out, ld
 
@@ -186,7 +189,8 @@ def mx4_dequantize(table, dtype=torch.float32, rows=None, out=None):
     if rows is not None:
         _vector('rows', rows, torch.int32)
     n = len(table) if rows is None else rows.numel()
-    out, ld = _result('out', out, (n, table.width), dtype, table.device, table.codes, table.scales)
+    out, ld = _result('out', out, (n, table.width), dtype, table.device, table.codes, table.scales,
+                      rows)
     device = _device(table.codes, table.scales, rows, out)
     _call(device, 'alsmi_mx4_dequantize', _CODES[dtype], n, _p(rows), len(table), table.width,
           _p(table.codes), _p(table.scales), _p(out), ld)
@@ -220,7 +224,8 @@ def mx4_scores(a, table, rows=None, out_dtype=None, out=None):
     m = a.shape[0] if rows is None else rows.numel()
     if m and a.shape[0] == 0:
         raise ValueError('rows of an empty a')
-    out, ldo = _result('out', out, (m, len(table)), out_dtype, table.device, data, table.codes)
+    out, ldo = _result('out', out, (m, len(table)), out_dtype, table.device, data, a_scales, rows,
+                       table.codes, table.scales)
     device = _device(table.codes, table.scales, data, a_scales, rows, out)
     n, width = table.shape
     size = _lib.load().alsmi_mx4_scores_workspace_bytes(code, m, n, width)
@@ -344,7 +349,8 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
     elif mask_rows is not None:
         raise ValueError('mask_rows needs a mask')
     if out is not scores:
-        out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores.device, scores)
+        out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores.device, scores,
+                                  *kept.values())
     else:
         args.ld_out = ld
     device = _device(scores, out, *kept.values())

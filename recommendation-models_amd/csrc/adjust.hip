@@ -14,6 +14,8 @@
 #include "alsmi_common.h"
 #include "elem.h"
 
+#include <algorithm>
+
 namespace alsmi {
 
 constexpr int ADJ_THREADS = 256;
@@ -65,7 +67,7 @@ __device__ __forceinline__ double keep(double x, unsigned bits, int i) {
 // words (looking at all of them cost 42 us instead of 37 there).
 template <typename T>
 __global__ __launch_bounds__(ADJ_THREADS) void adjust_kernel(alsmi_adjust a, const T *scores, T *out,
-                                                             unsigned tiles) {
+                                                             unsigned tiles, unsigned first_row) {
     typedef typename Elem<T>::wide W;
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
     __shared__ unsigned seen[ADJ_TILE / 32], biased[ADJ_TILE / 32];
@@ -73,7 +75,7 @@ __global__ __launch_bounds__(ADJ_THREADS) void adjust_kernel(alsmi_adjust a, con
     unsigned *count = reinterpret_cast<unsigned *>(count4), *last = reinterpret_cast<unsigned *>(last4);
     const unsigned tid = threadIdx.x;
     const unsigned r32 = blockIdx.x / tiles;
-    const int64_t row = r32;
+    const int64_t row = (int64_t)first_row + r32;
     const unsigned first = (blockIdx.x - r32 * tiles) * ADJ_TILE;
     const unsigned n_items = (unsigned)a.n_items;
     const unsigned in_tile = n_items - first < ADJ_TILE ? n_items - first : ADJ_TILE;
@@ -166,10 +168,14 @@ __global__ __launch_bounds__(ADJ_THREADS) void adjust_kernel(alsmi_adjust a, con
 template <typename T>
 static int run_adjust(const alsmi_adjust &a, const void *scores, void *out, hipStream_t st) {
     const int64_t tiles = (a.n_items + ADJ_TILE - 1) / ADJ_TILE;
-    ALSMI_REQUIRE(tiles * a.n_rows <= INT32_MAX, "alsmi_adjust_scores: too many rows x items");
-    hipLaunchKernelGGL((adjust_kernel<T>), dim3((unsigned)(tiles * a.n_rows)), dim3(ADJ_THREADS), 0, st, a,
-                       static_cast<const T *>(scores), static_cast<T *>(out), (unsigned)tiles);
-    ALSMI_HIP_CHECK(hipGetLastError());
+    const int64_t most = std::max<int64_t>(1, ((int64_t)1 << 23) / tiles);  // (under 2^32 threads a launch)
+    for (int64_t lo = 0; lo < a.n_rows; lo += most) {
+        const int64_t rows = std::min(a.n_rows - lo, most);
+        hipLaunchKernelGGL((adjust_kernel<T>), dim3((unsigned)(tiles * rows)), dim3(ADJ_THREADS), 0, st, a,
+                           static_cast<const T *>(scores), static_cast<T *>(out), (unsigned)tiles,
+                           (unsigned)lo);
+        ALSMI_HIP_CHECK(hipGetLastError());
+    }
     return ALSMI_OK;
 }
 

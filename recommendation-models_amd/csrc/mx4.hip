@@ -8,6 +8,7 @@
 #include "alsmi_common.h"
 #include "elem.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace alsmi {
@@ -596,7 +597,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void mx4_split_kernel(Rows rows, const T *__restrict__ a, int width,
                                                         int units, u32x4 *__restrict__ planes) {
     constexpr int NP = Parts<T>::N;
-    const int64_t i = blockIdx.x;  // one row per workgroup and turn, eight elements per thread
+    const int64_t i = blockIdx.x;  // one row per workgroup, eight elements per thread and turn
     const int64_t r = rows.of(i);
     for (int u = threadIdx.x; u < units; u += 256) {
         float x[8];
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(256) void mx4_split_kernel(Rows rows, const T *__re
 }
 
 template <typename TO, int NP>
-__global__ __launch_bounds__(256, 2) void mx4_scores_split_kernel(const u32x4 *__restrict__ planes,
+__global__ __launch_bounds__(256, NP > 2 ? 1 : 2) void mx4_scores_split_kernel(const u32x4 *__restrict__ planes,
                                                                   const uint8_t *__restrict__ codes,
                                                                   const uint8_t *__restrict__ scales,
                                                                   int nb, ScoreStore o, int row_tiles) {
@@ -1089,7 +1090,6 @@ static int launch_narrow(const Rows &rows, const void *a, int width, const uint8
     turns = turns < 1 ? 1 : (turns > 16 ? 16 : turns);
     const int64_t tpw = turns * NT;
     const int64_t blocks = (n_tiles + 4 * tpw - 1) / (4 * tpw) * groups;
-    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
     hipLaunchKernelGGL((mx4_scores_narrow_kernel<T, TO, NBL, UT, NT>), dim3((unsigned)blocks), dim3(256), 0,
                        st, rows, static_cast<const T *>(a), width, codes, scales, nb, o, (int)groups,
                        (int)tpw);
@@ -1103,7 +1103,6 @@ static int launch_wide(const Rows &rows, const void *a, int width, const uint8_t
     const int64_t groups = (rows.n_sel + 16 * MT - 1) / (16 * MT);
     const int64_t per = 16 * NT * (KW == 1 ? 4 : 1);
     const int64_t blocks = (o.n_items + per - 1) / per * groups;
-    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
     hipLaunchKernelGGL((mx4_scores_wide_kernel<T, TO, MT, NT, KW>), dim3((unsigned)blocks), dim3(256), 0,
                        st, rows, static_cast<const T *>(a), width, codes, scales, nb, o, (int)groups);
     ALSMI_HIP_CHECK(hipGetLastError());
@@ -1120,7 +1119,6 @@ static int launch_both_narrow(const Rows &rows, const void *a, const uint8_t *a_
     turns = turns < 1 ? 1 : (turns > 16 ? 16 : turns);
     const int64_t tpw = turns * NT;
     const int64_t blocks = (n_tiles + 4 * tpw - 1) / (4 * tpw) * groups;
-    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
     hipLaunchKernelGGL((mx4_scores_both_narrow_kernel<TO, NS, UT, NT>), dim3((unsigned)blocks), dim3(256),
                        0, st, rows, static_cast<const uint8_t *>(a), a_scales, codes, scales, nb, o,
                        (int)groups, (int)tpw);
@@ -1134,7 +1132,6 @@ static int launch_both(const Rows &rows, const void *a, const uint8_t *a_scales,
     const int64_t groups = (rows.n_sel + 16 * MT - 1) / (16 * MT);
     const int64_t per = 16 * NT * (KW == 1 ? 4 : 1);
     const int64_t blocks = (o.n_items + per - 1) / per * groups;
-    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
     hipLaunchKernelGGL((mx4_scores_both_kernel<TO, MT, NT, KW>), dim3((unsigned)blocks), dim3(256), 0, st, rows,
                        static_cast<const uint8_t *>(a), a_scales, codes, scales, nb, o, (int)groups);
     ALSMI_HIP_CHECK(hipGetLastError());
@@ -1147,7 +1144,6 @@ static int launch_tiled(const Rows &rows, const void *a, const uint8_t *a_scales
     constexpr int BM = WM * MT * 16, BN = WN * NT * 16;
     const int64_t row_tiles = (rows.n_sel + BM - 1) / BM;
     const int64_t blocks = (o.n_items + BN - 1) / BN * row_tiles;
-    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
     hipLaunchKernelGGL((mx4_scores_tiled_kernel<TO, WM, WN, MT, NT>), dim3((unsigned)blocks),
                        dim3(64 * WM * WN), 0, st, rows, static_cast<const uint8_t *>(a), a_scales, codes,
                        scales, nb, o, (int)row_tiles);
@@ -1188,6 +1184,16 @@ static bool splits(int64_t n_sel, int64_t n_items, int nb) {
 static int64_t split_bytes(int64_t n_sel, int nb, int parts) {
     return n_sel * ((nb + 3) / 4) * 256 * parts;
 }
+static int parts_of(int dtype) {
+    return dtype == ALSMI_F32 ? 3 : dtype == ALSMI_F16 ? 2 : dtype == ALSMI_BF16 ? 1 : 0;
+}
+// Rows that a product takes at once: what a launch of fewer than 2^32 threads covers whatever the
+// items, or where they are split first, whole tiles of rows whose parts take 256 MiB.
+static int64_t batch_rows(int dtype, int64_t n_sel, int64_t n_items, int nb) {
+    if (dtype == ALSMI_MX4 || !splits(n_sel, n_items, nb)) return (int64_t)1 << 22;
+    const int64_t fit = ((int64_t)256 << 20) / split_bytes(1, nb, parts_of(dtype));
+    return std::max<int64_t>(WT_ROWS, fit / WT_ROWS * WT_ROWS);
+}
 
 template <typename T, typename TO>
 static int launch_split(const Rows &rows, const void *a, int width, const uint8_t *codes,
@@ -1196,7 +1202,6 @@ static int launch_split(const Rows &rows, const void *a, int width, const uint8_
     u32x4 *planes = static_cast<u32x4 *>(workspace);
     const int64_t row_tiles = (rows.n_sel + WT_ROWS - 1) / WT_ROWS;
     const int64_t blocks = (o.n_items + WT_ITEMS - 1) / WT_ITEMS * row_tiles;
-    ALSMI_REQUIRE(blocks <= INT32_MAX, "alsmi_mx4_scores: too many rows x items");
     hipLaunchKernelGGL((mx4_split_kernel<T>), dim3((unsigned)rows.n_sel), dim3(256), 0, st, rows,
                        static_cast<const T *>(a), width, (nb + 3) / 4 * 16, planes);
     ALSMI_HIP_CHECK(hipGetLastError());
@@ -1208,9 +1213,9 @@ static int launch_split(const Rows &rows, const void *a, int width, const uint8_
 
 template <typename T, typename TO>
 static int run_scores(const Rows &rows, const void *a, int width, const uint8_t *codes,
-                      const uint8_t *scales, int nb, const ScoreStore &o, void *workspace,
+                      const uint8_t *scales, int nb, const ScoreStore &o, bool split, void *workspace,
                       hipStream_t st) {
-    if (splits(rows.n_sel, o.n_items, nb) && (uintptr_t)codes % 16 == 0)
+    if (split)
         return launch_split<T, TO>(rows, a, width, codes, scales, nb, o, workspace, st);
     const bool one = rows.n_sel <= 16;
     if (nb == 1)
@@ -1315,9 +1320,9 @@ int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t 
 size_t alsmi_mx4_scores_workspace_bytes(int dtype, int64_t n_sel, int64_t n_items, int64_t width) {
     using namespace alsmi;
     if (n_sel < 0 || n_items < 0 || width < 1 || width > MX4_MAX_WIDTH) return 0;
-    const int parts = dtype == ALSMI_F32 ? 3 : dtype == ALSMI_F16 ? 2 : dtype == ALSMI_BF16 ? 1 : 0;
     const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
-    return splits(n_sel, n_items, nb) ? (size_t)split_bytes(n_sel, nb, parts) : 0;
+    if (!splits(n_sel, n_items, nb)) return 0;
+    return (size_t)split_bytes(std::min(n_sel, batch_rows(dtype, n_sel, n_items, nb)), nb, parts_of(dtype));
 }
 
 int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, const void *a,
@@ -1351,22 +1356,38 @@ int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_ro
     ALSMI_REQUIRE(alsmi_mx4_scores_workspace_bytes(dtype, n_sel, n_items, width) == 0 ||
                       (workspace && (uintptr_t)workspace % 16 == 0),
                   "alsmi_mx4_scores: needs a workspace aligned to 16 bytes");
-    const Rows r = {n_sel, n_rows, lda, rows};
-    const ScoreStore o = {out, ldo, n_sel, n_items};
-#define ALSMI_CASE(TO)                                                                               \
-    do {                                                                                             \
-        if (dtype == ALSMI_F32)                                                                      \
-            return run_scores<float, TO>(r, a, (int)width, codes, scales, nb, o, workspace, st);     \
-        if (dtype == ALSMI_F16)                                                                      \
-            return run_scores<_Float16, TO>(r, a, (int)width, codes, scales, nb, o, workspace, st);             \
-        if (dtype == ALSMI_BF16)                                                                     \
-            return run_scores<__bf16, TO>(r, a, (int)width, codes, scales, nb, o, workspace, st);               \
-        return run_both<TO>(r, a, a_scales, codes, scales, nb, o, st);                              \
+    const bool split = splits(n_sel, n_items, nb) && (uintptr_t)codes % 16 == 0;
+    const int64_t most = batch_rows(dtype, n_sel, n_items, nb);
+    const int64_t out_size = out_dtype == ALSMI_F32 ? 4 : 2;
+    // bytes of a row of the activations
+    const int64_t a_row = dtype == ALSMI_MX4 ? 16 * nb : lda * (dtype == ALSMI_F32 ? 4 : 2);
+    for (int64_t lo = 0; lo < n_sel; lo += most) {
+        const int64_t n = std::min(n_sel - lo, most), skip = rows ? 0 : lo;
+        const Rows r = {n, n_rows - skip, lda, rows ? rows + lo : nullptr};
+        const ScoreStore o = {static_cast<char *>(out) + lo * ldo * out_size, ldo, n, n_items};
+        const void *from = static_cast<const char *>(a) + skip * a_row;
+        const uint8_t *from_scales = a_scales ? a_scales + skip * nb : nullptr;
+        int status = ALSMI_OK;
+#define ALSMI_CASE(TO)                                                                                  \
+    do {                                                                                                \
+        if (dtype == ALSMI_F32)                                                                         \
+            status = run_scores<float, TO>(r, from, (int)width, codes, scales, nb, o, split, workspace, st); \
+        else if (dtype == ALSMI_F16)                                                                    \
+            status =                                                                                    \
+                run_scores<_Float16, TO>(r, from, (int)width, codes, scales, nb, o, split, workspace, st); \
+        else if (dtype == ALSMI_BF16)                                                                   \
+            status =                                                                                    \
+                run_scores<__bf16, TO>(r, from, (int)width, codes, scales, nb, o, split, workspace, st); \
+        else                                                                                            \
+            status = run_both<TO>(r, from, from_scales, codes, scales, nb, o, st);                      \
     } while (0)
-    if (out_dtype == ALSMI_F32) ALSMI_CASE(float);
-    else if (out_dtype == ALSMI_BF16) ALSMI_CASE(__bf16);
-    else ALSMI_CASE(_Float16);
+        if (out_dtype == ALSMI_F32) ALSMI_CASE(float);
+        else if (out_dtype == ALSMI_BF16) ALSMI_CASE(__bf16);
+        else ALSMI_CASE(_Float16);
 #undef ALSMI_CASE
+        if (status != ALSMI_OK) return status;
+    }
+    return ALSMI_OK;
 }
 
 }  // extern "C"

@@ -637,3 +637,148 @@ def test_recommend_with_exclusion_bias_mask_and_quantised_items(dtype, monkeypat
     assert best not in als.recommend([0], k, exclude_seen=True)[0]
     with pytest.raises(ValueError):
         als.recommend([0], m + 1, exclude_seen=True)
+
+
+# ------------------------------------------------------------------------- the ends of the range
+def test_topk_of_rows_of_the_lowest_key():
+    """Rows of the one score that ranks below all others (every bit set), of as many items as an
+    index has room for: the last two differ from "no score" by their index alone."""
+    for n, k in ((128, 127), (128, 65), (1024, 1023), (16384, 1024), (32768, 1024), (65536, 700)):
+        for dtype, whole in ((F32, torch.int32), (BF16, torch.int16), (F64, torch.int64)):
+            s = torch.full((2, n), -1, dtype=whole, device='cuda').view(dtype)
+            s[1, n - 1], s[1, n // 2] = 1.0, 2.0
+            items, best = rk.topk_rows(s, k)
+            assert torch.equal(items[0].cpu(), torch.arange(k, dtype=torch.int32))
+            want = torch.tensor([n // 2, n - 1] + [i for i in range(k) if i != n // 2][:k - 2])
+            assert torch.equal(items[1].cpu(), want.to(torch.int32))
+            assert bool((best[0].view(whole) == -1).all()) and best[1, :2].tolist() == [2.0, 1.0]
+
+
+@pytest.mark.parametrize('n,m,k', [(2 ** 23 + 5, 3, 2), (2 ** 21 + 3, 66, 65), (70001, 1000, 64),
+                                   (70001, 1024, 1)])
+def test_topk_of_very_many_short_rows(n, m, k):
+    """More rows than one launch has room for."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(m)
+    s = torch.randint(-40, 40, (n, m), generator=g, device='cuda', dtype=torch.int8).to(BF16)
+    items, best = rk.topk_rows(s, k)
+    for lo, hi in ((0, 1000), (2 ** 21 - 500, 2 ** 21 + 500), (n - 1000, n)):
+        want, order = torch.sort(s[lo:hi], dim=1, descending=True, stable=True)
+        assert torch.equal(items[lo:hi], order[:, :k].to(torch.int32))
+        assert torch.equal(best[lo:hi], want[:, :k])
+    assert torch.equal(best, s.gather(1, items.to(torch.int64)))
+    assert bool((best[:, :-1] >= best[:, 1:]).all()) if k > 1 else True
+
+
+def test_adjust_very_many_short_rows():
+    n, m = 2 ** 23 + 9, 3
+    g = torch.Generator(device='cuda')
+    g.manual_seed(3)
+    s = torch.rand(n, m, generator=g, device='cuda')
+    ids = torch.randint(-1, m, (n,), generator=g, device='cuda', dtype=torch.int32)
+    ptr = torch.arange(n + 1, device='cuda')
+    mask_rows = torch.randint(-1, 2, (n,), generator=g, device='cuda', dtype=torch.int32)
+    mask = gpu(rk.pack_mask(np.array([[1, 1, 0], [1, 0, 1]], dtype=bool)))
+    got = rk.adjust_scores(s, history=(ptr, ids), exclude=True, mask=mask, mask_rows=mask_rows)
+    gone = torch.arange(m, device='cuda') == ids[:, None]
+    gone[:, 2] |= mask_rows == 0
+    gone[:, 1] |= mask_rows == 1
+    assert torch.equal(got, s.masked_fill(gone, -INF))
+
+
+@pytest.mark.parametrize('kind', ['f32', 'f16', 'mx4'])
+def test_scores_of_very_many_rows(kind):
+    n, m, width = 2 ** 22 + 70, 3, 5
+    g = torch.Generator(device='cuda')
+    g.manual_seed(4)
+    table = rk.mx4_quantize(torch.randn(m, width, generator=g, device='cuda'))
+    a = torch.randn(n, width, generator=g, device='cuda')
+    at = rk.mx4_quantize(a) if kind == 'mx4' else a.to({'f32': F32, 'f16': F16}[kind])
+    av = rk.mx4_dequantize(at, F64) if kind == 'mx4' else at.to(F64)
+    values = rk.mx4_dequantize(table, F64)
+    order = torch.randperm(n, generator=g, device='cuda').to(torch.int32)
+    order[n - 3] = n
+    for rows in (None, order):
+        got = rk.mx4_scores(at, table, rows=rows, out_dtype=F32).to(F64)
+        if rows is not None:
+            assert bool(torch.isnan(got[n - 3]).all())
+            got[n - 3] = 0
+            rows[n - 3] = 0
+        x = av if rows is None else av[rows.to(torch.int64)]
+        if rows is not None:
+            x[n - 3] = 0
+        tol = 3 * width * 2.0 ** -23 * (x.abs() @ values.abs().T) + 2.0 ** -126
+        assert bool(((got - x @ values.T).abs() <= tol).all())
+
+
+@pytest.mark.parametrize('kind,m', [('f32', 700), ('f16', 1100)])
+def test_scores_of_very_long_rows(kind, m):
+    """Activations whose parts are split in more than one batch of rows; the first rows against the
+    definition, all against their own values for one item picked out of the batch."""
+    n, width = 2800, 65536
+    g = torch.Generator(device='cuda')
+    g.manual_seed(m)
+    table = rk.mx4_quantize(torch.randn(n, width, generator=g, device='cuda'))
+    a = torch.randn(m, width, generator=g, device='cuda').to({'f32': F32, 'f16': F16}[kind])
+    got = rk.mx4_scores(a, table, out_dtype=F32).to(F64)
+    values = rk.mx4_dequantize(table, F64)
+    x = a.to(F64)
+    tol = 3 * width * 2.0 ** -23 * (x.abs() @ values.abs().T)
+    assert bool(((got - x @ values.T).abs() <= tol).all())
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'mx4'])
+@pytest.mark.parametrize('m,n,width', [(300, 20000, 544), (300, 9000, 64), (2, 9000, 300)])
+def test_scores_of_codes_at_any_word(m, n, width, kind):
+    """Codes aligned to four bytes and no more."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(width)
+
+    def shifted(t):
+        flat = torch.empty(t.codes.numel() + 4, dtype=torch.uint8, device='cuda')
+        flat[4:] = t.codes.view(-1)
+        return rk.Mx4Table(flat[4:].view(t.codes.shape), t.scales, t.width)
+    table = rk.mx4_quantize(torch.randn(n, width, generator=g, device='cuda'))
+    a = torch.randn(m, width, generator=g, device='cuda')
+    at = shifted(rk.mx4_quantize(a)) if kind == 'mx4' else a.to({'f32': F32, 'bf16': BF16}[kind])
+    av = host(rk.mx4_dequantize(at)) if kind == 'mx4' else host(at)
+    got = rk.mx4_scores(at, shifted(table), out_dtype=F32)
+    check_scores(host(got), av, host(rk.mx4_dequantize(table)), F32)
+
+
+def test_offsets_past_32_bits():
+    """Blocks of scores of more than 2^31 elements, a table of more than 2^32 bytes of codes: their last
+    rows are those of the same rows by themselves."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(1)
+    n, m = 70000, 32768
+    table = rk.mx4_quantize(torch.randn(m, 32, generator=g, device='cuda'))
+    a = torch.randn(n, 32, generator=g, device='cuda').to(BF16)
+    s = rk.mx4_scores(a, table)
+    tail = rk.mx4_scores(a[-200:], table)
+    assert torch.equal(s[-200:], tail)
+    ids = torch.randint(0, m, (n * 4,), generator=g, device='cuda', dtype=torch.int32)
+    ptr = torch.arange(0, 4 * n + 1, 4, device='cuda')
+    rk.adjust_scores(s, history=(ptr, ids), exclude=True, out=s)
+    rk.adjust_scores(tail, history=(ptr[-201:].clone(), ids), exclude=True, out=tail)
+    assert torch.equal(s[-200:], tail)
+    for k in (10, 100):
+        items, best = rk.topk_rows(s, k)
+        items1, best1 = rk.topk_rows(tail, k)
+        assert torch.equal(items[-200:], items1) and torch.equal(best[-200:], best1)
+    del s, tail
+    n, width = 262144 + 100, 32800
+    x = torch.zeros(n, width, dtype=BF16, device='cuda')
+    x[-100:] = torch.randn(100, width, generator=g, device='cuda')
+    table, last = rk.mx4_quantize(x), rk.mx4_quantize(x[-100:])
+    assert torch.equal(table.codes[-100:], last.codes)
+    assert torch.equal(table.scales[-100:], last.scales)
+    ids = torch.arange(n - 100, n, device='cuda', dtype=torch.int32)
+    assert torch.equal(rk.mx4_dequantize(table, BF16, rows=ids), rk.mx4_dequantize(last, BF16))
+    rk.mx4_dequantize(table, BF16, out=x)
+    assert torch.equal(x[-100:], rk.mx4_dequantize(last, BF16))
+    a, values = host(x[-3:]), host(x[-100:])
+    check_scores(host(rk.mx4_scores(x[-3:], table, out_dtype=F32)[:, -100:]), a, values, F32)
+    check_scores(host(rk.mx4_scores(table, last, rows=ids[-3:])), a, values, F32)
+    many = torch.cat((ids, ids, ids))
+    check_scores(host(rk.mx4_scores(table, last, rows=many)), np.tile(values, (3, 1)), values, F32)

@@ -215,3 +215,30 @@ def test_recommend_refuses():
             als.recommend([0, 1], k=2, **kw)
     with pytest.raises(IndexError):
         als.recommend([4], k=2, exclude_seen=True)
+
+
+def test_output_over_any_operand_is_refused():
+    flat = torch.zeros(4096, dtype=torch.uint8)
+    ids = flat[:8].view(torch.int32)
+    t = rk.Mx4Table(torch.zeros(2, 32, dtype=torch.uint8), flat[64:68].view(2, 2), 40)
+    over = lambda n: flat[:16 * n * 4].view(torch.float32)
+    with pytest.raises(ValueError, match='overlap'):
+        rk.mx4_dequantize(t, rows=ids, out=over(5).view(2, 40))
+    with pytest.raises(ValueError, match='overlap'):
+        rk.mx4_scores(torch.zeros(2, 40), t, out=flat[64:80].view(torch.float32).view(2, 2))
+    with pytest.raises(ValueError, match='overlap'):
+        rk.mx4_scores(torch.zeros(2, 40), t, rows=ids, out=flat[:16].view(torch.float32).view(2, 2))
+    with pytest.raises(ValueError, match='overlap'):
+        rk.adjust_scores(torch.zeros(1, 4), item_bias=flat[:16].view(torch.float32),
+                         out=flat[8:24].view(torch.float32).view(1, 4))
+
+
+def test_score_items_refuses():
+    from alsmi import device as dev
+    U, V = torch.zeros(5, 16), torch.zeros(7, 16)
+    users = torch.zeros(4, dtype=torch.int32)
+    for bad in ((users.long(), U, V), (users[::2], U, V), (users, U, V.double())):
+        with pytest.raises(ValueError):
+            dev.score_items(3, *bad)
+    with pytest.raises(ValueError):
+        dev.score_items(3, users, U, V, out=torch.zeros(4, 8))
