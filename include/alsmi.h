@@ -182,7 +182,8 @@ int alsmi_topk_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
 
 /* The dense score block that alsmi_topk_items ranks: out [n_sel x n_items] of dtype,
  * out[p, i] = <user_factors[users[p]], item_factors[i]>, by the same kernels (ALSMI_F32: scaled fp16
- * split, fp32 accuracy).  For callers that change the scores before they select from them.
+ * split, fp32 accuracy).  For callers that change the scores before they select from them.  As there
+ * users[] must be rows of user_factors: the ids are not looked at.
  * workspace: 16 bytes, aligned to 4. */
 int alsmi_score_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
                       const void *user_factors, const void *item_factors, int64_t n_items,
@@ -216,7 +217,8 @@ int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t 
  * F16 or BF16 (every product exact, fp32 sums), or with ALSMI_MX4 is a table's codes and a_scales
  * its scales (a_scales is ignored otherwise).  rows as in alsmi_mx4_dequantize: a row of NaN where
  * there is no such row.  workspace: alsmi_mx4_scores_workspace_bytes() bytes, aligned to 16 (large
- * products of float activations split them there first); may be NULL where that is 0. */
+ * products of float activations split them there first, 256 MiB at a time or 128 rows); may be
+ * NULL where that is 0. */
 size_t alsmi_mx4_scores_workspace_bytes(int dtype, int64_t n_sel, int64_t n_items, int64_t width);
 int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, const void *a,
                      int64_t ld_a, const uint8_t *a_scales, int64_t n_items, int64_t width,
@@ -234,10 +236,10 @@ int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_ro
  * Any pointer may be NULL: no history / bias list / item bias / mask.  repetition, frequency and
  * presence are [n_rows] fp32 arrays, or NULL for the *_value fields.  The history of row r is list
  * history_rows[r] of the n_history_rows lists (list r where history_rows is NULL; none where it is
- * outside), the mask of row r row mask_rows[r] (where mask_rows is NULL row r, or the
- * only one; a negative id: no mask; one past the masks: nothing is on offer).  List r is entries [ptr[r], ptr[r+1]) of the ids;
- * ids outside 0 .. n_items-1 are skipped, so lists may be padded.  Lists need no order and may
- * repeat an id.  repetition > 0. */
+ * outside), the mask of row r row mask_rows[r] (where mask_rows is NULL row r, or the only one; a
+ * negative id: no mask; one past the masks: nothing is on offer).  List r is entries [ptr[r],
+ * ptr[r+1]) of the ids; ids outside 0 .. n_items-1 are skipped, so lists may be padded.  Lists need
+ * no order and may repeat an id.  repetition > 0. */
 typedef struct alsmi_adjust {
     int64_t n_rows, n_items, ld_scores, ld_out;
     const int64_t *history_ptr;

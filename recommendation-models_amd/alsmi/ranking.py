@@ -22,9 +22,12 @@ from . import _lib
 _CODES = {torch.float32: _lib.F32, torch.float64: _lib.F64, torch.float16: _lib.F16,
           torch.bfloat16: _lib.BF16}
 _FLOATS = tuple(_CODES)
-# the current stream's handle without a Stream object around it (a microsecond of a small call)
+# A small call is mostly its host time, so what every call does is kept short: the current device and
+# the current stream's handle without the objects around them, entry points looked up once.
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
+_entry = {}
 _NARROW = (torch.float32, torch.float16, torch.bfloat16)
 BLOCK = 32
 MAX_K = 1024
@@ -33,7 +36,7 @@ MAX_WIDTH = 1 << 20
 
 def _matrix(name, t, dtypes):
     """Row stride of a 2-D tensor of one of `dtypes` with unit stride inside a row."""
-    if not torch.is_tensor(t) or t.dim() != 2:
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise ValueError('%s must be a 2-D tensor' % name)
     if t.dtype not in dtypes:
         raise ValueError('%s must be one of %s, got %s'
@@ -53,7 +56,8 @@ def _matrix(name, t, dtypes):
 
 
 def _vector(name, t, dtype, size=None):
-    if not torch.is_tensor(t) or t.dim() != 1 or t.dtype != dtype or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dim() != 1 or t.dtype != dtype or \
+            not t.is_contiguous():
         raise ValueError('%s must be a contiguous 1-D %s tensor' % (name, dtype))
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError('%s requires a gradient, which this operator does not give; detach it'
@@ -79,9 +83,11 @@ def _p(t):
 
 def _call(device, name, *args):
     """Enqueue an entry point on the current stream of `device`."""
-    fn = getattr(_lib.load(), name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_lib.load(), name)
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
@@ -230,8 +236,9 @@ def mx4_scores(a, table, rows=None, out_dtype=None, out=None):
     n, width = table.shape
     size = _lib.load().alsmi_mx4_scores_workspace_bytes(code, m, n, width)
     ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _call(device, 'alsmi_mx4_scores', code, m, _p(rows), a.shape[0], _p(data), ld, _p(a_scales), n,
-          width, _p(table.codes), _p(table.scales), _CODES[out_dtype], _p(out), ldo, _p(ws))
+    _call(device, 'alsmi_mx4_scores', code, m, _p(rows), a.shape[0], data.data_ptr(), ld,
+          _p(a_scales), n, width, table.codes.data_ptr(), table.scales.data_ptr(),
+          _CODES[out_dtype], out.data_ptr(), ldo, _p(ws))
     return out
 
 
@@ -262,18 +269,18 @@ def _lists(name, lists, n_values):
     return lists[0].numel() - 1
 
 
-def _penalty(name, value, n_rows, args):
-    """A penalty as a per-row array or one number in the argument block; the array or None."""
-    if torch.is_tensor(value):
+def _penalty(name, value, n_rows, args, kept):
+    """A penalty in the argument block, as a per-row array or one number."""
+    if isinstance(value, torch.Tensor):
         _vector(name, value, torch.float32, n_rows)
-        setattr(args, name, _p(value))
-        return value
+        kept.append(value)
+        setattr(args, name, value.data_ptr())
+        return
     value = float(value)
     if math.isnan(value) or (name == 'repetition' and not (0 < value < math.inf)):
         raise ValueError('%s must be %s, got %r' % (
             name, 'a positive number' if name == 'repetition' else 'a number', value))
     setattr(args, name + '_value', value)
-    return None
 
 
 def adjust_scores(scores, history=None, history_rows=None, repetition=None, frequency=None,
@@ -305,59 +312,65 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
     n, m = scores.shape
     args = _lib.Adjust()
     args.n_rows, args.n_items, args.ld_scores = n, m, ld
-    args.repetition_value, args.exclude = 1.0, int(bool(exclude))
-    kept = {}
+    args.repetition_value = 1.0
+    kept = []  # every tensor the call reads beside the scores
     if history is not None:
         lists = _lists('history', history, 0)
-        kept['history_ptr'], kept['history_ids'] = history
+        kept += history
+        args.history_ptr, args.history_ids = history[0].data_ptr(), history[1].data_ptr()
+        args.n_history, args.n_history_rows = history[1].numel(), lists
         if history_rows is not None:
             _vector('history_rows', history_rows, torch.int32, n)
-            kept['history_rows'] = history_rows
+            kept.append(history_rows)
+            args.history_rows = history_rows.data_ptr()
         elif lists != n:
             raise ValueError('history has %d lists for %d rows' % (lists, n))
-        args.n_history, args.n_history_rows = history[1].numel(), lists
+        if exclude:
+            args.exclude = 1
     elif history_rows is not None or exclude:
         raise ValueError('history_rows and exclude need a history')
     for name, value in (('repetition', repetition), ('frequency', frequency),
                         ('presence', presence)):
-        if value is None:
-            continue
-        if history is None or exclude:
-            raise ValueError('%s needs a history that is not excluded' % name)
-        kept[name] = _penalty(name, value, n, args)
+        if value is not None:
+            if history is None or exclude:
+                raise ValueError('%s needs a history that is not excluded' % name)
+            _penalty(name, value, n, args, kept)
     if item_bias is not None:
         _vector('item_bias', item_bias, torch.float32, m)
-        kept['item_bias'] = item_bias
+        kept.append(item_bias)
+        args.item_bias = item_bias.data_ptr()
     if row_bias is not None:
         if _lists('row_bias', row_bias, 1) != n:
             raise ValueError('row_bias must have one list for each of the %d rows' % n)
-        kept['bias_ptr'], kept['bias_ids'], kept['bias_values'] = row_bias
-        args.n_bias = row_bias[1].numel()
+        kept += row_bias
+        args.bias_ptr, args.bias_ids = row_bias[0].data_ptr(), row_bias[1].data_ptr()
+        args.bias_values, args.n_bias = row_bias[2].data_ptr(), row_bias[1].numel()
     if mask is not None:
-        if not torch.is_tensor(mask) or mask.dtype != torch.int32 or mask.dim() != 2 or \
+        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.int32 or mask.dim() != 2 or \
                 mask.shape[1] != (m + 31) // 32 or not mask.is_contiguous():
             raise ValueError('mask must be a contiguous int32 tensor [masks, %d]'
                              % ((m + 31) // 32))
         if mask.shape[0] == 0:
             raise ValueError('mask has no rows')
+        kept.append(mask)
+        args.mask, args.n_masks = mask.data_ptr(), mask.shape[0]
         if mask_rows is not None:
             _vector('mask_rows', mask_rows, torch.int32, n)
-            kept['mask_rows'] = mask_rows
+            kept.append(mask_rows)
+            args.mask_rows = mask_rows.data_ptr()
         elif mask.shape[0] not in (1, n):
             raise ValueError('mask must have one row or one for each of the %d rows' % n)
-        kept['mask'], args.n_masks = mask, mask.shape[0]
     elif mask_rows is not None:
         raise ValueError('mask_rows needs a mask')
     if out is not scores:
-        out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores.device, scores,
-                                  *kept.values())
+        out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores.device, scores, *kept)
     else:
         args.ld_out = ld
-    device = _device(scores, out, *kept.values())
-    for name, t in kept.items():
-        setattr(args, name, _p(t))
-    _call(device, 'alsmi_adjust_scores', _CODES[scores.dtype], ctypes.byref(args), _p(scores),
-          _p(out))
+        if any(_overlap(out, t) for t in kept):
+            raise ValueError('out must not overlap the operands')
+    device = _device(scores, out, *kept)
+    _call(device, 'alsmi_adjust_scores', _CODES[scores.dtype], ctypes.byref(args),
+          scores.data_ptr(), out.data_ptr())
     return out
 
 
