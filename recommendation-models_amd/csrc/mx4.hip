@@ -330,33 +330,42 @@ struct ScoreStore {
     void *out;
     int64_t ld, n_sel, n_items;
 };
-// The NT tiles of a wave share out 16 NT items in pairs: row i of tile n is item item_of(n, i), so that
-// a lane (group g) holds eight consecutive items of a pair and the four groups 32: 64 bytes of a
-// row of bf16 scores in one store (with 4 NT consecutive items per lane, every store a quarter of
-// each line it touches, 2048 x 16384 x 4096 took 94 us instead of 81).
+// Row i of a wave's tile n is item item_of<TO>(n, i) of its 16 NT items, so that a store of 16 bytes per
+// lane (group g) leaves the four groups' side by side, 64 bytes of a score row: fp32 tiles as they
+// come, 16-bit ones in pairs, where a lane holds eight consecutive items.  (With 4 NT consecutive
+// items per lane, every store a quarter or half of each line it touches, 2048 x 16384 x 4096 bf16
+// took 94 us instead of 79, 512 x 26744 x 64 fp32 20.7 instead of 18.3.)
+template <typename TO>
 __device__ __forceinline__ int item_of(int n, int i) {
-    return (n >> 1) * 32 + (i >> 2) * 8 + (n & 1) * 4 + (i & 3);
+    return sizeof(TO) == 4 ? 16 * n + i : (n >> 1) * 32 + (i >> 2) * 8 + (n & 1) * 4 + (i & 3);
 }
-// A lane's part of one output row from the NT tiles' results v[n]; `item` is the first of the pair 0.
+// Group g's part of one output row from the NT tiles' results v[n]; `item` is the wave's first.
 template <typename TO, int NT>
-__device__ __forceinline__ void put_row(TO *row, int64_t item, int64_t n_items, const f32x4 (&v)[NT]) {
-    static_assert(NT % 2 == 0, "eight items per store");
-    typedef TO vec_t __attribute__((ext_vector_type(8), aligned(sizeof(TO))));
+__device__ __forceinline__ void put_row(TO *row, int64_t item, int g, int64_t n_items,
+                                        const f32x4 (&v)[NT]) {
+    static_assert(NT % 2 == 0, "tiles in pairs");
+    typedef TO vec_t __attribute__((ext_vector_type(16 / sizeof(TO)), aligned(sizeof(TO))));
     if (!row) return;
-    if (item + 16 * NT - 24 <= n_items) {
+    if (item + 16 * NT <= n_items) {
+        TO *p = row + item + item_of<TO>(0, 4 * g);
+        if constexpr (sizeof(TO) == 4) {
 #pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-            vec_t w;
+            for (int n = 0; n < NT; ++n) *reinterpret_cast<vec_t *>(p + 16 * n) = v[n];
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (TO)v[n][i], w[4 + i] = (TO)v[n + 1][i];
-            *reinterpret_cast<vec_t *>(row + item + 16 * n) = w;
+            for (int n = 0; n < NT; n += 2) {
+                vec_t w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = (TO)v[n][i], w[4 + i] = (TO)v[n + 1][i];
+                *reinterpret_cast<vec_t *>(p + 16 * n) = w;
+            }
         }
     } else {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int64_t at = item + 16 * (n & ~1) + 4 * (n & 1) + i;
+                const int64_t at = item + item_of<TO>(n, 4 * g + i);
                 if (at < n_items) row[at] = (TO)v[n][i];
             }
     }
@@ -393,7 +402,7 @@ __global__ __launch_bounds__(256) void mx4_scores_narrow_kernel(Rows rows, const
     auto fetch = [&](int64_t tile) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            int64_t item = 16 * tile + item_of(n, q);
+            int64_t item = 16 * tile + item_of<TO>(n, q);
             item = item < o.n_items ? item : o.n_items - 1;
             const uint8_t *from = codes + item * (16 * (int64_t)nb) + g * NBL * 4;
 #pragma unroll
@@ -468,7 +477,7 @@ __global__ __launch_bounds__(256) void mx4_scores_narrow_kernel(Rows rows, const
                                                                             acc[t][n], 0, 0, 0);
 #pragma unroll
         for (int t = 0; t < UT; ++t)
-            put_row<TO, NT>(dst[t], 16 * tile + 8 * g, o.n_items, acc[t]);
+            put_row<TO, NT>(dst[t], 16 * tile, g, o.n_items, acc[t]);
     }
 }
 
@@ -531,7 +540,7 @@ __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T
     int64_t it[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int64_t i = item_base + item_of(n, q);
+        const int64_t i = item_base + item_of<TO>(n, q);
         it[n] = i < o.n_items ? i : o.n_items - 1;
     }
     f32x4 acc[MT][NT];
@@ -583,7 +592,7 @@ __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{} + __builtin_nanf("");
         }
-        put_row<TO, NT>(out_row<TO>(o, row_base + 16 * t + q), item_base + 8 * g, o.n_items, acc[t]);
+        put_row<TO, NT>(out_row<TO>(o, row_base + 16 * t + q), item_base, g, o.n_items, acc[t]);
     }
 }
 
@@ -653,8 +662,7 @@ __global__ __launch_bounds__(256, NP > 2 ? 1 : 2) void mx4_scores_split_kernel(c
     }
     const int64_t plane = o.n_sel * units;
     const int place = tid >> 1;
-    const int64_t bsrc =
-        b_row((place & 67) | (place >> 4 & 1) << 2 | (place >> 2 & 3) << 3 | (place & 32)) * nb;
+    const int64_t bsrc = b_row((place & 64) + item_of<TO>(place >> 4 & 3, place & 15)) * nb;
     auto load_step = [&](unsigned step, u32x4 *to_a, u32x4 *to_b) __attribute__((always_inline)) {
         // (one step is loaded past the last turn, and not used)
         const unsigned s = step < 2u * turns ? step : 0u;
@@ -677,7 +685,7 @@ __global__ __launch_bounds__(256, NP > 2 ? 1 : 2) void mx4_scores_split_kernel(c
     const int ar = wm * 64 + q, sa = ar >> 1 & 7;
     const uint8_t *srow[NT];  // the scales of this lane's items
 #pragma unroll
-    for (int n = 0; n < NT; ++n) srow[n] = scales + b_row(wn * 64 + item_of(n, q)) * nb;
+    for (int n = 0; n < NT; ++n) srow[n] = scales + b_row(wn * 64 + item_of<TO>(n, q)) * nb;
     unsigned sw[NT];
     auto load_scales = [&](int turn) {  // the turn's four scales; 1 behind the row's end
         typedef unsigned word_t __attribute__((aligned(1)));
@@ -746,7 +754,7 @@ __global__ __launch_bounds__(256, NP > 2 ? 1 : 2) void mx4_scores_split_kernel(c
     __builtin_amdgcn_s_waitcnt(0x0f70);  // (the step loaded for nothing)
 #pragma unroll
     for (int t = 0; t < MT; ++t)
-        put_row<TO, NT>(out_row<TO>(o, row_base + ar + 16 * t), item_base + wn * 64 + 8 * g, o.n_items,
+        put_row<TO, NT>(out_row<TO>(o, row_base + ar + 16 * t), item_base + wn * 64, g, o.n_items,
                         acc[t]);
 }
 
@@ -787,7 +795,7 @@ __global__ __launch_bounds__(256) void mx4_scores_both_narrow_kernel(
     auto fetch = [&](int64_t tile) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            int64_t item = 16 * tile + item_of(n, q);
+            int64_t item = 16 * tile + item_of<TO>(n, q);
             item = item < o.n_items ? item : o.n_items - 1;
 #pragma unroll
             for (int s = 0; s < NS; ++s)
@@ -827,7 +835,7 @@ __global__ __launch_bounds__(256) void mx4_scores_both_narrow_kernel(
         if (tile + NT < t1) fetch(tile + NT);
 #pragma unroll
         for (int t = 0; t < UT; ++t)
-            put_row<TO, NT>(dst[t], 16 * tile + 8 * g, o.n_items, acc[t]);
+            put_row<TO, NT>(dst[t], 16 * tile, g, o.n_items, acc[t]);
     }
 }
 
@@ -858,7 +866,7 @@ __global__ __launch_bounds__(256) void mx4_scores_both_kernel(Rows rows,
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int64_t i = item_base + item_of(n, q);
+        const int64_t i = item_base + item_of<TO>(n, q);
         it[n] = i < o.n_items ? i : o.n_items - 1;
     }
     f32x4 acc[MT][NT];
@@ -890,7 +898,7 @@ __global__ __launch_bounds__(256) void mx4_scores_both_kernel(Rows rows,
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{} + __builtin_nanf("");
         }
-        put_row<TO, NT>(out_row<TO>(o, row_base + 16 * t + q), item_base + 8 * g, o.n_items, acc[t]);
+        put_row<TO, NT>(out_row<TO>(o, row_base + 16 * t + q), item_base, g, o.n_items, acc[t]);
     }
 }
 
@@ -943,7 +951,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
     // slot s of a buffer: row s / 8, chunk (s % 8) ^ swizzle of the row; a thread's slots are THREADS
     // apart, THREADS / 8 rows, which leaves the swizzles as they are
     auto a_swz = [](unsigned row) { return row >> 1 & 7u; };
-    auto b_swz = [](unsigned row) { return (row >> 1 & 1u) | (row >> 3 & 3u) << 1; };
+    auto b_swz = [](unsigned row) {  // (rows as item_of deals them to 16 lanes)
+        return sizeof(TO) == 4 ? row >> 1 & 7u : (row >> 1 & 1u) | (row >> 3 & 3u) << 1;
+    };
     static_assert(THREADS / 8 % 32 == 0, "rows between a thread's slots");
     const unsigned ca = (tid & 7) ^ a_swz(tid >> 3), cb = (tid & 7) ^ b_swz(tid >> 3);
     unsigned src[LA + LB];  // first block of the row (the host makes sure that 32 bits do)
@@ -976,7 +986,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
     const int wm = wave % WM, wn = wave / WM;
     // rows in the buffers
     const int ar = wm * MT * 16 + q;
-    const int br = wn * NT * 16 + item_of(0, q);
+    const int br = wn * NT * 16 + item_of<TO>(0, q);
     const int sa = a_swz(ar), sb = b_swz(br);  // (the same for all of the wave's tiles)
     // the products of one step; SECOND: of the second step of a turn
     auto products = [&](auto second, const u32x4 *buf, const int (&as)[MT], const int (&bs)[NT])
@@ -990,7 +1000,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
                 af[t] = as_operand(buf[(ar + 16 * t) * 8 + ((2 * g + h) ^ sa)]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const i32x8 bf = as_operand(buf[(BM + br + item_of(n, 0)) * 8 + ((2 * g + h) ^ sb)]);
+                const i32x8 bf = as_operand(buf[(BM + br + item_of<TO>(n, 0)) * 8 + ((2 * g + h) ^ sb)]);
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
                     acc[t][n] = h == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
@@ -1037,7 +1047,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
 #pragma unroll
             for (int t = 0; t < MT; ++t) as[t] = sw[(ar + 16 * t) * 4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) bs[n] = sw[(BM + br + item_of(n, 0)) * 4];
+            for (int n = 0; n < NT; ++n) bs[n] = sw[(BM + br + item_of<TO>(n, 0)) * 4];
             products(std::integral_constant<int, 0>{}, sc0, as, bs);
             spread(std::integral_constant<int, MT + NT>{});
             __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -1058,7 +1068,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
             load_block(acodes, ascales, a_row(ar + 16 * t), blk, nb, af[t], as[t]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            load_block(codes, scales, b_row(br + item_of(n, 0)), blk, nb, bf, bs);
+            load_block(codes, scales, b_row(br + item_of<TO>(n, 0)), blk, nb, bf, bs);
 #pragma unroll
             for (int t = 0; t < MT; ++t)
                 acc[t][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
@@ -1074,7 +1084,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[t][n] = f32x4{} + __builtin_nanf("");
         }
-        put_row<TO, NT>(dst, item_base + wn * NT * 16 + 8 * g, o.n_items, acc[t]);
+        put_row<TO, NT>(dst, item_base + wn * NT * 16, g, o.n_items, acc[t]);
     }
 }
 
