@@ -1094,9 +1094,12 @@ static int launch_narrow(const Rows &rows, const void *a, int width, const uint8
                          const uint8_t *scales, int nb, const ScoreStore &o, hipStream_t st) {
     const int64_t groups = (rows.n_sel + 16 * UT - 1) / (16 * UT);
     const int64_t n_tiles = (o.n_items + 15) / 16;
-    // one turn per wave until there are TARGET waves (what the registers let run at once), then
-    // longer walks
-    constexpr int TARGET = UT == 1 ? 4096 : 2048;
+    // one turn per wave until there are TARGET waves (what the registers let run at once; fewer where
+    // eight blocks of activations are split beforehand), then longer walks: 1024, 2048 and 4096
+    // waves took 13.8, 14.6 and 11.9 us for 1 x 1000000 x 64 fp32, 18.7, 18.5 and 19.8 for 512 x
+    // 26744 x 64, 20.6, 23.6 and 27.8 for 512 x 26744 x 200 bf16, 25.7, 38 and 32 for 1 x 1000000 x
+    // 200 fp32
+    constexpr int TARGET = NBL == 8 ? 1024 : UT == 1 ? 4096 : 2048;
     int64_t turns = n_tiles * groups / (TARGET * NT);
     turns = turns < 1 ? 1 : (turns > 16 ? 16 : turns);
     const int64_t tpw = turns * NT;
@@ -1172,25 +1175,37 @@ static int run_both(const Rows &rows, const void *a, const uint8_t *a_scales, co
     if (nb <= 8)
         return one ? launch_both_narrow<TO, 2, 1, 2>(rows, a, a_scales, codes, scales, nb, o, st)
                    : launch_both_narrow<TO, 2, 4, 2>(rows, a, a_scales, codes, scales, nb, o, st);
+    // (each wave on its own instead of four per row: 1 x 1000000 x 512 72 us instead of 49)
+    if (one) return launch_both<TO, 1, 2, 4>(rows, a, a_scales, codes, scales, nb, o, st);
+    // the tiled forms keep the loads of a long row in flight, which a few tiles cannot fill the
+    // chip with (17 x 4000 x 1024 5.6 us against 4.4, 40 x 16384 x 4096 15 against 32) and rows of
+    // less than a turn have no use for (256 x 4000 x 384 7.3 against 4.6, 128 x 20000 x 300 8.4
+    // against 7.2, 1024 x 26744 x 384 33 against 41)
     const int64_t tiles = (rows.n_sel + 15) / 16 * ((o.n_items + 15) / 16);
-    if (one)
-        return tiles < 32768 ? launch_both<TO, 1, 2, 4>(rows, a, a_scales, codes, scales, nb, o, st)
-                             : launch_both<TO, 1, 4, 1>(rows, a, a_scales, codes, scales, nb, o, st);
-    // (the tiled form counts blocks in 32 bits and loads 16 bytes at a time)
+    if (tiles < (nb >= 16 ? 2048 : 32768))
+        return launch_both<TO, 2, 2, 4>(rows, a, a_scales, codes, scales, nb, o, st);
+    // (they count blocks in 32 bits and load 16 bytes at a time)
     const bool aligned = (uintptr_t)a % 16 == 0 && (uintptr_t)codes % 16 == 0 &&
                          rows.n_rows * nb < (int64_t)1 << 32 && o.n_items * nb < (int64_t)1 << 32;
+    if (!aligned || nb < 16) return launch_both<TO, 4, 4, 1>(rows, a, a_scales, codes, scales, nb, o, st);
+    // A tile of 256 x 256 fills a CU and takes 1.15 times less per score than four of 128 x 128, two
+    // of which run on a CU at a time; it loses where its last round is not full: 2048 x 16384 x
+    // 4096 86 us against 100, 512 x 32768 x 1024 21.5 against 26, but 512 x 26744 x 1024 26.3
+    // against 23.1, 300 x 65536 x 2048 53 against 45, 1000 x 8192 x 4096 38 against 28.
     const int64_t t256 = (rows.n_sel + 255) / 256 * ((o.n_items + 255) / 256);
-    if (aligned && nb >= 16 && t256 >= 192)
+    const int64_t t128 = (rows.n_sel + 127) / 128 * ((o.n_items + 127) / 128);
+    if ((t256 + 255) / 256 * 102400 <= t128 * 115)
         return launch_tiled<TO, 4, 2, 4, 8>(rows, a, a_scales, codes, scales, nb, o, st);
-    if (aligned && nb >= 16 && rows.n_sel > 64)
-        return launch_tiled<TO, 2, 2, 4, 4>(rows, a, a_scales, codes, scales, nb, o, st);
-    return launch_both<TO, 4, 4, 1>(rows, a, a_scales, codes, scales, nb, o, st);
+    return launch_tiled<TO, 2, 2, 4, 4>(rows, a, a_scales, codes, scales, nb, o, st);
 }
 
-// Whether a float product is split first: enough whole tiles, and rows long enough for a few turns.
+// Whether a float product is split first: enough whole tiles (bf16, 128 x 16384 x 512 11.8 us against
+// 15.8 from memory, 512 x 4096 x 1024 18.9 against 27.6, but 128 x 8192 x 4096 53 against 48), for up
+// to 64 rows, which leave half of a tile empty, only long rows and more tiles (64 x 65536 x 2048 fp32
+// 107 against 133, 64 x 100000 x 512 fp32 62 against 43, 64 x 16384 x 4096 bf16 53 against 47).
 static bool splits(int64_t n_sel, int64_t n_items, int nb) {
     const int64_t tiles = (n_sel + WT_ROWS - 1) / WT_ROWS * ((n_items + WT_ITEMS - 1) / WT_ITEMS);
-    return n_sel > 64 && nb > 8 && tiles >= 128;
+    return n_sel > 64 ? nb > 8 && tiles >= 128 : n_sel > 32 && nb >= 32 && tiles >= 192;
 }
 static int64_t split_bytes(int64_t n_sel, int nb, int parts) {
     return n_sel * ((nb + 3) / 4) * 256 * parts;
@@ -1244,12 +1259,21 @@ static int run_scores(const Rows &rows, const void *a, int width, const uint8_t 
     if (nb <= 8)
         return one ? launch_narrow<T, TO, 8, 1, 2>(rows, a, width, codes, scales, nb, o, st)
                    : launch_narrow<T, TO, 8, 4 / Parts<T>::N, 2>(rows, a, width, codes, scales, nb, o, st);
+    // Four waves share a row's contraction, or each forms tiles of its own and reads the activations
+    // less often, which pays for several parts and many items against short rows: 1 x 1000000 x 512
+    // fp32 105 us against 84, 16 x 400000 x 1024 141 against 109, but 1 x 100000 x 4096 80 against
+    // 121; bf16 1 x 400000 x 1024 70 against 85, 16 x 1000000 x 512 120 against 108.
     const int64_t tiles = (rows.n_sel + 15) / 16 * ((o.n_items + 15) / 16);
+    const int steps = (nb + 3) / 4;
     if (one)
-        return tiles < 32768 ? launch_wide<T, TO, 1, 2, 4>(rows, a, width, codes, scales, nb, o, st)
-                             : launch_wide<T, TO, 1, 4, 1>(rows, a, width, codes, scales, nb, o, st);
-    return tiles < 16384 ? launch_wide<T, TO, 2, 2, 4>(rows, a, width, codes, scales, nb, o, st)
-                         : launch_wide<T, TO, 4, 4, 1>(rows, a, width, codes, scales, nb, o, st);
+        return Parts<T>::N == 1 || tiles < 2048 * (int64_t)steps
+                   ? launch_wide<T, TO, 1, 2, 4>(rows, a, width, codes, scales, nb, o, st)
+                   : launch_wide<T, TO, 1, 4, 1>(rows, a, width, codes, scales, nb, o, st);
+    // two row tiles a wave, or four: 17 x 200000 x 1024 bf16 59 us against 81, 64 x 16384 x 2000 fp32
+    // 39 against 110, but 64 x 65536 x 512 45 against 37, 33 x 100000 x 512 60 against 39
+    return rows.n_sel <= 32 || tiles < 16384
+               ? launch_wide<T, TO, 2, 2, 4>(rows, a, width, codes, scales, nb, o, st)
+               : launch_wide<T, TO, 4, 4, 1>(rows, a, width, codes, scales, nb, o, st);
 }
 
 }  // namespace alsmi

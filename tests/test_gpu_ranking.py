@@ -183,7 +183,9 @@ def test_scores_match_definition(m, n, width, kind):
                                        (1, 70001, 200), (257, 9001, 128), (2048, 2049, 192),
                                        (513, 2000, 2080), (300, 6001, 300), (1000, 2100, 1100),
                                        (129, 8300, 135), (4000, 3333, 520), (70, 16385, 512),
-                                       (40, 30001, 256), (90, 9000, 250)])
+                                       (40, 30001, 256), (90, 9000, 250), (1020, 16300, 700),
+                                       (40, 25000, 1100), (3, 140000, 300), (300, 60000, 300),
+                                       (18, 70000, 1030)])
 def test_scores_large(m, n, width, kind):
     """Sizes that take the long-walk and one-step forms; a strip of items against the definition,
     the rest against another order of the same items."""
@@ -205,7 +207,8 @@ def test_scores_large(m, n, width, kind):
 
 
 @pytest.mark.parametrize('kind', ['f32', 'bf16', 'f16', 'mx4'])
-@pytest.mark.parametrize('m,n,width', [(200, 9001, 300), (300, 70000, 544), (17, 40000, 700)])
+@pytest.mark.parametrize('m,n,width', [(200, 9001, 300), (300, 70000, 544), (17, 40000, 700),
+                                       (1010, 16250, 544), (50, 24999, 1030)])
 def test_scores_of_picked_rows_large(m, n, width, kind):
     """Rows by id, some missing, out of strided activations into a strided output, at sizes of the
     tiled forms; blocks that are no number reach their items alone."""
