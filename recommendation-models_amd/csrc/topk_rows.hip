@@ -1,24 +1,28 @@
 // The k largest scores of every row of a score block, best first, ties to the lowest index.
 //
 // Scores are ranked through the order-preserving integer image of their bits joined with the
-// complement of their index: (image << 32) | ~index, 48, 64 or 96 bits.  These keys are all different, so "the k-th
+// complement of their index, up to 96 bits.  These keys are all different, so "the k-th
 // largest" is one element however many scores are equal (rows that a mask left mostly at -inf, 16-bit
 // scores), comparing keys is the whole tie rule, and any set of candidates can be merged in any
 // order.  0 is below every key.
 //
-// k <= 64: a wave keeps its k best, sorted, one per lane, and streams over its part of the row: a key at
+// Small k: a wave keeps its k best, sorted, one per lane, and streams over its part of the row: a key at
 //   or below the k-th best is dropped by one comparison, the few others wait in LDS until 64 of them
 //   are sorted and merged into the list at once.  Four waves per workgroup, as many workgroups per row
-//   as fill the chip; a second launch merges their lists.
-// k > 64: a workgroup holds a tile of 8192 keys in registers, finds the tile's k-th largest by a radix
-//   descent over LDS histograms (2048 bins a digit) and keeps the k keys at or above it; the kept
-//   keys of all tiles are the next, 8192 / k times shorter, row.  The last level takes up to 16384 keys
-//   in one workgroup and sorts.
+//   as fill the chip; a second launch merges their lists.  Bound by the reads for many rows (1024 x
+//   26744 fp32, k = 10: 24 us, 4.6 TB/s), by two launches' latencies for one (1 x 1000000: 14 us).
+// Larger k: a workgroup of 512 threads keeps the k best of its part of the row: of the first 8192 keys,
+//   held in registers, it finds the k-th largest by a radix descent over LDS histograms (2048 bins
+//   a digit), from then on only keys above it are looked at again.  Parts as many as run at once;
+//   the kept keys of a row's parts are the next, much shorter, row.  The last level sorts.  Bound by
+//   the latencies of the descent and the sort (1024 x 26744 fp32, k = 100: 44 us, 1000: 70; 37 x
+//   100003 bf16, k = 1000: 31).
 #include "alsmi_common.h"
 #include "elem.h"
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 namespace alsmi {
 
@@ -26,9 +30,10 @@ constexpr int TR_MAX_K = 1024;
 constexpr int TR_LIST = 64;         // the longest list one wave keeps
 constexpr int TR_CHUNK = 1024;      // keys a wave looks at per turn, 16 per lane
 constexpr int TR_PART = 4 * TR_CHUNK;
-constexpr int TR_THREADS = 512;     // k > 64: threads and keys per workgroup
+constexpr int TR_THREADS = 512;     // larger k: threads of a workgroup, keys they look at per turn,
 constexpr int TR_TILE = 8192;
-constexpr int TR_LAST = 16384;      // and of the last level's 1024 threads
+constexpr int TR_LAST = 16384;      // keys of a last turn by 1024 threads,
+constexpr int TR_GROUPS = 1024;     // and workgroups that run at once
 
 typedef unsigned __int128 u128;
 
@@ -41,8 +46,7 @@ struct RowKey {  // fp32: 32 bits of image, 32 of index
         const unsigned b = __builtin_bit_cast(unsigned, s);
         return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
     }
-    static __device__ __forceinline__ T score(type k) {
-        const unsigned i = (unsigned)(k >> 32);
+    static __device__ __forceinline__ T score(image_t i) {
         return __builtin_bit_cast(T, (i & 0x80000000u) ? (i & 0x7fffffffu) : ~i);
     }
 };
@@ -53,8 +57,7 @@ struct RowKey16 {  // fp16, bf16: 16 bits of image
     static __device__ __forceinline__ image_t image(unsigned short b) {
         return (b ^ ((unsigned)((int)(short)b >> 31) | 0x8000u)) & 0xffffu;
     }
-    static __device__ __forceinline__ unsigned short bits(type k) {
-        const unsigned i = (unsigned)(k >> 32);
+    static __device__ __forceinline__ unsigned short bits(image_t i) {
         return (unsigned short)((i & 0x8000u) ? (i & 0x7fffu) : ~i);
     }
 };
@@ -63,8 +66,8 @@ struct RowKey<_Float16> : RowKey16 {
     static __device__ __forceinline__ image_t image(_Float16 s) {
         return RowKey16::image(__builtin_bit_cast(unsigned short, s));
     }
-    static __device__ __forceinline__ _Float16 score(type k) {
-        return __builtin_bit_cast(_Float16, bits(k));
+    static __device__ __forceinline__ _Float16 score(image_t i) {
+        return __builtin_bit_cast(_Float16, bits(i));
     }
 };
 template <>
@@ -72,7 +75,7 @@ struct RowKey<__bf16> : RowKey16 {
     static __device__ __forceinline__ image_t image(__bf16 s) {
         return RowKey16::image(__builtin_bit_cast(unsigned short, s));
     }
-    static __device__ __forceinline__ __bf16 score(type k) { return __builtin_bit_cast(__bf16, bits(k)); }
+    static __device__ __forceinline__ __bf16 score(image_t i) { return __builtin_bit_cast(__bf16, bits(i)); }
 };
 template <>
 struct RowKey<double> {
@@ -83,8 +86,7 @@ struct RowKey<double> {
         const unsigned long long b = __builtin_bit_cast(unsigned long long, s);
         return b ^ ((unsigned long long)((long long)b >> 63) | 0x8000000000000000ull);
     }
-    static __device__ __forceinline__ double score(type k) {
-        const unsigned long long i = (unsigned long long)(k >> 32);
+    static __device__ __forceinline__ double score(image_t i) {
         return __builtin_bit_cast(double, (i >> 63) ? (i & 0x7fffffffffffffffull) : ~i);
     }
 };
@@ -340,11 +342,11 @@ __global__ __launch_bounds__(256) void topk_list_kernel(KeySource<T, FROM_KEYS> 
         kept[(row * parts + part) * k + lane] = list;
     } else {
         items_out[row * k + lane] = (int32_t)~(unsigned)list;
-        scores_out[row * k + lane] = RowKey<T>::score(list);
+        scores_out[row * k + lane] = RowKey<T>::score((typename RowKey<T>::image_t)(list >> 32));
     }
 }
 
-// ---- k > 64 --------------------------------------------------------------------------------------
+// ---- larger k ------------------------------------------------------------------------------------
 // Sum over lanes 0 .. lane.
 __device__ __forceinline__ unsigned wave_prefix(unsigned x) {
     auto add = [&](auto ctrl, auto rows) {
@@ -361,15 +363,15 @@ __device__ __forceinline__ unsigned wave_prefix(unsigned x) {
 }
 
 // The smallest of the k largest keys of a workgroup (THREADS x E keys of at most `bits` bits in
-// registers, all different but for zeros), by digits of 11 bits from the top; 0 if there are no k
-// keys above it.  A pass costs its atomics and two barriers: every wave reads the whole histogram
+// registers, all different but for zeros, which stand for none), by digits of 11 bits from the top; 0
+// if there are fewer than k.  A pass costs its atomics and two barriers: every wave reads the whole histogram
 // and finds the digit by itself (one wave, or sums by thread and prefix sums over the workgroup,
 // with more barriers, took longer), and the other of two histograms is cleared meanwhile.
-template <typename K, int THREADS, int E>
-__device__ __forceinline__ K kth_key(const K (&key)[E], int k, int bits) {
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    constexpr int DIGIT = 11, BINS = 1 << DIGIT, LANE_BINS = BINS / 64;
-    __shared__ u32x4 hist4[2][BINS / 4];
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+constexpr int TR_DIGIT = 11, TR_BINS = 1 << TR_DIGIT;
+template <typename K, int THREADS, int E, int HELD>
+__device__ __forceinline__ K kth_key(const K (&key)[HELD], int k, int bits, u32x4 (&hist4)[2][TR_BINS / 4]) {
+    constexpr int DIGIT = TR_DIGIT, BINS = TR_BINS, LANE_BINS = BINS / 64;
     const int tid = threadIdx.x, lane = tid & 63;
     K prefix = 0;
     unsigned want = k;
@@ -386,7 +388,7 @@ __device__ __forceinline__ K kth_key(const K (&key)[E], int k, int bits) {
         unsigned run = 0;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            if ((key[j] & upper) != prefix) continue;
+            if ((key[j] & upper) != prefix || key[j] == 0) continue;
             const int b = (int)((unsigned)(key[j] >> low) & mask);
             if (b != run_bin) {
                 if (run) atomicAdd(&hist[run_bin], run);
@@ -407,7 +409,8 @@ __device__ __forceinline__ K kth_key(const K (&key)[E], int k, int bits) {
             sum += h[0] + h[1] + h[2] + h[3];
         }
         unsigned upto = wave_prefix(sum);
-        unsigned long long found = __ballot(upto >= want);  // (never 0: zeros are counted too)
+        unsigned long long found = __ballot(upto >= want);
+        if (found == 0) return 0;
         const int owner = __builtin_ctzll(found);
         unsigned above = (unsigned)__builtin_amdgcn_readlane((int)(upto - sum), owner);
         // and the bin among the owner's
@@ -426,103 +429,192 @@ __device__ __forceinline__ K kth_key(const K (&key)[E], int k, int bits) {
     return prefix;
 }
 
-// One tile of a row; SORT: the only tile of its row, whose k best are sorted and written out.
-template <typename T, bool FROM_KEYS, bool SORT, int THREADS, int E>
+// Workgroup (row, part) keeps the k best of its part of the row and writes them to `kept`, or, SORT, the
+// whole row's sorted.  It walks the part in tiles of TILE keys: those above the k-th best so far
+// are appended to the kept ones in LDS (one barrier a tile), and where these would be more than
+// 2 TR_MAX_K, as for the first tile, kept ones and tile are cut down to the best k together.
+// Keys here are image << index_bits | n_items - index, never 0.
+template <typename T, bool FROM_KEYS, bool SORT, int THREADS, int TILE>
 __global__ __launch_bounds__(THREADS) void topk_tile_kernel(KeySource<T, FROM_KEYS> src, int k,
-                                                            int index_bits, unsigned tiles,
-                                                            typename RowKey<T>::type *__restrict__ kept,
-                                                            int32_t *__restrict__ items_out,
-                                                            T *__restrict__ scores_out) {
+                                                               unsigned n_items, int index_bits,
+                                                               unsigned parts, int64_t part_len,
+                                                               typename RowKey<T>::type *__restrict__ kept,
+                                                               int32_t *__restrict__ items_out,
+                                                               T *__restrict__ scores_out) {
     typedef typename RowKey<T>::type key_t;
-    constexpr int VEC = FROM_KEYS ? 16 / (int)sizeof(key_t) : 16 / (int)sizeof(T);
-    static_assert(!SORT || THREADS == TR_MAX_K, "one key per thread to sort");
-    __shared__ key_t sel[SORT ? TR_MAX_K : 1];
-    __shared__ int n_kept;
+    typedef KeySource<T, FROM_KEYS> source;
+    constexpr int E = TILE / THREADS;
+    constexpr int VEC = 16 / (int)sizeof(typename source::raw_t);
+    constexpr int ROOM = 2 * TR_MAX_K;
+    constexpr int KEEP = ROOM / THREADS, SORTED = TR_MAX_K / THREADS;  // keys of a thread of these
+    __shared__ key_t sel[ROOM];
+    __shared__ u32x4 hist[2][TR_BINS / 4];
+    __shared__ int added[3];  // keys added by a step; the one after the next step's is cleared meanwhile
     const int tid = threadIdx.x, lane = tid & 63;
-    const unsigned r32 = blockIdx.x / tiles;
+    const unsigned r32 = blockIdx.x / parts;
     const int64_t row = r32;
-    const unsigned tile = blockIdx.x - r32 * tiles;
-    const int64_t first = (int64_t)tile * (THREADS * E);
-    key_t key[E];
+    const unsigned part = blockIdx.x - r32 * parts;
+    const int64_t first = (int64_t)part * part_len;
+    const int64_t end = first + part_len < src.n ? first + part_len : src.n;
+    const typename source::raw_t *data = src.data + row * src.ld;
+    key_t floor_key = 0;  // keys at or below it are out
+    int have = 0, step = 0;
+    key_t key[E + KEEP];  // a tile's, and of the kept ones when these are cut down
+    // the first N keys that are above floor_key go behind the `have` kept ones; how many there are
+    auto append = [&](auto n, auto put) __attribute__((always_inline)) {
+        constexpr int N = decltype(n)::value;
+        unsigned mine = 0;
 #pragma unroll
-    for (int j = 0; j < E; j += VEC) {
-        typedef KeySource<T, FROM_KEYS> source;
-        typename source::raw_t raw[VEC];
-        const int64_t at = first + j * THREADS + tid * VEC;
-        source::load(raw, src.data + row * src.ld, at, src.n);
+        for (int j = 0; j < N; ++j) mine += key[j] > floor_key;
+        int *count = &added[step];
+        if (__any(mine)) {
+            const unsigned upto = wave_prefix(mine);
+            int place = 0;
+            if (lane == 63) place = atomicAdd(count, (int)upto);
+            place = have + __builtin_amdgcn_readlane(place, 63) + (int)(upto - mine);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) key[j + i] = source::key(raw[i], at + i, src.n);
-    }
-    if (tid == 0) n_kept = 0;
-    key_t floor_key = 1;
-    if (src.n - first > k) {
-        // without the bits between image and index, which are ones in every key
-        const unsigned index_mask = 0xffffffffu >> (32 - index_bits);
-        auto without = [&](key_t x) { return ((x >> 32) << index_bits) | ((unsigned)x & index_mask); };
-        key_t dense[E];
+            for (int j = 0; j < N; ++j)
+                if (key[j] > floor_key) put(place++, key[j]);
+        }
+        __syncthreads();
+        const int got = *count;
+        step = step == 2 ? 0 : step + 1;
+        if (tid == 0) added[step == 2 ? 0 : step + 1] = 0;
+        return got;
+    };
+    auto to_sel = [&](int place, key_t x) {
+        if (place < ROOM) sel[place] = x;
+    };
+    const int bits = RowKey<T>::BITS - 32 + index_bits;
+    // kept ones and key[0 .. E) cut down to the k best
+    auto cut = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) dense[j] = without(key[j]);
-        const key_t kth =
-            kth_key<key_t, THREADS, E>(dense, k, RowKey<T>::BITS - 32 + index_bits);
-        if (kth != 0)
-            floor_key = ((kth >> index_bits) << 32) | (unsigned)~index_mask | ((unsigned)kth & index_mask);
-    }
+        for (int i = 0; i < KEEP; ++i)
+            key[E + i] = i * THREADS + tid < have ? sel[i * THREADS + tid] : (key_t)0;
+        const key_t kth = kth_key<key_t, THREADS, E + KEEP>(key, k, bits, hist);
+        floor_key = kth ? kth - 1 : 0;
+        have = 0;
+        __syncthreads();
+        have = append(std::integral_constant<int, E + KEEP>{}, to_sel);
+        floor_key = kth;
+    };
+    typename source::raw_t raw[E / VEC][VEC];
+    auto fetch = [&](int64_t at0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < E / VEC; ++j) source::load(raw[j], data, at0 + (j * THREADS + tid) * VEC, end);
+    };
+    fetch(first);
+    if (tid < 3) added[tid] = 0;
     __syncthreads();
-    key_t *dst = SORT ? sel : kept + (row * tiles + tile) * k;
-    unsigned mine_kept = 0;
+    for (int64_t at0 = first; at0 < end; at0 += TILE) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) mine_kept += key[j] >= floor_key;
-    const unsigned upto = wave_prefix(mine_kept);
-    int place = 0;
-    if (lane == 63) place = atomicAdd(&n_kept, (int)upto);
-    place = __builtin_amdgcn_readlane(place, 63) + (int)(upto - mine_kept);
+        for (int j = 0; j < E / VEC; ++j)
 #pragma unroll
-    for (int j = 0; j < E; ++j)
-        if (key[j] >= floor_key) dst[place++] = key[j];
-    __syncthreads();
-    const int have = n_kept;
+            for (int i = 0; i < VEC; ++i) {
+                const int64_t at = at0 + (j * THREADS + tid) * VEC + i;
+                if constexpr (FROM_KEYS) key[j * VEC + i] = raw[j][i];
+                else
+                    key[j * VEC + i] = at < end ? (key_t)RowKey<T>::image(raw[j][i]) << index_bits |
+                                                      (n_items - (unsigned)at)
+                                                : (key_t)0;
+            }
+        fetch(at0 + TILE);  // (on its way while this one is looked at)
+        if constexpr (!SORT) {
+            if (first + TILE >= end) {  // the only tile: straight from the registers
+                key_t *dst = kept + (row * parts + part) * k;
+                const key_t kth = kth_key<key_t, THREADS, E>(key, k, bits, hist);
+                floor_key = kth ? kth - 1 : 0;
+                have = append(std::integral_constant<int, E>{}, [&](int place, key_t x) { dst[place] = x; });
+                for (int i = have + tid; i < k; i += THREADS) dst[i] = 0;
+                return;
+            }
+        }
+        // (before there is a bound every key of a tile would be added)
+        if (floor_key != 0 || have + (end - at0) <= ROOM) {
+            const int got = append(std::integral_constant<int, E>{}, to_sel);
+            if (have + got <= ROOM) {
+                have += got;
+                continue;
+            }
+        }
+        cut();
+    }
+    if (have > k) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) key[j] = 0;
+        cut();
+    }
     if constexpr (!SORT) {
-        for (int i = have + tid; i < k; i += THREADS) dst[i] = 0;
+        key_t *dst = kept + (row * parts + part) * k;
+        for (int i = tid; i < k; i += THREADS) dst[i] = i < have ? sel[i] : (key_t)0;
     } else {
-        // one key per thread: sorted by wave, then runs of 64, 128, ... meet the mirror image of the next
-        // run; steps within a wave go through the lanes, the others through LDS
-        key_t mine = wave_sort(tid < have ? sel[tid] : (key_t)0, lane);
+        // sorted by wave, then runs of 64, 128, ... meet the mirror image of the next run; steps within a
+        // wave go through the lanes, the others through LDS
+        key_t mine[SORTED];
+#pragma unroll
+        for (int r = 0; r < SORTED; ++r) {
+            const int i = r * THREADS + tid;
+            mine[r] = wave_sort(i < have ? sel[i] : (key_t)0, lane);
+        }
         for (int size = 128; size < 2 * k; size <<= 1) {  // (runs behind the k-th key hold zeros)
             int mask = size - 1;
             for (int top = size >> 1; top >= 64; top >>= 1) {
                 __syncthreads();
-                sel[tid] = mine;
+#pragma unroll
+                for (int r = 0; r < SORTED; ++r) sel[r * THREADS + tid] = mine[r];
                 __syncthreads();
-                const key_t o = sel[tid ^ mask];
-                mine = (o > mine) != ((tid & top) != 0) ? o : mine;
+#pragma unroll
+                for (int r = 0; r < SORTED; ++r) {
+                    const int i = r * THREADS + tid;
+                    const key_t o = sel[i ^ mask];
+                    mine[r] = (o > mine[r]) != ((i & top) != 0) ? o : mine[r];
+                }
                 mask = top >> 1;
             }
-            mine = wave_merge(mine, lane);
+#pragma unroll
+            for (int r = 0; r < SORTED; ++r) mine[r] = wave_merge(mine[r], lane);
         }
-        if (tid < k) {
-            items_out[row * k + tid] = (int32_t)~(unsigned)mine;
-            scores_out[row * k + tid] = RowKey<T>::score(mine);
+#pragma unroll
+        for (int r = 0; r < SORTED; ++r) {
+            const int i = r * THREADS + tid;
+            if (i >= k) continue;
+            items_out[row * k + i] =
+                (int32_t)(n_items - ((unsigned)mine[r] & (0xffffffffu >> (32 - index_bits))));
+            scores_out[row * k + i] =
+                RowKey<T>::score((typename RowKey<T>::image_t)(mine[r] >> index_bits));
         }
     }
 }
 
 // ---- launches ------------------------------------------------------------------------------------
-// k <= 64: workgroups per row, so that the launch has about 1024, at least 4096 keys each.
+// Lists: workgroups per row, so that the launch has about 1024, at least 4096 keys each.
 static int64_t list_parts(int64_t n_rows, int64_t n_items, int64_t &part_len) {
     const int64_t most = (n_items + TR_PART - 1) / TR_PART;
-    int64_t parts = 1024 / n_rows;
+    int64_t parts = most <= 4 ? 1 : 1024 / n_rows;  // (a second launch costs more than four turns)
     parts = parts < 1 ? 1 : (parts > most ? most : parts);
     part_len = ((n_items + parts - 1) / parts + TR_PART - 1) / TR_PART * TR_PART;
     return (n_items + part_len - 1) / part_len;
 }
-static int64_t tiles_of(int64_t n) { return (n + TR_TILE - 1) / TR_TILE; }
-// Rows that are worked on at once: a launch has fewer than 2^32 threads.
-static int64_t batch_rows(int64_t n_items, int k) {
-    return k <= TR_LIST ? (int64_t)1 << 23 : std::max<int64_t>(1, ((int64_t)1 << 21) / tiles_of(n_items));
+// Tiles: workgroups per row, so that a launch has about TR_GROUPS, of whole tiles.
+static int64_t tile_parts(int64_t n_rows, int64_t n, int64_t &part_len) {
+    const int64_t most = (n + TR_TILE - 1) / TR_TILE;
+    int64_t parts = most <= 2 ? 1 : TR_GROUPS / n_rows;  // (a second launch costs more than a second tile)
+    parts = parts < 1 ? 1 : (parts > most ? most : parts);
+    part_len = (most + parts - 1) / parts * TR_TILE;
+    return (n + part_len - 1) / part_len;
 }
+// Which of the two forms: sorted lists take 29 us against 42 for 1024 x 26744 fp32 and k = 64, 13.4
+// against 21 for 512 x 16384 and k = 32, but 28 against 18 for 1 x 1000000 and k = 64, 17.5 against 14 for
+// 1 x 100000 and k = 32 (14.4 either way for k = 10): a row of many parts has many lists to merge.
+static bool by_lists(int64_t n_rows, int64_t n_items, int k) {
+    return k <= 24 || (k <= TR_LIST && (n_rows > 128 || n_items <= 4 * TR_PART));
+}
+// Rows that are worked on at once: a launch has fewer than 2^32 threads.  Their number decides over the
+// parts of a row for a smaller rest as well, so that the workspace does.
+static int64_t batch_rows(int64_t n_rows) { return std::min(n_rows, (int64_t)1 << 21); }
 
 template <typename T>
-static int run_lists(int64_t n_rows, const KeySource<T, false> &src, int k, int32_t *items_out,
+static int run_lists(int64_t n_rows, int64_t batch, const KeySource<T, false> &src, int k, int32_t *items_out,
                      T *scores_out, typename RowKey<T>::type *kept, hipStream_t st) {
     typedef typename RowKey<T>::type key_t;
     if (src.n <= TR_CHUNK) {
@@ -532,7 +624,7 @@ static int run_lists(int64_t n_rows, const KeySource<T, false> &src, int k, int3
         return ALSMI_OK;
     }
     int64_t part_len = 0;
-    const int64_t parts = list_parts(n_rows, src.n, part_len);
+    const int64_t parts = list_parts(batch, src.n, part_len);
     hipLaunchKernelGGL((topk_list_kernel<T, false, false>), dim3((unsigned)(parts * n_rows)), dim3(256), 0,
                        st, src, n_rows, k, (unsigned)parts, part_len, kept, items_out, scores_out);
     ALSMI_HIP_CHECK(hipGetLastError());
@@ -546,44 +638,59 @@ static int run_lists(int64_t n_rows, const KeySource<T, false> &src, int k, int3
     return ALSMI_OK;
 }
 
-template <typename T>
-static int run_tiles(int64_t n_rows, const KeySource<T, false> &src, int k, int32_t *items_out,
-                     T *scores_out, typename RowKey<T>::type *kept, hipStream_t st) {
+// The level that sorts: a workgroup per row.  Rows of one to two tiles go as one larger one while
+// there are not enough of them to fill the chip (200 x 16384 fp32, k = 100: 13.1 us instead of 15.6;
+// 1024 x 16384: 44 instead of 36).
+template <typename T, bool FROM_KEYS>
+static int run_last(int64_t n_rows, const KeySource<T, FROM_KEYS> &src, int k, unsigned n_items, int index_bits,
+                    int64_t part_len, int32_t *items_out, T *scores_out, hipStream_t st) {
     typedef typename RowKey<T>::type key_t;
-    const dim3 last_grid((unsigned)n_rows), last_block(TR_MAX_K);
-    int index_bits = 1;
-    while (index_bits < 31 && (src.n - 1) >> index_bits) ++index_bits;
-    if (src.n <= TR_LAST) {
-        hipLaunchKernelGGL((topk_tile_kernel<T, false, true, TR_MAX_K, TR_LAST / TR_MAX_K>), last_grid,
-                           last_block, 0, st, src, k, index_bits, 1u, (key_t *)nullptr, items_out, scores_out);
-        ALSMI_HIP_CHECK(hipGetLastError());
-        return ALSMI_OK;
+    auto kernel = topk_tile_kernel<T, FROM_KEYS, true, TR_THREADS, TR_TILE>;
+    int threads = TR_THREADS;
+    if constexpr (sizeof(key_t) == 8) {  // (16 keys of 96 bits are too many registers for 1024 threads)
+        if (src.n > TR_TILE && src.n <= TR_LAST && n_rows <= 512) {
+            kernel = topk_tile_kernel<T, FROM_KEYS, true, TR_MAX_K, TR_LAST>;
+            threads = TR_MAX_K;
+        }
     }
-    int64_t tiles = tiles_of(src.n);
-    hipLaunchKernelGGL((topk_tile_kernel<T, false, false, TR_THREADS, TR_TILE / TR_THREADS>),
-                       dim3((unsigned)(tiles * n_rows)), dim3(TR_THREADS), 0, st, src, k, index_bits,
-                       (unsigned)tiles, kept, (int32_t *)nullptr, (T *)nullptr);
-    ALSMI_HIP_CHECK(hipGetLastError());
-    // the levels alternate between the two parts of the workspace
-    key_t *from = kept, *to = kept + n_rows * tiles * k;
-    int64_t n = tiles * k;
-    while (n > TR_LAST) {
-        tiles = tiles_of(n);
-        const KeySource<T, true> left = {from, n, n};
-        hipLaunchKernelGGL((topk_tile_kernel<T, true, false, TR_THREADS, TR_TILE / TR_THREADS>),
-                           dim3((unsigned)(tiles * n_rows)), dim3(TR_THREADS), 0, st, left, k, index_bits,
-                           (unsigned)tiles, to, (int32_t *)nullptr, (T *)nullptr);
-        ALSMI_HIP_CHECK(hipGetLastError());
-        key_t *t = from;
-        from = to;
-        to = t;
-        n = tiles * k;
-    }
-    const KeySource<T, true> left = {from, n, n};
-    hipLaunchKernelGGL((topk_tile_kernel<T, true, true, TR_MAX_K, TR_LAST / TR_MAX_K>), last_grid,
-                       last_block, 0, st, left, k, index_bits, 1u, (key_t *)nullptr, items_out, scores_out);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n_rows), dim3(threads), 0, st, src, k, n_items, index_bits, 1u,
+                       part_len, (key_t *)nullptr, items_out, scores_out);
     ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
+}
+
+template <typename T>
+static int run_tiles(int64_t n_rows, int64_t batch, const KeySource<T, false> &src, int k, int32_t *items_out,
+                     T *scores_out, typename RowKey<T>::type *kept, hipStream_t st) {
+    typedef typename RowKey<T>::type key_t;
+    int index_bits = 1;
+    while (src.n >> index_bits) ++index_bits;
+    int64_t part_len = 0, parts = tile_parts(batch, src.n, part_len);
+    const dim3 block(TR_THREADS);
+    if (parts == 1) {
+        return run_last<T, false>(n_rows, src, k, (unsigned)src.n, index_bits, part_len, items_out, scores_out,
+                                  st);
+    }
+    hipLaunchKernelGGL((topk_tile_kernel<T, false, false, TR_THREADS, TR_TILE>), dim3((unsigned)(parts * n_rows)), block, 0, st, src,
+                       k, (unsigned)src.n, index_bits, (unsigned)parts, part_len, kept, (int32_t *)nullptr,
+                       (T *)nullptr);
+    ALSMI_HIP_CHECK(hipGetLastError());
+    // the levels alternate between the two parts of the workspace
+    key_t *from = kept, *to = kept + n_rows * parts * k;
+    for (;;) {
+        const int64_t n = parts * k;
+        const KeySource<T, true> left = {from, n, n};
+        parts = tile_parts(batch, n, part_len);
+        if (parts == 1) {
+            return run_last<T, true>(n_rows, left, k, (unsigned)src.n, index_bits, part_len, items_out,
+                                     scores_out, st);
+        }
+        hipLaunchKernelGGL((topk_tile_kernel<T, true, false, TR_THREADS, TR_TILE>), dim3((unsigned)(parts * n_rows)), block, 0, st,
+                           left, k, (unsigned)src.n, index_bits, (unsigned)parts, part_len, to,
+                           (int32_t *)nullptr, (T *)nullptr);
+        ALSMI_HIP_CHECK(hipGetLastError());
+        std::swap(from, to);
+    }
 }
 
 template <typename T>
@@ -592,13 +699,13 @@ static int run_topk_rows(int64_t n_rows, int64_t n_items, const void *scores, in
     typedef typename RowKey<T>::type key_t;
     T *so = static_cast<T *>(scores_out);
     key_t *kept = static_cast<key_t *>(workspace);
-    const int64_t most = batch_rows(n_items, k);  // (the workspace serves one batch after the other)
-    for (int64_t lo = 0; lo < n_rows; lo += most) {
-        const int64_t rows = std::min(n_rows - lo, most);
+    const int64_t batch = batch_rows(n_rows);  // (the workspace serves one batch after the other)
+    const bool lists = by_lists(n_rows, n_items, k);
+    for (int64_t lo = 0; lo < n_rows; lo += batch) {
+        const int64_t rows = std::min(n_rows - lo, batch);
         const KeySource<T, false> src = {static_cast<const T *>(scores) + lo * ld, ld, n_items};
-        const int status = k <= TR_LIST
-                               ? run_lists<T>(rows, src, k, items_out + lo * k, so + lo * k, kept, st)
-                               : run_tiles<T>(rows, src, k, items_out + lo * k, so + lo * k, kept, st);
+        const int status = lists ? run_lists<T>(rows, batch, src, k, items_out + lo * k, so + lo * k, kept, st)
+                                 : run_tiles<T>(rows, batch, src, k, items_out + lo * k, so + lo * k, kept, st);
         if (status != ALSMI_OK) return status;
     }
     return ALSMI_OK;
@@ -613,17 +720,16 @@ size_t alsmi_topk_rows_workspace_bytes(int dtype, int64_t n_rows, int64_t n_item
     if (dtype < ALSMI_F32 || dtype > ALSMI_BF16 || n_rows < 0 || n_items < 0 || k < 1 || k > TR_MAX_K)
         return 0;
     if (n_rows == 0 || n_items == 0) return 16;
-    int64_t keys = 0;
-    n_rows = std::min(n_rows, batch_rows(n_items, k));
-    if (k <= TR_LIST) {
-        int64_t part_len = 0;
-        const int64_t parts = list_parts(n_rows, n_items, part_len);
-        keys = parts > 1 ? parts * k : 0;
-    } else if (n_items > TR_LAST) {
-        const int64_t n = tiles_of(n_items) * k;
-        keys = n + (n > TR_LAST ? tiles_of(n) * k : 0);
+    const int64_t batch = batch_rows(n_rows);
+    int64_t keys = 0, part_len = 0;
+    if (by_lists(n_rows, n_items, k)) {
+        const int64_t parts = list_parts(batch, n_items, part_len);
+        if (parts > 1) keys = parts * k;
+    } else {
+        const int64_t parts = tile_parts(batch, n_items, part_len);
+        if (parts > 1) keys = (parts + tile_parts(batch, parts * k, part_len)) * k;
     }
-    return (size_t)n_rows * (size_t)keys * (dtype == ALSMI_F64 ? 16 : 8) + 16;
+    return (size_t)batch * (size_t)keys * (dtype == ALSMI_F64 ? 16 : 8) + 16;
 }
 
 int alsmi_topk_rows(int dtype, int64_t n_rows, int64_t n_items, const void *scores, int64_t ld_scores,

@@ -785,3 +785,24 @@ def test_offsets_past_32_bits():
     check_scores(host(rk.mx4_scores(table, last, rows=ids[-3:])), a, values, F32)
     many = torch.cat((ids, ids, ids))
     check_scores(host(rk.mx4_scores(table, last, rows=many)), np.tile(values, (3, 1)), values, F32)
+
+
+@pytest.mark.parametrize('n,m,k,limit', [(4, 5000000, 10, 3), (4, 1000000, 64, 3), (502, 100000, 1000, 400)])
+def test_topk_of_a_last_batch_of_fewer_rows(n, m, k, limit):
+    """A rest of the rows, which is cut into more parts than a full batch; the workspace is not left."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(n)
+    s = torch.randn(n, m, generator=g, device='cuda')
+    need = rk._lib.load().alsmi_topk_rows_workspace_bytes
+    items, best = rk.topk_rows(s, k, max_workspace_bytes=limit * need(0, 1, m, k))
+    want, order = torch.sort(s, dim=1, descending=True, stable=True)
+    assert torch.equal(best, want[:, :k]) and torch.equal(items, order[:, :k].to(torch.int32))
+    del want, order
+    for rows in (1, 2, 100, 102, 128, 129, n):
+        if rows > n:
+            continue
+        size = need(0, rows, m, k)
+        ws = torch.full((size + 4096,), 77, dtype=torch.uint8, device='cuda')
+        rk._call(s.device, 'alsmi_topk_rows', 0, rows, m, s.data_ptr(), m, k, items.data_ptr(),
+                 best.data_ptr(), ws.data_ptr())
+        assert bool((ws[size:] == 77).all())
