@@ -10,13 +10,13 @@
 //   or below the k-th best is dropped by one comparison, the few others wait in LDS until 64 of them
 //   are sorted and merged into the list at once.  Four waves per workgroup, as many workgroups per row
 //   as fill the chip; a second launch merges their lists.  Bound by the reads for many rows (1024 x
-//   26744 fp32, k = 10: 24 us, 4.6 TB/s), by two launches' latencies for one (1 x 1000000: 14 us).
+//   26744 fp32, k = 10: 23.4 us, 4.7 TB/s), by two launches' latencies for one (1 x 1000000: 14 us).
 // Larger k: a workgroup of 512 threads keeps the k best of its part of the row: of the first 8192 keys,
 //   held in registers, it finds the k-th largest by a radix descent over LDS histograms (2048 bins
 //   a digit), from then on only keys above it are looked at again.  Parts as many as run at once;
 //   the kept keys of a row's parts are the next, much shorter, row.  The last level sorts.  Bound by
 //   the latencies of the descent and the sort (1024 x 26744 fp32, k = 100: 44 us, 1000: 70; 37 x
-//   100003 bf16, k = 1000: 31).
+//   100003 bf16, k = 1000: 30).
 #include "alsmi_common.h"
 #include "elem.h"
 
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256) void topk_list_kernel(KeySource<T, FROM_KEYS> 
         for (int j = 0; j < LOADS; ++j)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) now[j][i] = raw[j][i];
-        if (!SHORT) fetch(at + 4 * TR_CHUNK);  // (on its way while this chunk is looked at)
+        if (!SHORT && at + 4 * TR_CHUNK < end) fetch(at + 4 * TR_CHUNK);  // (on its way while this chunk is looked at)
         auto key_at = [&](int j, int i) {
             return source::key(now[j][i], at + (j * 64 + lane) * VEC + i, end);
         };
@@ -518,7 +518,7 @@ __global__ __launch_bounds__(THREADS) void topk_tile_kernel(KeySource<T, FROM_KE
                                                       (n_items - (unsigned)at)
                                                 : (key_t)0;
             }
-        fetch(at0 + TILE);  // (on its way while this one is looked at)
+        if (at0 + TILE < end) fetch(at0 + TILE);  // (on its way while this one is looked at)
         if constexpr (!SORT) {
             if (first + TILE >= end) {  // the only tile: straight from the registers
                 key_t *dst = kept + (row * parts + part) * k;
