@@ -806,3 +806,72 @@ def test_topk_of_a_last_batch_of_fewer_rows(n, m, k, limit):
         rk._call(s.device, 'alsmi_topk_rows', 0, rows, m, s.data_ptr(), m, k, items.data_ptr(),
                  best.data_ptr(), ws.data_ptr())
         assert bool((ws[size:] == 77).all())
+
+
+@pytest.mark.parametrize('dtype', [F32, F64, F16, BF16])
+@pytest.mark.parametrize('n,m', [(600, 30011), (1100, 8193), (3, 70000), (130, 40000)])
+def test_topk_of_ordered_rows(n, m, dtype):
+    """Rows in which every key beats the ones before it, none does, all are equal, hardly any is
+    there, or they come in runs: the most and the fewest candidates a walk can meet."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(n)
+    up = torch.arange(m, device='cuda', dtype=F32) / 3 - 5000
+    few = torch.full((m,), -INF, device='cuda')
+    few[m - 30:] = torch.randn(30, generator=g, device='cuda')
+    rows = [up, -up, torch.zeros_like(up), few, few.flip(0), up % 97, -(up % 8192), up.abs(),
+            torch.randn(m, generator=g, device='cuda'),
+            torch.randint(-3, 3, (m,), generator=g, device='cuda').to(F32)]
+    rows = torch.stack([r.to(dtype) for r in rows])
+    # an order of the whole block by the order of its ten rows
+    which = torch.arange(n, device='cuda') % len(rows)
+    s = rows[which]
+    want, order = torch.sort(rows + 0.0, dim=1, descending=True, stable=True)  # (+0 and -0 as one)
+    s = s + 0.0
+    for k in (1, 24, 25, 64, 65, 300, 1000, 1024):
+        items, best = rk.topk_rows(s, k)
+        assert torch.equal(items, order[:, :k].to(torch.int32)[which])
+        assert torch.equal(best, want[:, :k][which])
+
+
+def test_every_form_captured_and_replayed():
+    """Calls of each form in a graph of their own, replayed on other inputs in the same memory with
+    eager work between the replays."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(9)
+    rand = lambda *shape: torch.randn(*shape, generator=g, device='cuda')
+    forms = []
+    for m, n, width in ((1, 3000, 64), (40, 3000, 200), (5, 3000, 900), (300, 9000, 520),
+                        (1020, 16300, 520), (50, 700, 300)):
+        table = rk.mx4_quantize(rand(n, width))
+        for dtype in (F32, BF16):
+            a = rand(m, width).to(dtype)
+            forms.append((a, lambda a=a, t=table: rk.mx4_scores(a, t, out_dtype=F32)))
+        a = rand(m, width)
+        forms.append((a, lambda a=a, t=table: rk.mx4_scores(rk.mx4_quantize(a), t)))
+    for n, m, k in ((1, 50000, 10), (2, 900, 7), (1, 50000, 60), (3, 70000, 500), (700, 20000, 100),
+                    (1, 1000000, 1024)):
+        s = rand(n, m)
+        forms.append((s, lambda s=s, k=k: rk.topk_rows(s, k)))
+    ptr = torch.arange(0, 401, 100, device='cuda')
+    ids = torch.randint(0, 9000, (400,), generator=g, device='cuda').to(torch.int32)
+    s = rand(4, 9000)
+    forms.append((s, lambda s=s: rk.adjust_scores(s, history=(ptr, ids), repetition=1.5, presence=0.5,
+                                                  row_bias=(ptr, ids, s[0, :400].clone()))))
+    forms.append((s, lambda s=s: rk.mx4_dequantize(rk.mx4_quantize(s))))
+    graphs = []
+    for source, call in forms:
+        call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out if isinstance(out, tuple) else (out,)))
+    for step in range(3):
+        for source, _ in forms:
+            source.copy_(torch.randn(source.shape, generator=g, device='cuda'))
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, call), (_, out) in zip(forms, graphs):
+            want = call()
+            for a, b in zip(out, want if isinstance(want, tuple) else (want,)):
+                assert torch.equal(a, b)
