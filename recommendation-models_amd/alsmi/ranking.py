@@ -110,10 +110,10 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
-def _result(name, out, shape, dtype, device, *sources):
-    """`out` checked, or a new tensor, and its row stride."""
+def _result(name, out, shape, dtype, like, *sources):
+    """`out` checked, or a new tensor on the device of `like`, and its row stride."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device), shape[1]
+        return like.new_empty(shape, dtype=dtype), shape[1]
     ld = _matrix(name, out, (dtype,))
     if tuple(out.shape) != tuple(shape):
         raise ValueError('%s must have shape %s, got %s' % (name, tuple(shape), tuple(out.shape)))
@@ -178,8 +178,8 @@ def mx4_quantize(x):
         raise ValueError('x must have between 1 and %d columns, got %d' % (MAX_WIDTH, width))
     device = _device(x)
     blocks = (width + BLOCK - 1) // BLOCK
-    codes = torch.empty((n, blocks * 16), dtype=torch.uint8, device=device)
-    scales = torch.empty((n, blocks), dtype=torch.uint8, device=device)
+    codes = x.new_empty((n, blocks * 16), dtype=torch.uint8)
+    scales = x.new_empty((n, blocks), dtype=torch.uint8)
     _call(device, 'alsmi_mx4_quantize', _CODES[x.dtype], n, width, _p(x), ld, _p(codes),
           _p(scales))
     return Mx4Table._of(codes, scales, width)
@@ -195,7 +195,7 @@ def mx4_dequantize(table, dtype=torch.float32, rows=None, out=None):
     if rows is not None:
         _vector('rows', rows, torch.int32)
     n = len(table) if rows is None else rows.numel()
-    out, ld = _result('out', out, (n, table.width), dtype, table.device, table.codes, table.scales,
+    out, ld = _result('out', out, (n, table.width), dtype, table.codes, table.codes, table.scales,
                       rows)
     device = _device(table.codes, table.scales, rows, out)
     _call(device, 'alsmi_mx4_dequantize', _CODES[dtype], n, _p(rows), len(table), table.width,
@@ -219,26 +219,25 @@ def mx4_scores(a, table, rows=None, out_dtype=None, out=None):
     else:
         ld, data, a_scales = _matrix('a', a, _NARROW), a, None
         code = _CODES[a.dtype]
-    if a.shape[1] != table.width:
-        raise ValueError('a has %d columns, the table %d' % (a.shape[1], table.width))
+    codes, scales, width = table.codes, table.scales, table.width
+    n, (n_rows, a_width) = codes.shape[0], a.shape
+    if a_width != width:
+        raise ValueError('a has %d columns, the table %d' % (a_width, width))
     if rows is not None:
         _vector('rows', rows, torch.int32)
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else (torch.float32 if held else a.dtype)
     if out_dtype not in _NARROW:
         raise ValueError('out_dtype must be one of %s' % ', '.join(str(d) for d in _NARROW))
-    m = a.shape[0] if rows is None else rows.numel()
-    if m and a.shape[0] == 0:
+    m = n_rows if rows is None else rows.numel()
+    if m and n_rows == 0:
         raise ValueError('rows of an empty a')
-    out, ldo = _result('out', out, (m, len(table)), out_dtype, table.device, data, a_scales, rows,
-                       table.codes, table.scales)
-    device = _device(table.codes, table.scales, data, a_scales, rows, out)
-    n, width = table.shape
+    out, ldo = _result('out', out, (m, n), out_dtype, codes, data, a_scales, rows, codes, scales)
+    device = _device(codes, scales, data, a_scales, rows, out)
     size = _lib.load().alsmi_mx4_scores_workspace_bytes(code, m, n, width)
-    ws = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _call(device, 'alsmi_mx4_scores', code, m, _p(rows), a.shape[0], data.data_ptr(), ld,
-          _p(a_scales), n, width, table.codes.data_ptr(), table.scales.data_ptr(),
-          _CODES[out_dtype], out.data_ptr(), ldo, _p(ws))
+    ws = codes.new_empty(size) if size else None
+    _call(device, 'alsmi_mx4_scores', code, m, _p(rows), n_rows, data.data_ptr(), ld, _p(a_scales), n,
+          width, codes.data_ptr(), scales.data_ptr(), _CODES[out_dtype], out.data_ptr(), ldo, _p(ws))
     return out
 
 
@@ -363,7 +362,7 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
     elif mask_rows is not None:
         raise ValueError('mask_rows needs a mask')
     if out is not scores:
-        out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores.device, scores, *kept)
+        out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores, scores, *kept)
     else:
         args.ld_out = ld
         if any(_overlap(out, t) for t in kept):
@@ -385,8 +384,8 @@ def topk_rows(scores, k, max_workspace_bytes=1 << 30):
         raise ValueError('k must be between 1 and min(%d, number of items), got %r' % (MAX_K, k))
     device = _device(scores)
     code = _CODES[scores.dtype]
-    items = torch.empty((n, k), dtype=torch.int32, device=device)
-    best = torch.empty((n, k), dtype=scores.dtype, device=device)
+    items = scores.new_empty((n, k), dtype=torch.int32)
+    best = scores.new_empty((n, k))
     if n == 0:
         return items, best
     need = _lib.load().alsmi_topk_rows_workspace_bytes
@@ -396,7 +395,7 @@ def topk_rows(scores, k, max_workspace_bytes=1 << 30):
         batch = max(1, min(n, max_workspace_bytes // need(code, 1, m, k)))
         # (fewer rows are cut into more parts: the last batch may need more than a full one)
         size = max(need(code, batch, m, k), need(code, n % batch, m, k) if n % batch else 0)
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    ws = scores.new_empty(size, dtype=torch.uint8)
     for lo in range(0, n, batch):
         hi = min(n, lo + batch)
         part = scores if batch == n else scores[lo:hi]
