@@ -42,6 +42,19 @@ __device__ __forceinline__ unsigned long long abs_bits(double x) {
     return __builtin_bit_cast(unsigned long long, x) & 0x7fffffffffffffffull;
 }
 
+// The value of another lane of the group that a block shares, as a vector instruction: steps 1 and 2
+// exchange within four lanes, then all four agree and step 4 takes the other four's.
+template <int STEP>
+__device__ __forceinline__ unsigned group_lane(unsigned x) {
+    constexpr int CTRL = STEP == 1 ? 0xb1 : STEP == 2 ? 0x4e : 0x141;  // (lane ^ 1, lane ^ 2, mirror of 8)
+    return (unsigned)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true);
+}
+template <int STEP>
+__device__ __forceinline__ unsigned long long group_lane(unsigned long long x) {
+    return ((unsigned long long)group_lane<STEP>((unsigned)(x >> 32)) << 32) |
+           group_lane<STEP>((unsigned)x);
+}
+
 // E (4 or 8) elements to as many codes, element 0 in the lowest four bits.
 template <int E>
 __device__ __forceinline__ unsigned to_codes(const float (&x)[E], unsigned byte) {
@@ -137,11 +150,10 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(int64_t n_rows, int w
             const auto b = abs_bits(v[t][i]);
             m = b > m ? b : m;
         }
-#pragma unroll
-        for (int off = 1; off < LANES; off <<= 1) {
-            const auto b = __shfl_xor(m, off);
-            m = b > m ? b : m;
-        }
+        auto join = [&](auto b) { m = b > m ? b : m; };
+        join(group_lane<1>(m));
+        join(group_lane<2>(m));
+        if constexpr (LANES == 8) join(group_lane<4>(m));
         const unsigned byte = scale_byte(m);
         const unsigned c = to_codes(v[t], byte);
         if (!in[t]) continue;  // (a block's lanes are all in or all out)
