@@ -300,7 +300,8 @@ __global__ __launch_bounds__(256) void topk_list_kernel(KeySource<T, FROM_KEYS> 
         for (int j = 0; j < LOADS; ++j)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) now[j][i] = raw[j][i];
-        if (!SHORT && at + 4 * TR_CHUNK < end) fetch(at + 4 * TR_CHUNK);  // (on its way while this chunk is looked at)
+        // (the next chunk is on its way while this one is looked at)
+        if (!SHORT && at + 4 * TR_CHUNK < end) fetch(at + 4 * TR_CHUNK);
         auto key_at = [&](int j, int i) {
             return source::key(now[j][i], at + (j * 64 + lane) * VEC + i, end);
         };
@@ -671,9 +672,9 @@ static int run_tiles(int64_t n_rows, int64_t batch, const KeySource<T, false> &s
         return run_last<T, false>(n_rows, src, k, (unsigned)src.n, index_bits, part_len, items_out, scores_out,
                                   st);
     }
-    hipLaunchKernelGGL((topk_tile_kernel<T, false, false, TR_THREADS, TR_TILE>), dim3((unsigned)(parts * n_rows)), block, 0, st, src,
-                       k, (unsigned)src.n, index_bits, (unsigned)parts, part_len, kept, (int32_t *)nullptr,
-                       (T *)nullptr);
+    hipLaunchKernelGGL((topk_tile_kernel<T, false, false, TR_THREADS, TR_TILE>),
+                       dim3((unsigned)(parts * n_rows)), block, 0, st, src, k, (unsigned)src.n, index_bits,
+                       (unsigned)parts, part_len, kept, (int32_t *)nullptr, (T *)nullptr);
     ALSMI_HIP_CHECK(hipGetLastError());
     // the levels alternate between the two parts of the workspace
     key_t *from = kept, *to = kept + n_rows * parts * k;
@@ -685,9 +686,9 @@ static int run_tiles(int64_t n_rows, int64_t batch, const KeySource<T, false> &s
             return run_last<T, true>(n_rows, left, k, (unsigned)src.n, index_bits, part_len, items_out,
                                      scores_out, st);
         }
-        hipLaunchKernelGGL((topk_tile_kernel<T, true, false, TR_THREADS, TR_TILE>), dim3((unsigned)(parts * n_rows)), block, 0, st,
-                           left, k, (unsigned)src.n, index_bits, (unsigned)parts, part_len, to,
-                           (int32_t *)nullptr, (T *)nullptr);
+        hipLaunchKernelGGL((topk_tile_kernel<T, true, false, TR_THREADS, TR_TILE>),
+                           dim3((unsigned)(parts * n_rows)), block, 0, st, left, k, (unsigned)src.n,
+                           index_bits, (unsigned)parts, part_len, to, (int32_t *)nullptr, (T *)nullptr);
         ALSMI_HIP_CHECK(hipGetLastError());
         std::swap(from, to);
     }
