@@ -613,12 +613,13 @@ __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T
 
 // ---- large products of float activations ---------------------------------------------------------
 // A first kernel splits the activations into their bf16 parts, rows picked and padded to whole turns
-// (planes[p][row][steps * 64]); a second one forms 128 rows x 128 items per workgroup through LDS,
-// four waves of 64 x 64, in steps of 64 elements, two steps a turn.  Parts and codes go from
+// (planes[p][row][steps * 64]); a second one forms 128 rows x 64 WN items per workgroup through LDS,
+// 2 WN waves of 64 x 64, in steps of 64 elements, two steps a turn.  Parts and codes go from
 // memory straight into LDS, into two buffers; the codes become bf16 in registers, once per wave
 // and step for all parts of 64 rows.  Each part costs one matrix instruction: fp32 activations run at a
-// third of the bf16 rate (2000 x 16000 x 2000: bf16 158 us, 0.81 PFLOP/s, fp16 260, fp32 448).  Bound
-// by the barriers' waits for the loads, one step ahead.
+// third of the bf16 rate (2000 x 16000 x 2000: bf16 156 us, 0.82 PFLOP/s, fp16 255, fp32 338, 1.15 counted
+// by parts).  Bound by the loads of the parts (without them bf16 116, fp16 185, fp32 of WN = 2 336 instead
+// of 447; a third buffer changes nothing).
 constexpr int WT_ROWS = 128, WT_ITEMS = 128;
 
 template <typename T>
@@ -642,16 +643,17 @@ __global__ __launch_bounds__(256) void mx4_split_kernel(Rows rows, const T *__re
     }
 }
 
-template <typename TO, int NP>
-__global__ __launch_bounds__(256, NP > 2 ? 1 : 2) void mx4_scores_split_kernel(const u32x4 *__restrict__ planes,
-                                                                  const uint8_t *__restrict__ codes,
-                                                                  const uint8_t *__restrict__ scales,
-                                                                  int nb, ScoreStore o, int row_tiles) {
-    constexpr int MT = 4, NT = 4;
+template <typename TO, int NP, int WN>
+__global__ __launch_bounds__(128 * WN, NP > 2 && WN == 2 ? 1 : 2) void mx4_scores_split_kernel(
+    const u32x4 *__restrict__ planes, const uint8_t *__restrict__ codes,
+    const uint8_t *__restrict__ scales, int nb, ScoreStore o, int row_tiles) {
+    constexpr int MT = 4, NT = 4, THREADS = 128 * WN, ITEMS = 64 * WN;
+    constexpr int LA = WT_ROWS * 8 / THREADS;  // 16-byte loads per thread, part and step
+    static_assert(ITEMS * 2 == THREADS, "one block of codes per thread and step");
     // rows of the parts (eight chunks of eight elements each, permuted as in mx4_scores_tiled_kernel)
     // and of the items (two blocks each); separate arrays: see there
     __shared__ u32x4 sa0[NP * WT_ROWS * 8], sa1[NP * WT_ROWS * 8];
-    __shared__ u32x4 sb0[WT_ITEMS * 2], sb1[WT_ITEMS * 2];
+    __shared__ u32x4 sb0[ITEMS * 2], sb1[ITEMS * 2];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, q = lane & 15;
@@ -659,37 +661,37 @@ __global__ __launch_bounds__(256, NP > 2 ? 1 : 2) void mx4_scores_split_kernel(c
     const unsigned per = total >> 3, extra = total & 7u;
     const unsigned tile = xcd * per + (xcd < extra ? xcd : extra) + nth;
     const int64_t row_base = (int64_t)(tile % (unsigned)row_tiles) * WT_ROWS;
-    const int64_t item_base = (int64_t)(tile / (unsigned)row_tiles) * WT_ITEMS;
+    const int64_t item_base = (int64_t)(tile / (unsigned)row_tiles) * ITEMS;
     const int turns = (nb + 3) / 4;
     const int64_t units = (int64_t)turns * 16;  // chunks of a row of the planes
     auto b_row = [&](int i) {
         const int64_t r = item_base + i;
         return r < o.n_items ? r : o.n_items - 1;
     };
-    // A thread's slots in a part's rows: row 32 i + tid / 8, chunk (tid % 8) ^ (row / 2 % 8), the same
+    // A thread's slots in a part's rows: row THREADS / 8 i + tid / 8, chunk (tid % 8) ^ (row / 2 % 8), the same
     // for every i; its slot of the items: place tid / 2, block tid % 2.  The item at a place: the 16
     // items that a matrix operand reads at once lie side by side.
     const int chunk = (tid & 7) ^ (tid >> 4 & 7);
-    const u32x4 *asrc[4];
+    const u32x4 *asrc[LA];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t r = row_base + i * 32 + (tid >> 3);
+    for (int i = 0; i < LA; ++i) {
+        const int64_t r = row_base + i * (THREADS / 8) + (tid >> 3);
         asrc[i] = planes + (r < o.n_sel ? r : o.n_sel - 1) * units + chunk;
     }
     const int64_t plane = o.n_sel * units;
     const int place = tid >> 1;
-    const int64_t bsrc = b_row((place & 64) + item_of<TO>(place >> 4 & 3, place & 15)) * nb;
+    const int64_t bsrc = b_row((place & ~63) + item_of<TO>(place >> 4 & 3, place & 15)) * nb;
     auto load_step = [&](unsigned step, u32x4 *to_a, u32x4 *to_b) __attribute__((always_inline)) {
         // (one step is loaded past the last turn, and not used)
         const unsigned s = step < 2u * turns ? step : 0u;
 #pragma unroll
         for (int p = 0; p < NP; ++p)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < LA; ++i)
                 __builtin_amdgcn_global_load_lds(
                     (const __attribute__((address_space(1))) void *)(asrc[i] + p * plane + s * 8u),
-                    (__attribute__((address_space(3))) void *)&to_a[(p * 4 + i) * 256 + wave * 64], 16, 0,
-                    0);
+                    (__attribute__((address_space(3))) void *)&to_a[(p * LA + i) * THREADS + wave * 64], 16,
+                    0, 0);
         // (a block behind the row's end meets zeros of the activations: any codes will do)
         const unsigned k = 2u * s + (tid & 1);
         __builtin_amdgcn_global_load_lds(
@@ -1219,7 +1221,7 @@ static int run_both(const Rows &rows, const void *a, const uint8_t *a_scales, co
 // Whether a float product is split first: enough whole tiles (bf16, 128 x 16384 x 512 11.8 us against
 // 15.8 from memory, 512 x 4096 x 1024 18.9 against 27.6, but 128 x 8192 x 4096 53 against 48), for up
 // to 64 rows, which leave half of a tile empty, only long rows and more tiles (64 x 65536 x 2048 fp32
-// 107 against 133, 64 x 100000 x 512 fp32 62 against 43, 64 x 16384 x 4096 bf16 53 against 47).
+// 87 against 133, 64 x 100000 x 512 fp32 49 against 45, 64 x 16384 x 4096 bf16 53 against 47).
 static bool splits(int64_t n_sel, int64_t n_items, int nb) {
     const int64_t tiles = (n_sel + WT_ROWS - 1) / WT_ROWS * ((n_items + WT_ITEMS - 1) / WT_ITEMS);
     return n_sel > 64 ? nb > 8 && tiles >= 128 : n_sel > 32 && nb >= 32 && tiles >= 192;
@@ -1238,18 +1240,18 @@ static int64_t batch_rows(int dtype, int64_t n_sel, int64_t n_items, int nb) {
     return std::max<int64_t>(WT_ROWS, fit / WT_ROWS * WT_ROWS);
 }
 
-template <typename T, typename TO>
+template <typename T, typename TO, int WN>
 static int launch_split(const Rows &rows, const void *a, int width, const uint8_t *codes,
                         const uint8_t *scales, int nb, const ScoreStore &o, void *workspace,
                         hipStream_t st) {
     u32x4 *planes = static_cast<u32x4 *>(workspace);
     const int64_t row_tiles = (rows.n_sel + WT_ROWS - 1) / WT_ROWS;
-    const int64_t blocks = (o.n_items + WT_ITEMS - 1) / WT_ITEMS * row_tiles;
+    const int64_t blocks = (o.n_items + 64 * WN - 1) / (64 * WN) * row_tiles;
     hipLaunchKernelGGL((mx4_split_kernel<T>), dim3((unsigned)rows.n_sel), dim3(256), 0, st, rows,
                        static_cast<const T *>(a), width, (nb + 3) / 4 * 16, planes);
     ALSMI_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((mx4_scores_split_kernel<TO, Parts<T>::N>), dim3((unsigned)blocks), dim3(256), 0, st,
-                       planes, codes, scales, nb, o, (int)row_tiles);
+    hipLaunchKernelGGL((mx4_scores_split_kernel<TO, Parts<T>::N, WN>), dim3((unsigned)blocks),
+                       dim3(128 * WN), 0, st, planes, codes, scales, nb, o, (int)row_tiles);
     ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
 }
@@ -1258,8 +1260,16 @@ template <typename T, typename TO>
 static int run_scores(const Rows &rows, const void *a, int width, const uint8_t *codes,
                       const uint8_t *scales, int nb, const ScoreStore &o, bool split, void *workspace,
                       hipStream_t st) {
-    if (split)
-        return launch_split<T, TO>(rows, a, width, codes, scales, nb, o, workspace, st);
+    if (split) {
+        // 256 items a workgroup read each part half as often, which pays for three parts and enough
+        // tiles (65 x 40000 x 512 fp32 24.6 us against 33.4, 2048 x 16384 x 4096 629 against 819, but 128 x
+        // 16384 x 512 25.6 against 19.8; fp16 2000 x 16000 x 2000 257 against 262, bf16 171 against 156)
+        if constexpr (Parts<T>::N > 2) {
+            if ((rows.n_sel + WT_ROWS - 1) / WT_ROWS * ((o.n_items + 255) / 256) >= 128)
+                return launch_split<T, TO, 4>(rows, a, width, codes, scales, nb, o, workspace, st);
+        }
+        return launch_split<T, TO, 2>(rows, a, width, codes, scales, nb, o, workspace, st);
+    }
     const bool one = rows.n_sel <= 16;
     if (nb == 1)
         return one ? launch_narrow<T, TO, 1, 1, 2>(rows, a, width, codes, scales, nb, o, st)
