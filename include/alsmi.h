@@ -218,7 +218,7 @@ int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t 
  * its scales (a_scales is ignored otherwise).  rows as in alsmi_mx4_dequantize: a row of NaN where
  * there is no such row.  workspace: alsmi_mx4_scores_workspace_bytes() bytes, aligned to 16 (large
  * products of float activations split them there first, 256 MiB at a time or 128 rows); may be
- * NULL where that is 0. */
+ * NULL where that is 0; what is enough for some rows, items and width is for fewer. */
 size_t alsmi_mx4_scores_workspace_bytes(int dtype, int64_t n_sel, int64_t n_items, int64_t width);
 int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, const void *a,
                      int64_t ld_a, const uint8_t *a_scales, int64_t n_items, int64_t width,
@@ -264,7 +264,8 @@ int alsmi_adjust_scores(int dtype, const alsmi_adjust *args, const void *scores,
 
 /* The k largest scores of every row, best first, ties by the smaller index: items_out [n_rows x k]
  * int32, scores_out [n_rows x k] of dtype.  1 <= k <= min(1024, n_items); the order of scores is that
- * of alsmi_topk_items.  workspace: alsmi_topk_rows_workspace_bytes() bytes, aligned to 16. */
+ * of alsmi_topk_items.  workspace: alsmi_topk_rows_workspace_bytes() bytes, aligned to 16; what is
+ * enough for some rows, items and k is for fewer. */
 size_t alsmi_topk_rows_workspace_bytes(int dtype, int64_t n_rows, int64_t n_items, int k);
 int alsmi_topk_rows(int dtype, int64_t n_rows, int64_t n_items, const void *scores,
                     int64_t ld_scores, int k, int32_t *items_out, void *scores_out, void *workspace,

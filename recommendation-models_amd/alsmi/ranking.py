@@ -393,8 +393,7 @@ def topk_rows(scores, k, max_workspace_bytes=1 << 30):
     size = need(code, n, m, k)
     if size > max_workspace_bytes and n > 1:
         batch = max(1, min(n, max_workspace_bytes // need(code, 1, m, k)))
-        # (fewer rows are cut into more parts: the last batch may need more than a full one)
-        size = max(need(code, batch, m, k), need(code, n % batch, m, k) if n % batch else 0)
+        size = need(code, batch, m, k)
     ws = scores.new_empty(size, dtype=torch.uint8)
     for lo in range(0, n, batch):
         hi = min(n, lo + batch)

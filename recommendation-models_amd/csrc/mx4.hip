@@ -621,6 +621,7 @@ __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T
 // by parts).  Bound by the loads of the parts (without them bf16 116, fp16 185, fp32 of WN = 2 336 instead
 // of 447; a third buffer changes nothing).
 constexpr int WT_ROWS = 128, WT_ITEMS = 128;
+constexpr int64_t MX4_SPLIT_BYTES = (int64_t)256 << 20;  // of parts at a time
 
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_split_kernel(Rows rows, const T *__restrict__ a, int width,
@@ -1236,7 +1237,7 @@ static int parts_of(int dtype) {
 // items, or where they are split first, whole tiles of rows whose parts take 256 MiB.
 static int64_t batch_rows(int dtype, int64_t n_sel, int64_t n_items, int nb) {
     if (dtype == ALSMI_MX4 || !splits(n_sel, n_items, nb)) return (int64_t)1 << 22;
-    const int64_t fit = ((int64_t)256 << 20) / split_bytes(1, nb, parts_of(dtype));
+    const int64_t fit = MX4_SPLIT_BYTES / split_bytes(1, nb, parts_of(dtype));
     return std::max<int64_t>(WT_ROWS, fit / WT_ROWS * WT_ROWS);
 }
 
@@ -1384,7 +1385,9 @@ size_t alsmi_mx4_scores_workspace_bytes(int dtype, int64_t n_sel, int64_t n_item
     if (n_sel < 0 || n_items < 0 || width < 1 || width > MX4_MAX_WIDTH) return 0;
     const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
     if (!splits(n_sel, n_items, nb)) return 0;
-    return (size_t)split_bytes(std::min(n_sel, batch_rows(dtype, n_sel, n_items, nb)), nb, parts_of(dtype));
+    // (enough for fewer rows or items or a smaller width as well)
+    const int64_t all = split_bytes(n_sel, nb, parts_of(dtype)), least = split_bytes(WT_ROWS, nb, parts_of(dtype));
+    return (size_t)std::min(all, std::max(MX4_SPLIT_BYTES, least));
 }
 
 int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows, const void *a,

@@ -27,13 +27,14 @@
 namespace alsmi {
 
 constexpr int TR_MAX_K = 1024;
-constexpr int TR_LIST = 64;         // the longest list one wave keeps
+constexpr int TR_LIST = 64;         // the longest list one wave keeps,
+constexpr int TR_FEW = 24;          // and the longest kept whatever the rows
 constexpr int TR_CHUNK = 1024;      // keys a wave looks at per turn, 16 per lane
 constexpr int TR_PART = 4 * TR_CHUNK;
 constexpr int TR_THREADS = 512;     // larger k: threads of a workgroup, keys they look at per turn,
 constexpr int TR_TILE = 8192;
 constexpr int TR_LAST = 16384;      // keys of a last turn by 1024 threads,
-constexpr int TR_GROUPS = 1024;     // and workgroups that run at once
+constexpr int TR_GROUPS = 1024;     // and workgroups that a launch of few rows is cut into
 
 typedef unsigned __int128 u128;
 
@@ -588,10 +589,10 @@ __global__ __launch_bounds__(THREADS) void topk_tile_kernel(KeySource<T, FROM_KE
 }
 
 // ---- launches ------------------------------------------------------------------------------------
-// Lists: workgroups per row, so that the launch has about 1024, at least 4096 keys each.
+// Lists: workgroups per row, so that a launch has about TR_GROUPS, at least 4096 keys each.
 static int64_t list_parts(int64_t n_rows, int64_t n_items, int64_t &part_len) {
     const int64_t most = (n_items + TR_PART - 1) / TR_PART;
-    int64_t parts = most <= 4 ? 1 : 1024 / n_rows;  // (a second launch costs more than four turns)
+    int64_t parts = most <= 4 ? 1 : TR_GROUPS / n_rows;  // (a second launch costs more than four turns)
     parts = parts < 1 ? 1 : (parts > most ? most : parts);
     part_len = ((n_items + parts - 1) / parts + TR_PART - 1) / TR_PART * TR_PART;
     return (n_items + part_len - 1) / part_len;
@@ -608,7 +609,7 @@ static int64_t tile_parts(int64_t n_rows, int64_t n, int64_t &part_len) {
 // against 21 for 512 x 16384 and k = 32, but 28 against 18 for 1 x 1000000 and k = 64, 17.5 against 14 for
 // 1 x 100000 and k = 32 (14.4 either way for k = 10): a row of many parts has many lists to merge.
 static bool by_lists(int64_t n_rows, int64_t n_items, int k) {
-    return k <= 24 || (k <= TR_LIST && (n_rows > 128 || n_items <= 4 * TR_PART));
+    return k <= TR_FEW || (k <= TR_LIST && (n_rows > 128 || n_items <= 4 * TR_PART));
 }
 // Rows that are worked on at once: a launch has fewer than 2^32 threads.  Their number decides over the
 // parts of a row for a smaller rest as well, so that the workspace does.
@@ -721,16 +722,11 @@ size_t alsmi_topk_rows_workspace_bytes(int dtype, int64_t n_rows, int64_t n_item
     if (dtype < ALSMI_F32 || dtype > ALSMI_BF16 || n_rows < 0 || n_items < 0 || k < 1 || k > TR_MAX_K)
         return 0;
     if (n_rows == 0 || n_items == 0) return 16;
-    const int64_t batch = batch_rows(n_rows);
-    int64_t keys = 0, part_len = 0;
-    if (by_lists(n_rows, n_items, k)) {
-        const int64_t parts = list_parts(batch, n_items, part_len);
-        if (parts > 1) keys = parts * k;
-    } else {
-        const int64_t parts = tile_parts(batch, n_items, part_len);
-        if (parts > 1) keys = (parts + tile_parts(batch, parts * k, part_len)) * k;
-    }
-    return (size_t)batch * (size_t)keys * (dtype == ALSMI_F64 ? 16 : 8) + 16;
+    // enough for any number of rows up to n_rows, of items up to n_items and for any smaller k: rows of up
+    // to 16384 items are not cut, the parts of others at most TR_GROUPS (once more for the next level)
+    if (n_items <= 4 * TR_PART) return 16;
+    const int64_t parts = std::min<int64_t>(TR_GROUPS, n_rows * ((n_items + TR_PART - 1) / TR_PART));
+    return (size_t)parts * (size_t)k * (k > TR_FEW ? 2 : 1) * (dtype == ALSMI_F64 ? 16 : 8) + 16;
 }
 
 int alsmi_topk_rows(int dtype, int64_t n_rows, int64_t n_items, const void *scores, int64_t ld_scores,

@@ -242,3 +242,25 @@ def test_score_items_refuses():
             dev.score_items(3, *bad)
     with pytest.raises(ValueError):
         dev.score_items(3, users, U, V, out=torch.zeros(4, 8))
+
+
+def test_workspaces_serve_smaller_calls():
+    """A caller sizes a workspace for its largest call."""
+    from alsmi import _lib
+    lib = _lib.load()
+    rng = np.random.default_rng(5)
+    log = lambda top: int(np.exp(rng.random() * np.log(top)))
+    for _ in range(3000):
+        n, m, k = log(5000000), 1 + log(3000000), 1 + log(1023)
+        code = int(rng.integers(0, 4))
+        most = lib.alsmi_topk_rows_workspace_bytes(code, n, m, k)
+        assert most <= 2 * 1024 * 1024 * 16 + 16
+        assert lib.alsmi_topk_rows_workspace_bytes(code, log(n), m, k) <= most
+        assert lib.alsmi_topk_rows_workspace_bytes(code, n, log(m), k) <= most
+        assert lib.alsmi_topk_rows_workspace_bytes(code, n, m, log(k)) <= most
+        rows, width = log(20000), 1 + log(100000)
+        code = int(rng.choice([_lib.F32, _lib.F16, _lib.BF16, _lib.MX4]))
+        most = lib.alsmi_mx4_scores_workspace_bytes(code, rows, m, width)
+        assert most <= 1 << 28
+        for other in ((log(rows), m, width), (rows, log(m), width), (rows, m, log(width))):
+            assert lib.alsmi_mx4_scores_workspace_bytes(code, *other) <= most
