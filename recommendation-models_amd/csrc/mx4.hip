@@ -611,6 +611,21 @@ __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T
     }
 }
 
+// ---- loads straight into LDS ---------------------------------------------------------------------
+// 16 bytes per lane from `bytes` behind `from` + `offset` (both the same for the whole wave) to the
+// wave's 1024 bytes at `to`, lane by lane.  Through a buffer descriptor and not by address: while a
+// load of the latter kind is in flight the compiler lets every read of LDS wait for all reads before
+// it (2048 x 16384 x 4096 79 us instead of 76).
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+__device__ __forceinline__ buffer_t buffer_of(const void *from) {
+    constexpr int DATA_32 = 4 << 15;  // (4 GiB of 32-bit words, no stride)
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(from), 0, -1, DATA_32);
+}
+__device__ __forceinline__ void load_to_lds(buffer_t from, unsigned offset, unsigned bytes, u32x4 *to) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16,
+                                             (int)bytes, (int)offset, 0, 0);
+}
+
 // ---- large products of float activations ---------------------------------------------------------
 // A first kernel splits the activations into their bf16 parts, rows picked and padded to whole turns
 // (planes[p][row][steps * 64]); a second one forms 128 rows x 64 WN items per workgroup through LDS,
@@ -673,15 +688,18 @@ __global__ __launch_bounds__(128 * WN, NP > 2 && WN == 2 ? 1 : 2) void mx4_score
     // for every i; its slot of the items: place tid / 2, block tid % 2.  The item at a place: the 16
     // items that a matrix operand reads at once lie side by side.
     const int chunk = (tid & 7) ^ (tid >> 4 & 7);
-    const u32x4 *asrc[LA];
+    // (in bytes: the parts of a call take less than 4 GiB, a tile's codes 128 MiB at most)
+    const buffer_t a_mem = buffer_of(planes), b_mem = buffer_of(codes + item_base * nb * 16);
+    unsigned asrc[LA];
 #pragma unroll
     for (int i = 0; i < LA; ++i) {
         const int64_t r = row_base + i * (THREADS / 8) + (tid >> 3);
-        asrc[i] = planes + (r < o.n_sel ? r : o.n_sel - 1) * units + chunk;
+        asrc[i] = (unsigned)((r < o.n_sel ? r : o.n_sel - 1) * units + chunk) * 16u;
     }
-    const int64_t plane = o.n_sel * units;
+    const unsigned plane = (unsigned)(o.n_sel * units) * 16u;
     const int place = tid >> 1;
-    const int64_t bsrc = b_row((place & ~63) + item_of<TO>(place >> 4 & 3, place & 15)) * nb;
+    const unsigned bsrc =
+        (unsigned)(b_row((place & ~63) + item_of<TO>(place >> 4 & 3, place & 15)) - item_base) * (unsigned)nb;
     auto load_step = [&](unsigned step, u32x4 *to_a, u32x4 *to_b) __attribute__((always_inline)) {
         // (one step is loaded past the last turn, and not used)
         const unsigned s = step < 2u * turns ? step : 0u;
@@ -689,16 +707,11 @@ __global__ __launch_bounds__(128 * WN, NP > 2 && WN == 2 ? 1 : 2) void mx4_score
         for (int p = 0; p < NP; ++p)
 #pragma unroll
             for (int i = 0; i < LA; ++i)
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void *)(asrc[i] + p * plane + s * 8u),
-                    (__attribute__((address_space(3))) void *)&to_a[(p * LA + i) * THREADS + wave * 64], 16,
-                    0, 0);
+                load_to_lds(a_mem, p * plane + s * 128u, asrc[i],
+                            &to_a[(p * LA + i) * THREADS + wave * 64]);
         // (a block behind the row's end meets zeros of the activations: any codes will do)
         const unsigned k = 2u * s + (tid & 1);
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void *)(codes +
-                                                             (bsrc + (k < (unsigned)nb ? k : nb - 1)) * 16),
-            (__attribute__((address_space(3))) void *)&to_b[wave * 64], 16, 0, 0);
+        load_to_lds(b_mem, 0, (bsrc + (k < (unsigned)nb ? k : nb - 1)) * 16u, &to_b[wave * 64]);
     };
     const int wm = wave & 1, wn = wave >> 1;
     const int ar = wm * 64 + q, sa = ar >> 1 & 7;
@@ -976,25 +989,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
     };
     static_assert(THREADS / 8 % 32 == 0, "rows between a thread's slots");
     const unsigned ca = (tid & 7) ^ a_swz(tid >> 3), cb = (tid & 7) ^ b_swz(tid >> 3);
-    unsigned src[LA + LB];  // first block of the row (the host makes sure that 32 bits do)
+    // bytes of the thread's chunk of a step from the tile's first row on (from the table's where rows are
+    // picked: the host makes sure that 32 bits do)
+    const int64_t a_first = rows.ids ? 0 : row_base;
+    const buffer_t a_mem = buffer_of(acodes + a_first * nb * 16),
+                   b_mem = buffer_of(codes + item_base * nb * 16);
+    unsigned src[LA + LB];
 #pragma unroll
     for (int i = 0; i < LA + LB; ++i) {
         const int row = (i < LA ? i : i - LA) * (THREADS / 8) + (tid >> 3);
-        src[i] = (unsigned)(i < LA ? a_row(row) : b_row(row)) * (unsigned)nb;
+        src[i] = i < LA ? ((unsigned)(a_row(row) - a_first) * (unsigned)nb + ca) * 16u
+                        : ((unsigned)(b_row(row) - item_base) * (unsigned)nb + cb) * 16u;
     }
+    const int turns = nb / 16;
     auto load_step = [&](unsigned step, u32x4 *to) __attribute__((always_inline)) {
-        // (one step is loaded past the last turn, and not used: any block of the row will do)
-        auto held = [&](unsigned k) { return k < (unsigned)nb ? k : (unsigned)nb - 1u; };
-        const unsigned ka = held(8u * step + ca), kb = held(8u * step + cb);
+        // (one step is loaded past the last turn, and not used)
+        const unsigned s = step < 2u * turns ? step : 0u;
 #pragma unroll
-        for (int i = 0; i < LA + LB; ++i) {
-            const unsigned at = src[i] + (i < LA ? ka : kb);
-            const uint8_t *p = (i < LA ? acodes : codes) + ((uint64_t)at << 4);
-            // (the destination is the wave's: lane l writes the l-th 16 bytes behind it)
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void *)p,
-                (__attribute__((address_space(3))) void *)&to[i * THREADS + wave * 64], 16, 0, 0);
-        }
+        for (int i = 0; i < LA + LB; ++i)
+            load_to_lds(i < LA ? a_mem : b_mem, s * 128u, src[i], &to[i * THREADS + wave * 64]);
     };
     const uint8_t *scale_row = tid < BM ? ascales + a_row(tid) * nb : scales + b_row(tid - BM) * nb;
     typedef unsigned unaligned_t __attribute__((ext_vector_type(4), aligned(1)));
@@ -1044,7 +1057,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    const int turns = nb / 16;
     if (turns > 0) {
         u32x4 sr = *reinterpret_cast<const unaligned_t *>(scale_row);
         load_step(0, sc0);
@@ -1204,9 +1216,9 @@ static int run_both(const Rows &rows, const void *a, const uint8_t *a_scales, co
     const int64_t tiles = (rows.n_sel + 15) / 16 * ((o.n_items + 15) / 16);
     if (tiles < (nb >= 16 ? 2048 : 32768))
         return launch_both<TO, 2, 2, 4>(rows, a, a_scales, codes, scales, nb, o, st);
-    // (they count blocks in 32 bits and load 16 bytes at a time)
+    // (they load 16 bytes at a time and count a picked row's bytes in 32 bits)
     const bool aligned = (uintptr_t)a % 16 == 0 && (uintptr_t)codes % 16 == 0 &&
-                         rows.n_rows * nb < (int64_t)1 << 32 && o.n_items * nb < (int64_t)1 << 32;
+                         (!rows.ids || rows.n_rows * nb < (int64_t)1 << 28);
     if (!aligned || nb < 16) return launch_both<TO, 4, 4, 1>(rows, a, a_scales, codes, scales, nb, o, st);
     // A tile of 256 x 256 fills a CU and takes 1.15 times less per score than four of 128 x 128, two
     // of which run on a CU at a time; it loses where its last round is not full: 2048 x 16384 x
