@@ -947,8 +947,8 @@ __global__ __launch_bounds__(256) void mx4_scores_both_kernel(Rows rows,
 //    keeps all their operands.  The blocks of a row behind the last whole turn are read from memory.
 //  - An operand is needed every MT products; the reads are spread between them by hand.
 // Workgroups are dealt to the eight XCDs in contiguous ranges, so that neighbours in a cache
-// share their operands.  2048 x 16384 x 4096 -> bf16 79 us, 3.5 PFLOP/s; the matrix instructions alone
-// 54 us, without the stores 70, the reads of LDS and the loads into it the difference.
+// share their operands.  2048 x 16384 x 4096 -> bf16 74 us, 3.7 PFLOP/s; the matrix instructions alone
+// 54 us, the reads of LDS and the loads into it some 10 more, the stores the rest.
 template <typename TO, int WM, int WN, int MT, int NT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
     Rows rows, const uint8_t *__restrict__ acodes, const uint8_t *__restrict__ ascales,
