@@ -308,15 +308,32 @@ def csr_to_csc(indptr, indices, vals, shape):
     return cptr, cidx, cvals
 
 
+def _check_ranked(rank, users, row_table, col_table):
+    """What the kernels that score `users` (rows of `row_table`) against `col_table` rely on: ids
+    and tables as they read them, with the whole padded rank of every row."""
+    if row_table.dtype != col_table.dtype or col_table.device != row_table.device:
+        raise ValueError('factor tables must share a dtype and a device')
+    if row_table.dtype not in (torch.float32, torch.float64):
+        raise ValueError('factor tables must be float32 or float64, got %s' % row_table.dtype)
+    ld = padded_rank(rank)
+    for t in (row_table, col_table):
+        if t.dim() != 2 or t.shape[1] != ld or not t.is_contiguous():
+            raise ValueError('factor tables must be contiguous [rows x %d] for rank %d'
+                             % (ld, rank))
+    if users.dtype != torch.int32 or users.device != row_table.device or not users.is_contiguous():
+        raise ValueError('users must be a contiguous int32 tensor on the device of the tables')
+    if not row_table.is_cuda:
+        raise ValueError('tensors must be on a HIP device; there is no CPU fallback')
+
+
 def topk_items(rank, users, row_table, col_table, k, max_workspace_bytes=1 << 30):
     """The k best items of each user in `users` (int32 device tensor): (items int32 [n x k],
     scores [n x k]) device tensors, best first, ties by the smaller item id.  The users are
     processed in batches whose dense score block stays under `max_workspace_bytes`."""
     lib = _lib.load()
     device = row_table.device
+    _check_ranked(rank, users, row_table, col_table)
     n_sel, n_items = int(users.numel()), int(col_table.shape[0])
-    if users.dtype != torch.int32:
-        raise ValueError('users must be an int32 device tensor')
     if not 1 <= k <= min(1024, n_items):
         raise ValueError('k must be between 1 and min(1024, number of items), got %r' % (k,))
     np_dtype = np.float32 if row_table.dtype == torch.float32 else np.float64
@@ -342,11 +359,8 @@ def score_items(rank, users, row_table, col_table, out=None):
     select (src/als.py:347-364 for a block of users).  `users` must be rows of `row_table`: the
     ids are not looked at."""
     device = row_table.device
+    _check_ranked(rank, users, row_table, col_table)
     n_sel, n_items = int(users.numel()), int(col_table.shape[0])
-    if users.dtype != torch.int32 or users.device != device or not users.is_contiguous():
-        raise ValueError('users must be a contiguous int32 tensor on the device of the tables')
-    if row_table.dtype != col_table.dtype or col_table.device != device:
-        raise ValueError('factor tables must share a dtype and a device')
     np_dtype = np.float32 if row_table.dtype == torch.float32 else np.float64
     if out is None:
         out = torch.empty((n_sel, n_items), dtype=row_table.dtype, device=device)

@@ -264,3 +264,33 @@ def test_workspaces_serve_smaller_calls():
         assert most <= 1 << 28
         for other in ((log(rows), m, width), (rows, log(m), width), (rows, m, log(width))):
             assert lib.alsmi_mx4_scores_workspace_bytes(code, *other) <= most
+
+
+BAD_TABLES = {
+    'bf16': (lambda u, U, V: (u, U.bfloat16(), V.bfloat16()), 'float32 or float64'),
+    'fp16': (lambda u, U, V: (u, U.half(), V.half()), 'float32 or float64'),
+    'integers': (lambda u, U, V: (u, U.int(), V.int()), 'float32 or float64'),
+    'two types': (lambda u, U, V: (u, U, V.double()), 'share a dtype'),
+    'the rank alone': (lambda u, U, V: (u, U[:, :3], V), 'contiguous'),
+    'items: the rank alone': (lambda u, U, V: (u, U, V[:, :3].contiguous()), 'contiguous'),
+    'another rank': (lambda u, U, V: (u, torch.zeros(5, 32), torch.zeros(7, 32)), 'contiguous'),
+    'every other row': (lambda u, U, V: (u, U[::2], V), 'contiguous'),
+    'columns': (lambda u, U, V: (u, U, torch.zeros(16, 7).t()), 'contiguous'),
+    '1-D': (lambda u, U, V: (u, U.view(-1), V), 'contiguous'),
+    'user type': (lambda u, U, V: (u.long(), U, V), 'users'),
+    'every other user': (lambda u, U, V: (u[::2], U, V), 'users'),
+    'host': (lambda u, U, V: (u, U, V), 'HIP device'),
+}
+
+
+@pytest.mark.parametrize('name', sorted(BAD_TABLES))
+def test_tables_that_the_kernels_would_misread_are_refused(name):
+    """The kernels take whole padded rows of fp32 or fp64, one behind the other: 16-bit tables would be
+    read (and scores written) past their ends, narrower ones at wrong offsets."""
+    from alsmi import device as dev
+    make, match = BAD_TABLES[name]
+    users, U, V = make(torch.zeros(4, dtype=torch.int32), torch.zeros(5, 16), torch.zeros(7, 16))
+    with pytest.raises(ValueError, match=match):
+        dev.score_items(3, users, U, V)
+    with pytest.raises(ValueError, match=match):
+        dev.topk_items(3, users, U, V, 2)
