@@ -182,9 +182,13 @@ int alsmi_topk_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
 
 /* The dense score block that alsmi_topk_items ranks: out [n_sel x n_items] of dtype,
  * out[p, i] = <user_factors[users[p]], item_factors[i]>, by the same kernels (ALSMI_F32: scaled fp16
- * split, fp32 accuracy).  For callers that change the scores before they select from them.  As there
- * users[] must be rows of user_factors: the ids are not looked at.
+ * split, fp32 accuracy).  For callers that change the scores before they select from them.
+ * alsmi_score_rows takes the number of rows of user_factors: an id outside 0 .. n_users-1 gives a row
+ * of NaN.  alsmi_score_items leaves it to its caller that users[] are rows of user_factors.
  * workspace: 16 bytes, aligned to 4. */
+int alsmi_score_rows(int dtype, int rank, int64_t n_sel, const int32_t *users, int64_t n_users,
+                     const void *user_factors, const void *item_factors, int64_t n_items,
+                     void *scores_out, void *workspace, void *stream);
 int alsmi_score_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
                       const void *user_factors, const void *item_factors, int64_t n_items,
                       void *scores_out, void *workspace, void *stream);

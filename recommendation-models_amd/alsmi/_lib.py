@@ -70,6 +70,8 @@ def load():
         'alsmi_topk_workspace_bytes': (ctypes.c_size_t, [c_int, c_i64, c_i64]),
         'alsmi_topk_items': (c_int, [c_int, c_int, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_vp,
                                      c_vp, c_vp, c_vp]),
+        'alsmi_score_rows': (c_int, [c_int, c_int, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp,
+                                     c_vp, c_vp]),
         'alsmi_score_items': (c_int, [c_int, c_int, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp,
                                       c_vp]),
         'alsmi_mx4_quantize': (c_int, [c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp]),
@@ -107,9 +109,9 @@ EXPORTS = ('alsmi_version', 'alsmi_last_error', 'alsmi_padded_rank', 'alsmi_plan
            'alsmi_half_sweep_err',
            'alsmi_normal_equations', 'alsmi_sddmm_workspace_bytes', 'alsmi_sddmm',
            'alsmi_sddmm_noalloc', 'alsmi_topk_workspace_bytes', 'alsmi_topk_items',
-           'alsmi_score_items', 'alsmi_mx4_quantize', 'alsmi_mx4_dequantize',
-           'alsmi_mx4_scores', 'alsmi_mx4_scores_workspace_bytes', 'alsmi_adjust_scores',
-           'alsmi_topk_rows_workspace_bytes', 'alsmi_topk_rows',
+           'alsmi_score_rows', 'alsmi_score_items', 'alsmi_mx4_quantize',
+           'alsmi_mx4_dequantize', 'alsmi_mx4_scores', 'alsmi_mx4_scores_workspace_bytes',
+           'alsmi_adjust_scores', 'alsmi_topk_rows_workspace_bytes', 'alsmi_topk_rows',
            'alsmi_expand_rows', 'alsmi_sparse_workspace_bytes', 'alsmi_build_csr',
            'alsmi_csr_to_csc', 'alsmi_imc_padded_width', 'alsmi_imc_workspace_bytes',
            'alsmi_imc_eval', 'alsmi_imc_project')

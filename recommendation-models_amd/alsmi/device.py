@@ -3,6 +3,7 @@
 torch is used for device memory, streams and (in ``dist.py``) collectives only;
 every arithmetic step is a libalsmi kernel.
 """
+import contextlib
 import ctypes
 
 import numpy as np
@@ -356,8 +357,8 @@ def topk_items(rank, users, row_table, col_table, k, max_workspace_bytes=1 << 30
 def score_items(rank, users, row_table, col_table, out=None):
     """The dense score block [n, n_items] of `users` (int32 device tensor) that ``topk_items``
     ranks: <row_table[users[p]], col_table[i]>, for callers that change the scores before they
-    select (src/als.py:347-364 for a block of users).  `users` must be rows of `row_table`: the
-    ids are not looked at."""
+    select (src/als.py:347-364 for a block of users); a row of NaN for a user that `row_table`
+    does not have."""
     device = row_table.device
     _check_ranked(rank, users, row_table, col_table)
     n_sel, n_items = int(users.numel()), int(col_table.shape[0])
@@ -369,8 +370,10 @@ def score_items(rank, users, row_table, col_table, out=None):
         raise ValueError('out must be contiguous [%d x %d] %s on the device of the tables'
                          % (n_sel, n_items, row_table.dtype))
     ws = torch.empty(4, dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
-        _lib.check(_lib.load().alsmi_score_items(
-            _lib.dtype_code(np_dtype), int(rank), n_sel, _ptr(users), _ptr(row_table),
-            _ptr(col_table), n_items, _ptr(out), _ptr(ws), _stream()), 'alsmi_score_items')
+    here = device.index == torch.cuda.current_device()  # (changing the device costs microseconds)
+    with contextlib.nullcontext() if here else torch.cuda.device(device):
+        _lib.check(_lib.load().alsmi_score_rows(
+            _lib.dtype_code(np_dtype), int(rank), n_sel, _ptr(users), int(row_table.shape[0]),
+            _ptr(row_table), _ptr(col_table), n_items, _ptr(out), _ptr(ws), _stream()),
+            'alsmi_score_rows')
     return out

@@ -93,7 +93,11 @@ struct ScoreOut {
     T *cand_score;
     int64_t n_wchunks;
     const int *run_if;     // when not null: the launch does nothing unless *run_if != 0
+    int64_t n_users;       // MODE 0: rows of U; an id outside them gets a row of NaN
+    __device__ __forceinline__ bool has_user(int64_t u) const { return u >= 0 && u < n_users; }
 };
+// (a caller that answers for its ids)
+constexpr int64_t TOPK_ANY_USER = INT64_MAX;
 
 // MODE 2 bookkeeping of one wave: cnt[t][r] = candidates found so far for the user of tile t,
 // register r of this lane's group (the same value in the 16 lanes of the group).  A hit takes
@@ -140,9 +144,16 @@ __global__ __launch_bounds__(256) void topk_scores_kernel(int n_sel, const int32
     for (int t = 0; t < UT; ++t) {
         int64_t ui = user_base + 16 * t + q;
         ui = ui < n_sel ? ui : n_sel - 1;  // (rows past the end are computed and not stored)
-        const T *row = U + (int64_t)sel[ui] * KP + g * KS;
+        int64_t u = sel[ui];
+        const bool none = MODE == 0 && !o.has_user(u);
+        if (none) u = 0;
+        const T *row = U + u * KP + g * KS;
 #pragma unroll
         for (int c = 0; c < KS; c += 4) load_vec<T, 4>(*reinterpret_cast<T(*)[4]>(&a[t][c]), row + c);
+        if (none) {
+#pragma unroll
+            for (int c = 0; c < KS; ++c) a[t][c] = (T)__builtin_nan("");
+        }
     }
     const int64_t wchunk = (int64_t)blockIdx.y * 4 + wl;
     key_t kthr[MODE == 2 ? UT : 1][4];
@@ -201,11 +212,12 @@ __global__ __launch_bounds__(256) void topk_scores_kernel(int n_sel, const int32
     }
 }
 
-// Largest |x| over the given rows of a table (rows[] when not null, else rows 0 .. n_rows-1) as
-// the bit pattern of a non-negative float, combined into *out with atomicMax (zeroed by the
+// Largest |x| over the given rows of a table (rows[] when not null, those outside 0 .. n_table-1
+// left out, else rows 0 .. n_rows-1) as the bit pattern of a non-negative float, combined into *out with atomicMax (zeroed by the
 // caller): the power-of-two scale of the fp16 split is taken from it.
 __global__ __launch_bounds__(256) void topk_max_abs_kernel(int64_t n_rows,
                                                            const int32_t *__restrict__ rows,
+                                                           int64_t n_table,
                                                            const float *__restrict__ table, int kp,
                                                            unsigned *__restrict__ out) {
     typedef float vec_t __attribute__((ext_vector_type(4)));
@@ -216,6 +228,7 @@ __global__ __launch_bounds__(256) void topk_max_abs_kernel(int64_t n_rows,
          i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / per_row;
         const int64_t src = rows ? (int64_t)rows[r] : r;
+        if (src < 0 || src >= n_table) continue;
         const vec_t v = reinterpret_cast<const vec_t *>(table + src * kp)[i - r * per_row];
         m = fmaxf(m, fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
     }
@@ -291,7 +304,14 @@ __global__ __launch_bounds__(256) void topk_scores_f16_kernel(int n_sel,
     for (int t = 0; t < UT; ++t) {
         int64_t ui = user_base + 16 * t + q;
         ui = ui < n_sel ? ui : n_sel - 1;  // (rows past the end are computed and not stored)
-        split_row<NS>(U + (int64_t)sel[ui] * KP, KP, g, su, ah[t], al[t]);
+        int64_t u = sel[ui];
+        const bool none = MODE == 0 && !o.has_user(u);
+        if (none) u = 0;
+        split_row<NS>(U + u * KP, KP, g, su, ah[t], al[t]);
+        if (none) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) ah[t][s] = al[t][s] = f16x8{} + (_Float16)__builtin_nanf("");
+        }
     }
     const int64_t wchunk = (int64_t)blockIdx.y * 4 + wl;
     float thr[MODE == 2 ? UT : 1][4];
@@ -906,9 +926,10 @@ static int run_topk(int n_sel, const int32_t *sel, const void *U, const void *V,
             return (unsigned)(b < 1 ? 1 : (b > 512 ? 512 : b));
         };
         hipLaunchKernelGGL(topk_max_abs_kernel, dim3(blocks_for(n_sel)), dim3(256), 0, st,
-                           (int64_t)n_sel, sel, reinterpret_cast<const float *>(Ut), kp, max_bits);
+                           (int64_t)n_sel, sel, TOPK_ANY_USER, reinterpret_cast<const float *>(Ut), kp,
+                           max_bits);
         hipLaunchKernelGGL(topk_max_abs_kernel, dim3(blocks_for(n_items)), dim3(256), 0, st, n_items,
-                           (const int32_t *)nullptr, reinterpret_cast<const float *>(Vt), kp,
+                           (const int32_t *)nullptr, n_items, reinterpret_cast<const float *>(Vt), kp,
                            max_bits + 1);
         ALSMI_HIP_CHECK(hipGetLastError());
     }
@@ -1044,6 +1065,7 @@ static int run_topk(int n_sel, const int32_t *sel, const void *U, const void *V,
     all.scores = scores;
     all.row_len = n_items;
     all.run_if = flag;
+    all.n_users = TOPK_ANY_USER;
     launch_scores<T, NV, 0>(grid_all, st, n_sel, sel, Ut, Vt, n_items, all, itw, max_bits);
     ALSMI_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL((topk_select_kernel<T>), dim3(n_sel), dim3(256), 0, st, scores, n_items, k,
@@ -1054,7 +1076,7 @@ static int run_topk(int n_sel, const int32_t *sel, const void *U, const void *V,
 
 // The dense score block alone (MODE 0 over all items).
 template <typename T, int NV>
-static int run_score_items(int n_sel, const int32_t *sel, const void *U, const void *V,
+static int run_score_items(int n_sel, const int32_t *sel, int64_t n_users, const void *U, const void *V,
                            int64_t n_items, void *out, void *workspace, hipStream_t st) {
     const T *Ut = static_cast<const T *>(U), *Vt = static_cast<const T *>(V);
     constexpr int UPW = score_users_per_wave<T, NV>();
@@ -1072,41 +1094,39 @@ static int run_score_items(int n_sel, const int32_t *sel, const void *U, const v
         };
         hipLaunchKernelGGL(topk_zero_kernel, dim3(1), dim3(2), 0, st, max_bits);
         hipLaunchKernelGGL(topk_max_abs_kernel, dim3(blocks_for(n_sel)), dim3(256), 0, st,
-                           (int64_t)n_sel, sel, reinterpret_cast<const float *>(Ut), kp, max_bits);
+                           (int64_t)n_sel, sel, n_users, reinterpret_cast<const float *>(Ut), kp,
+                           max_bits);
         hipLaunchKernelGGL(topk_max_abs_kernel, dim3(blocks_for(n_items)), dim3(256), 0, st, n_items,
-                           (const int32_t *)nullptr, reinterpret_cast<const float *>(Vt), kp,
+                           (const int32_t *)nullptr, n_items, reinterpret_cast<const float *>(Vt), kp,
                            max_bits + 1);
         ALSMI_HIP_CHECK(hipGetLastError());
     }
     ScoreOut<T> all = {};
     all.scores = static_cast<T *>(out);
     all.row_len = n_items;
+    all.n_users = n_users;
     launch_scores<T, NV, 0>(dim3((unsigned)user_blocks, (unsigned)chunks), st, n_sel, sel, Ut, Vt,
                             n_items, all, itw, max_bits);
     ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
 }
 
-}  // namespace alsmi
-
-extern "C" {
-
-int alsmi_score_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
-                      const void *user_factors, const void *item_factors, int64_t n_items,
-                      void *scores_out, void *workspace, void *stream) {
-    using namespace alsmi;
-    ALSMI_REQUIRE(dtype == ALSMI_F32 || dtype == ALSMI_F64, "alsmi_score_items: bad dtype %d", dtype);
+static int score_block(const char *name, int dtype, int rank, int64_t n_sel, const int32_t *users,
+                       int64_t n_users, const void *user_factors, const void *item_factors,
+                       int64_t n_items, void *scores_out, void *workspace, void *stream) {
+    ALSMI_REQUIRE(dtype == ALSMI_F32 || dtype == ALSMI_F64, "%s: bad dtype %d", name, dtype);
     const int kp = alsmi_padded_rank(rank);
-    ALSMI_REQUIRE(kp > 0, "alsmi_score_items: rank %d outside 1..128", rank);
+    ALSMI_REQUIRE(kp > 0, "%s: rank %d outside 1..128", name, rank);
     ALSMI_REQUIRE(n_sel >= 0 && n_sel < INT32_MAX && n_items >= 0 && n_items <= INT32_MAX,
-                  "alsmi_score_items: bad user or item count");
+                  "%s: bad user or item count", name);
     if (n_sel == 0 || n_items == 0) return ALSMI_OK;
+    ALSMI_REQUIRE(n_users > 0, "%s: rows of an empty table", name);
     ALSMI_REQUIRE(users && user_factors && item_factors && scores_out && workspace,
-                  "alsmi_score_items: null pointer");
+                  "%s: null pointer", name);
     hipStream_t st = static_cast<hipStream_t>(stream);
-#define ALSMI_CASE(T, NV)                                                                         \
-    return run_score_items<T, NV>((int)n_sel, users, user_factors, item_factors, n_items, scores_out, \
-                                  workspace, st)
+#define ALSMI_CASE(T, NV)                                                                            \
+    return run_score_items<T, NV>((int)n_sel, users, n_users, user_factors, item_factors, n_items,   \
+                                  scores_out, workspace, st)
     const bool f32 = dtype == ALSMI_F32;
     switch (kp) {
         case 16: if (f32) ALSMI_CASE(float, 1); else ALSMI_CASE(double, 1);
@@ -1115,6 +1135,24 @@ int alsmi_score_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
         default: if (f32) ALSMI_CASE(float, 8); else ALSMI_CASE(double, 8);
     }
 #undef ALSMI_CASE
+}
+
+}  // namespace alsmi
+
+extern "C" {
+
+int alsmi_score_rows(int dtype, int rank, int64_t n_sel, const int32_t *users, int64_t n_users,
+                     const void *user_factors, const void *item_factors, int64_t n_items,
+                     void *scores_out, void *workspace, void *stream) {
+    return alsmi::score_block("alsmi_score_rows", dtype, rank, n_sel, users, n_users, user_factors,
+                              item_factors, n_items, scores_out, workspace, stream);
+}
+
+int alsmi_score_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
+                      const void *user_factors, const void *item_factors, int64_t n_items,
+                      void *scores_out, void *workspace, void *stream) {
+    return alsmi::score_block("alsmi_score_items", dtype, rank, n_sel, users, alsmi::TOPK_ANY_USER,
+                              user_factors, item_factors, n_items, scores_out, workspace, stream);
 }
 
 size_t alsmi_topk_workspace_bytes(int dtype, int64_t n_sel, int64_t n_items) {

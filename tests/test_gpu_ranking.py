@@ -875,3 +875,24 @@ def test_every_form_captured_and_replayed():
             want = call()
             for a, b in zip(out, want if isinstance(want, tuple) else (want,)):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('rank,m', [(3, 40), (20, 700), (64, 2000), (100, 333)])
+@pytest.mark.parametrize('dtype', ['float32', 'float64'])
+def test_score_items_of_users_the_table_does_not_have(rank, m, dtype):
+    """Rows of NaN for them, and the other rows as without them (the smallest user has the largest
+    factors, so rows read in place of the missing ones would show in the scale too)."""
+    from alsmi import device as dev
+    device = dev.require_gpu()
+    rng = np.random.default_rng(rank)
+    U, V = rng.standard_normal((rank, 50)), rng.standard_normal((rank, m))
+    U[:, 0] *= 1e6
+    Ud, Vd = dev.factors_to_device(U, dtype, device), dev.factors_to_device(V, dtype, device)
+    users = rng.integers(1, 50, 150).astype(np.int32)
+    none = rng.random(150) < 0.2
+    users[none] = rng.choice([-1, 50, 51, -2 ** 31, 2 ** 31 - 1], none.sum())
+    got = dev.score_items(rank, gpu(users), Ud, Vd)
+    assert torch.equal(torch.isnan(got), gpu(none)[:, None].expand(-1, m))
+    want = dev.score_items(rank, gpu(users[~none]), Ud, Vd)
+    assert torch.equal(got[gpu(~none)], want)
+    assert bool(torch.isnan(dev.score_items(rank, gpu(users[none][:1]), Ud, Vd)).all())

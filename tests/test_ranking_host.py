@@ -294,3 +294,14 @@ def test_tables_that_the_kernels_would_misread_are_refused(name):
         dev.score_items(3, users, U, V)
     with pytest.raises(ValueError, match=match):
         dev.topk_items(3, users, U, V, 2)
+
+
+def test_score_rows_refuses():
+    lib = _lib.load()
+    p = ctypes.cast((ctypes.c_double * 64)(), ctypes.c_void_p)
+    for bad in ((2, 4, 1, p, 1, p, p, 1, p, p), (0, 129, 1, p, 1, p, p, 1, p, p),
+                (0, 4, 1, None, 1, p, p, 1, p, p), (0, 4, 1, p, 0, p, p, 1, p, p),
+                (0, 4, 1, p, 1, p, p, -1, p, p), (0, 4, 1, p, 1, p, p, 1, p, None)):
+        assert lib.alsmi_score_rows(*bad, None) == -1
+        assert b'alsmi_score_rows' in lib.alsmi_last_error()
+    assert lib.alsmi_score_rows(0, 4, 0, None, 0, None, None, 5, None, None, None) == 0
