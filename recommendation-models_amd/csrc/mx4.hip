@@ -91,19 +91,24 @@ constexpr int mx4_lane() {
     return sizeof(T) == 2 ? 8 : 4;
 }
 // How a workgroup covers rows: `upr` lanes' worth (units) a row, TURNS * 256 units per workgroup, as whole
-// rows (`rpb` of them) or as part blockIdx.y of one row.
+// rows (`rpb` of them) or as part blockIdx.y of one row.  A launch covers at most MX4_GROUPS workgroups
+// of rows (its x extent has to stay below 2^32 threads); the host takes longer tables batch by batch.
 constexpr int MX4_TURNS = 4;
+constexpr int64_t MX4_GROUPS = (int64_t)1 << 22;
 struct RowGrid {
     unsigned upr, rpb, inverse;  // inverse: 2^32 / upr rounded up
-    dim3 grid;
+    int64_t most;                // rows of a launch
+    dim3 grid(int64_t n_rows) const {
+        return dim3((unsigned)((n_rows + rpb - 1) / rpb), (upr + 256 * MX4_TURNS - 1) / (256 * MX4_TURNS));
+    }
 };
-static RowGrid row_grid(int64_t n_rows, int nb, int per_lane) {
+static RowGrid row_grid(int nb, int per_lane) {
     RowGrid r;
     constexpr unsigned UNITS = 256 * MX4_TURNS;
     r.upr = (unsigned)nb * (MX4_BLOCK / per_lane);
     r.rpb = r.upr < UNITS ? UNITS / r.upr : 1;
     r.inverse = (unsigned)((((uint64_t)1 << 32) + r.upr - 1) / r.upr);
-    r.grid = dim3((unsigned)((n_rows + r.rpb - 1) / r.rpb), (r.upr + UNITS - 1) / UNITS);
+    r.most = MX4_GROUPS * r.rpb;
     return r;
 }
 // Row and unit of a thread in a turn; false where there is none.  (x < 1024: the product is exact.)
@@ -1337,19 +1342,23 @@ int alsmi_mx4_quantize(int dtype, int64_t n_rows, int64_t width, const void *x, 
     const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
 #define ALSMI_CASE(T)                                                                                \
     do {                                                                                             \
-        const RowGrid rg = row_grid(n_rows, nb, mx4_lane<T>());                                      \
+        const RowGrid rg = row_grid(nb, mx4_lane<T>());                                              \
         auto kernel = n_rows * width * (int64_t)sizeof(T) > MX4_STREAM_BYTES                         \
                           ? mx4_quantize_kernel<T, true>                                             \
                           : mx4_quantize_kernel<T, false>;                                           \
-        hipLaunchKernelGGL(kernel, rg.grid, dim3(256), 0, st, n_rows, (int)width,                    \
-                           static_cast<const T *>(x), ldx, codes, scales, rg.upr, rg.rpb, rg.inverse); \
+        for (int64_t lo = 0; lo < n_rows; lo += rg.most) {                                           \
+            const int64_t n = std::min(n_rows - lo, rg.most);                                        \
+            hipLaunchKernelGGL(kernel, rg.grid(n), dim3(256), 0, st, n, (int)width,                  \
+                               static_cast<const T *>(x) + lo * ldx, ldx, codes + lo * nb * 16,      \
+                               scales + lo * nb, rg.upr, rg.rpb, rg.inverse);                        \
+            ALSMI_HIP_CHECK(hipGetLastError());                                                      \
+        }                                                                                            \
     } while (0)
     if (dtype == ALSMI_F32) ALSMI_CASE(float);
     else if (dtype == ALSMI_F64) ALSMI_CASE(double);
     else if (dtype == ALSMI_F16) ALSMI_CASE(_Float16);
     else ALSMI_CASE(__bf16);
 #undef ALSMI_CASE
-    ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
 }
 
@@ -1375,20 +1384,23 @@ int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t 
     const int nb = (int)((width + MX4_BLOCK - 1) / MX4_BLOCK);
 #define ALSMI_CASE(T)                                                                                 \
     do {                                                                                              \
-        const RowGrid rg = row_grid(n_sel, nb, mx4_lane<T>());                                        \
+        const RowGrid rg = row_grid(nb, mx4_lane<T>());                                               \
         auto kernel = n_sel * width * (int64_t)sizeof(T) > MX4_STREAM_BYTES                           \
                           ? mx4_dequantize_kernel<T, true>                                            \
                           : mx4_dequantize_kernel<T, false>;                                          \
-        hipLaunchKernelGGL(kernel, rg.grid, dim3(256), 0, st, n_sel, rows, n_rows,                    \
-                           (int)width, codes, scales, static_cast<T *>(out), ldo, rg.upr, rg.rpb,     \
-                           rg.inverse);                                                               \
+        for (int64_t lo = 0; lo < n_sel; lo += rg.most) {                                             \
+            const int64_t n = std::min(n_sel - lo, rg.most), skip = rows ? 0 : lo;                    \
+            hipLaunchKernelGGL(kernel, rg.grid(n), dim3(256), 0, st, n, rows ? rows + lo : nullptr,   \
+                               n_rows - skip, (int)width, codes + skip * nb * 16, scales + skip * nb, \
+                               static_cast<T *>(out) + lo * ldo, ldo, rg.upr, rg.rpb, rg.inverse);    \
+            ALSMI_HIP_CHECK(hipGetLastError());                                                       \
+        }                                                                                             \
     } while (0)
     if (dtype == ALSMI_F32) ALSMI_CASE(float);
     else if (dtype == ALSMI_F64) ALSMI_CASE(double);
     else if (dtype == ALSMI_F16) ALSMI_CASE(_Float16);
     else ALSMI_CASE(__bf16);
 #undef ALSMI_CASE
-    ALSMI_HIP_CHECK(hipGetLastError());
     return ALSMI_OK;
 }
 

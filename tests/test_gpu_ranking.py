@@ -896,3 +896,32 @@ def test_score_items_of_users_the_table_does_not_have(rank, m, dtype):
     want = dev.score_items(rank, gpu(users[~none]), Ud, Vd)
     assert torch.equal(got[gpu(~none)], want)
     assert bool(torch.isnan(dev.score_items(rank, gpu(users[none][:1]), Ud, Vd)).all())
+
+
+def test_tables_of_more_rows_than_a_launch_has_room_for():
+    """As many rows as a call takes, of one element: 2^24 workgroups of 256 threads and more.  Every row
+    is one of the same thirteen, which a small table quantises too."""
+    n, period = 2 ** 31 - 1, 13
+    small = torch.linspace(-6.5, 7.0, period, device='cuda')[:, None]
+    few = rk.mx4_quantize(small)
+    want = rk.mx4_dequantize(few)
+    ids = torch.arange(n, dtype=torch.int32, device='cuda').remainder_(period)
+    whole = n - n % period
+
+    def check(got, rest):
+        assert bool((got[:whole].view(-1, period) == want.view(1, period)).all())
+        assert torch.equal(got[whole:], want[:rest])
+    x = torch.empty(n, 1, device='cuda')
+    step = 1 << 28
+    for lo in range(0, n, step):
+        x[lo:lo + step, 0] = small[:, 0].index_select(0, ids[lo:lo + step])
+    table = rk.mx4_quantize(x)
+    assert torch.equal(table.codes[-period:], few.codes.roll(-(n % period), 0))
+    assert torch.equal(table.scales[-period:], few.scales.roll(-(n % period), 0))
+    x.fill_(NAN)
+    rk.mx4_dequantize(table, out=x)
+    check(x, n % period)
+    del table
+    x.fill_(NAN)
+    rk.mx4_dequantize(few, rows=ids, out=x)
+    check(x, n % period)
