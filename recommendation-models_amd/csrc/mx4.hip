@@ -1250,8 +1250,10 @@ static int64_t split_bytes(int64_t n_sel, int nb, int parts) {
 static int parts_of(int dtype) {
     return dtype == ALSMI_F32 ? 3 : dtype == ALSMI_F16 ? 2 : dtype == ALSMI_BF16 ? 1 : 0;
 }
-// Rows that a product takes at once: what a launch of fewer than 2^32 threads covers whatever the
-// items, or where they are split first, whole tiles of rows whose parts take 256 MiB.
+// Rows and items that a product takes at once, so that a launch has fewer than 2^32 threads: where the
+// waves of a workgroup share rows it covers no more than 32 items (and then up to 32 rows, or fewer
+// than 32768 tiles, are left).  Rows that are split first: whole tiles whose parts take 256 MiB.
+constexpr int64_t MX4_ITEMS = (int64_t)1 << 28;
 static int64_t batch_rows(int dtype, int64_t n_sel, int64_t n_items, int nb) {
     if (dtype == ALSMI_MX4 || !splits(n_sel, n_items, nb)) return (int64_t)1 << 22;
     const int64_t fit = MX4_SPLIT_BYTES / split_bytes(1, nb, parts_of(dtype));
@@ -1450,32 +1452,34 @@ int alsmi_mx4_scores(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_ro
     const int64_t out_size = out_dtype == ALSMI_F32 ? 4 : 2;
     // bytes of a row of the activations
     const int64_t a_row = dtype == ALSMI_MX4 ? 16 * nb : lda * (dtype == ALSMI_F32 ? 4 : 2);
-    for (int64_t lo = 0; lo < n_sel; lo += most) {
+    auto product = [&](int64_t lo, int64_t first) {
         const int64_t n = std::min(n_sel - lo, most), skip = rows ? 0 : lo;
         const Rows r = {n, n_rows - skip, lda, rows ? rows + lo : nullptr};
-        const ScoreStore o = {static_cast<char *>(out) + lo * ldo * out_size, ldo, n, n_items};
+        const ScoreStore o = {static_cast<char *>(out) + (lo * ldo + first) * out_size, ldo, n,
+                              std::min(n_items - first, MX4_ITEMS)};
         const void *from = static_cast<const char *>(a) + skip * a_row;
         const uint8_t *from_scales = a_scales ? a_scales + skip * nb : nullptr;
-        int status = ALSMI_OK;
+        const uint8_t *c = codes + first * nb * 16, *sc = scales + first * nb;
 #define ALSMI_CASE(TO)                                                                                  \
     do {                                                                                                \
         if (dtype == ALSMI_F32)                                                                         \
-            status = run_scores<float, TO>(r, from, (int)width, codes, scales, nb, o, split, workspace, st); \
-        else if (dtype == ALSMI_F16)                                                                    \
-            status =                                                                                    \
-                run_scores<_Float16, TO>(r, from, (int)width, codes, scales, nb, o, split, workspace, st); \
-        else if (dtype == ALSMI_BF16)                                                                   \
-            status =                                                                                    \
-                run_scores<__bf16, TO>(r, from, (int)width, codes, scales, nb, o, split, workspace, st); \
-        else                                                                                            \
-            status = run_both<TO>(r, from, from_scales, codes, scales, nb, o, st);                      \
+            return run_scores<float, TO>(r, from, (int)width, c, sc, nb, o, split, workspace, st);      \
+        if (dtype == ALSMI_F16)                                                                         \
+            return run_scores<_Float16, TO>(r, from, (int)width, c, sc, nb, o, split, workspace, st);   \
+        if (dtype == ALSMI_BF16)                                                                        \
+            return run_scores<__bf16, TO>(r, from, (int)width, c, sc, nb, o, split, workspace, st);     \
+        return run_both<TO>(r, from, from_scales, c, sc, nb, o, st);                                    \
     } while (0)
         if (out_dtype == ALSMI_F32) ALSMI_CASE(float);
-        else if (out_dtype == ALSMI_BF16) ALSMI_CASE(__bf16);
-        else ALSMI_CASE(_Float16);
+        if (out_dtype == ALSMI_BF16) ALSMI_CASE(__bf16);
+        ALSMI_CASE(_Float16);
 #undef ALSMI_CASE
-        if (status != ALSMI_OK) return status;
-    }
+    };
+    for (int64_t lo = 0; lo < n_sel; lo += most)
+        for (int64_t first = 0; first < n_items; first += MX4_ITEMS) {
+            const int status = product(lo, first);
+            if (status != ALSMI_OK) return status;
+        }
     return ALSMI_OK;
 }
 

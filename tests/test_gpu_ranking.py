@@ -925,3 +925,30 @@ def test_tables_of_more_rows_than_a_launch_has_room_for():
     x.fill_(NAN)
     rk.mx4_dequantize(few, rows=ids, out=x)
     check(x, n % period)
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'mx4'])
+def test_scores_of_more_items_than_a_launch_has_room_for(kind):
+    """2^29 items of a few rows' product, in the form whose workgroups take 32 of them each.  All
+    elements of an item are alike, so its score is known; the scores are small whole numbers."""
+    n, width = 2 ** 29 + 5, 257
+    blocks = (width + 31) // 32
+    codes = torch.empty(n, 16 * blocks, dtype=torch.uint8, device='cuda')
+    # items in the order 1, 1.5, -2, 0, 4, 1, ...; two codes a byte, +0 behind the width
+    lut = torch.tensor([0x22, 0x33, 0xcc, 0x00, 0x66], dtype=torch.uint8, device='cuda')
+    value = torch.tensor([1.0, 1.5, -2.0, 0.0, 4.0], device='cuda')
+    whole = n - n % 5
+    codes[:whole].view(-1, 5, 16 * blocks).copy_(lut.view(1, 5, 1))
+    codes[whole:] = lut[:n % 5, None]
+    codes[:, width // 2] &= 0x0f
+    codes[:, width // 2 + 1:] = 0
+    scales = torch.full((n, blocks), 127, dtype=torch.uint8, device='cuda')
+    table = rk.Mx4Table(codes, scales, width)
+    a = torch.zeros(2, width, dtype=BF16, device='cuda')
+    a[0, ::8], a[1, 256], a[1, 0] = 0.5, 2.0, 1.0
+    at = rk.mx4_quantize(a) if kind == 'mx4' else a
+    got = rk.mx4_scores(at, table, out_dtype=BF16)
+    for r, total in ((0, 16.5), (1, 3.0)):
+        want = (value * total).to(BF16)
+        assert bool((got[r, :whole].view(-1, 5) == want).all())
+        assert torch.equal(got[r, whole:], want[:n % 5])
