@@ -253,7 +253,7 @@ typedef struct alsmi_adjust {
     int64_t n_history_rows;
     const float *repetition, *frequency, *presence;
     double repetition_value, frequency_value, presence_value;
-    const float *item_bias; /* [n_items] */
+    const void *item_bias; /* [n_items] of item_bias_dtype */
     const int64_t *bias_ptr; /* [n_rows + 1] */
     const int32_t *bias_ids;
     const float *bias_values;
@@ -262,6 +262,7 @@ typedef struct alsmi_adjust {
     int64_t n_masks;
     const int32_t *mask_rows;
     int exclude;
+    int item_bias_dtype; /* ALSMI_F32, or ALSMI_F64 for fp64 scores */
 } alsmi_adjust;
 int alsmi_adjust_scores(int dtype, const alsmi_adjust *args, const void *scores, void *out,
                         void *stream);

@@ -33,7 +33,7 @@ class Adjust(ctypes.Structure):
                 ('item_bias', _vp),
                 ('bias_ptr', _vp), ('bias_ids', _vp), ('bias_values', _vp), ('n_bias', _i64),
                 ('mask', _vp), ('n_masks', _i64), ('mask_rows', _vp),
-                ('exclude', ctypes.c_int)]
+                ('exclude', ctypes.c_int), ('item_bias_dtype', ctypes.c_int)]
 
 
 def load():

@@ -378,7 +378,8 @@ class ALS(BaseEstimator):
         (src/als.py:347-364), done on the device for a batch of users.
 
         exclude_seen : leave out the items a user has a stored rating for.
-        item_bias : array [n_items] added to every user's predictions before the ranking.
+        item_bias : array [n_items] added to every user's predictions before the ranking, in the
+            precision of the scores (that of the model; float32 for catalogue='mx4').
         allowed : truth values [n_items], or [len(users), n_items]: the items on offer.
         catalogue : 'factors', or 'mx4' to score against the item factors held in 4-bit
             microscaled floating point (an eighth of the fp32 table's bytes to read; made once
@@ -395,7 +396,7 @@ class ALS(BaseEstimator):
             raise IndexError('user index out of range')
         users = np.where(users < 0, users + n, users).astype(np.int32)
         if item_bias is not None:
-            item_bias = np.ascontiguousarray(item_bias, dtype=np.float32)
+            item_bias = np.ascontiguousarray(item_bias, dtype=np.float64)
             if item_bias.shape != (m,):
                 raise ValueError('item_bias must have %d entries' % m)
         if allowed is not None:
@@ -434,7 +435,9 @@ class ALS(BaseEstimator):
         if not 1 <= k <= min(ranking.MAX_K, m):
             raise ValueError('k must be between 1 and min(%d, number of items), got %r'
                              % (ranking.MAX_K, k))
-        item_bias = up(item_bias)
+        score_dtype = torch.float32 if catalogue == 'mx4' else U.dtype
+        if item_bias is not None:
+            item_bias = up(item_bias.astype(np.float32 if score_dtype == torch.float32 else np.float64))
         ptr, ids, list_rows = (up(a) for a in seen) if seen is not None else (None, None, None)
         if catalogue == 'mx4':
             held = getattr(self, '_mx4', None)  # quantised once for these item factors
@@ -443,8 +446,7 @@ class ALS(BaseEstimator):
             table = held[1]
         n = int(d_users.numel())
         items = torch.empty((n, k), dtype=torch.int32, device=device)
-        best = torch.empty((n, k), dtype=torch.float32 if catalogue == 'mx4' else U.dtype,
-                           device=device)
+        best = torch.empty((n, k), dtype=score_dtype, device=device)
         block = max(1, _BLOCK_SCORES // m)
         mask = None
         if allowed is not None and allowed.ndim == 1:

@@ -301,7 +301,7 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
                   list r, or list history_rows[r] (int32 [n]; none where that does not exist).
     repetition, frequency, presence
                   numbers or float32 tensors [n]; repetition > 0.  Defaults 1, 0, 0.
-    item_bias     float32 [items].
+    item_bias     float32 [items]; float64 too for float64 scores.
     row_bias      (ptr int64 [n + 1], ids int32, values float32), lists as in `history`.
     mask          int32 [masks, ceil(items / 32)], see ``pack_mask``; row r has mask r (a single mask
                   serves every row), or mask mask_rows[r] (int32 [n]): a negative id is no mask, one
@@ -335,7 +335,9 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
                 raise ValueError('%s needs a history that is not excluded' % name)
             _penalty(name, value, n, args, kept)
     if item_bias is not None:
-        _vector('item_bias', item_bias, torch.float32, m)
+        if scores.dtype == torch.float64 and getattr(item_bias, 'dtype', None) == torch.float64:
+            args.item_bias_dtype = _lib.F64
+        _vector('item_bias', item_bias, torch.float64 if args.item_bias_dtype else torch.float32, m)
         kept.append(item_bias)
         args.item_bias = item_bias.data_ptr()
     if row_bias is not None:

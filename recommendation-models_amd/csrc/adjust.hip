@@ -15,6 +15,7 @@
 #include "elem.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace alsmi {
 
@@ -145,10 +146,14 @@ __global__ __launch_bounds__(ADJ_THREADS) void adjust_kernel(alsmi_adjust a, con
         }
     }
     if (a.item_bias) {
-        float b[8];
-        load8<float>(b, a.item_bias + first + at, (int)(in_tile - at));
+        auto add = [&](const auto *bias) {
+            typename std::remove_const<typename std::remove_pointer<decltype(bias)>::type>::type b[8];
+            load8(b, bias + first + at, (int)(in_tile - at));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += (W)b[i];
+            for (int i = 0; i < 8; ++i) x[i] += (W)b[i];
+        };
+        if (sizeof(T) == 8 && a.item_bias_dtype == ALSMI_F64) add(static_cast<const double *>(a.item_bias));
+        else add(static_cast<const float *>(a.item_bias));
     }
     if (has_b) {
         const unsigned hits = reinterpret_cast<const uint8_t *>(biased)[at >> 3];
@@ -201,6 +206,9 @@ extern "C" int alsmi_adjust_scores(int dtype, const alsmi_adjust *args, const vo
     ALSMI_REQUIRE(!a.bias_ptr || (a.n_bias >= 0 && a.n_bias <= INT32_MAX &&
                                   (a.n_bias == 0 || (a.bias_ids && a.bias_values))),
                   "alsmi_adjust_scores: bias lists without ids or values");
+    ALSMI_REQUIRE(!a.item_bias || a.item_bias_dtype == ALSMI_F32 ||
+                      (a.item_bias_dtype == ALSMI_F64 && dtype == ALSMI_F64),
+                  "alsmi_adjust_scores: bad item bias dtype %d", a.item_bias_dtype);
     ALSMI_REQUIRE(!a.mask || (a.mask_rows ? a.n_masks >= 0 : a.n_masks == 1 || a.n_masks >= a.n_rows),
                   "alsmi_adjust_scores: fewer masks than rows");
     hipStream_t st = static_cast<hipStream_t>(stream);

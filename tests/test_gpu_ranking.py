@@ -952,3 +952,33 @@ def test_scores_of_more_items_than_a_launch_has_room_for(kind):
         want = (value * total).to(BF16)
         assert bool((got[r, :whole].view(-1, 5) == want).all())
         assert torch.equal(got[r, whole:], want[:n % 5])
+
+
+def test_item_bias_in_the_precision_of_fp64_scores():
+    """Biases that fp32 cannot hold, added in 64 bits: sums of few binary digits, so exact."""
+    rng = np.random.default_rng(8)
+    for n, m in ((1, 1), (3, 31), (5, 2049), (7, 5000)):
+        s = rng.integers(-8, 8, (n, m)) / 8
+        bias = rng.integers(-8, 8, m) / 8 + rng.integers(-8, 8, m) * 2.0 ** -40
+        got = rk.adjust_scores(gpu(s), item_bias=gpu(bias))
+        np.testing.assert_array_equal(host(got), s + bias)
+        # an element into its memory, and in fp32 as before
+        flat = gpu(np.concatenate(([7.0], bias)))
+        np.testing.assert_array_equal(host(rk.adjust_scores(gpu(s), item_bias=flat[1:])), s + bias)
+        single = bias.astype(np.float32)
+        got = rk.adjust_scores(gpu(s), item_bias=gpu(single))
+        np.testing.assert_array_equal(host(got), s + single.astype(np.float64))
+
+
+def test_recommend_adds_a_bias_in_the_precision_of_the_model():
+    """Items of equal factors whose biases differ by 1e-12 of them."""
+    from alsmi import ALS
+    m = 300
+    als = ALS(rank=2)
+    als.user_feats, als.item_feats = np.ones((2, 3)), np.ones((2, m))
+    bias = 1.0 + 1e-12 * np.random.default_rng(0).permutation(m)
+    items, scores = als.recommend([0, 2], 20, item_bias=bias)
+    want = np.argsort(-bias)[:20]
+    assert (items == want).all() and np.abs(scores - (2 + bias[want])).max() < 1e-14
+    items, scores = als.recommend([0], 20, item_bias=bias, catalogue='mx4')
+    assert np.abs(scores - 3.0).max() < 1e-6

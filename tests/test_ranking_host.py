@@ -305,3 +305,20 @@ def test_score_rows_refuses():
         assert lib.alsmi_score_rows(*bad, None) == -1
         assert b'alsmi_score_rows' in lib.alsmi_last_error()
     assert lib.alsmi_score_rows(0, 4, 0, None, 0, None, None, 5, None, None, None) == 0
+
+
+def test_item_bias_type_follows_the_scores():
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        with pytest.raises(ValueError, match='item_bias must be'):
+            rk.adjust_scores(X.to(dtype), item_bias=torch.zeros(8, dtype=torch.float64))
+    with pytest.raises(ValueError, match='entries'):
+        rk.adjust_scores(X.double(), item_bias=torch.zeros(7, dtype=torch.float64))
+    with pytest.raises(ValueError, match='HIP device'):
+        rk.adjust_scores(X.double(), item_bias=torch.zeros(8, dtype=torch.float64))
+    lib = _lib.load()
+    p = ctypes.cast((ctypes.c_double * 64)(), ctypes.c_void_p)
+    for dtype, bias in ((_lib.F32, _lib.F64), (_lib.BF16, _lib.F64), (_lib.F64, _lib.F16), (_lib.F64, -1)):
+        a = _lib.Adjust(n_rows=2, n_items=8, ld_scores=8, ld_out=8, repetition_value=1.0, item_bias=p,
+                        item_bias_dtype=bias)
+        assert lib.alsmi_adjust_scores(dtype, ctypes.byref(a), p, p, None) == -1
+        assert b'item bias' in lib.alsmi_last_error()
