@@ -103,11 +103,19 @@ def _span(t):
 
 
 def _overlap(a, b):
-    """Whether the memory spans of two tensors meet."""
+    """Whether two tensors (vectors, or rows of unit stride) share memory."""
     if a.numel() == 0 or b.numel() == 0:
         return False
     (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
+    if a0 >= b1 or b0 >= a1:
+        return False
+    # rows the same distance apart may lie beside each other, such as column ranges of one matrix
+    apart = {t.stride(0) * t.element_size() for t in (a, b) if t.dim() == 2 and t.shape[0] > 1}
+    if len(apart) != 1:
+        return True
+    apart, off = apart.pop(), b0 - a0
+    a_row, b_row = (t.shape[-1] * t.element_size() for t in (a, b))
+    return off % apart < a_row or off % apart + b_row > apart
 
 
 def _result(name, out, shape, dtype, like, *sources):
@@ -306,7 +314,8 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
     mask          int32 [masks, ceil(items / 32)], see ``pack_mask``; row r has mask r (a single mask
                   serves every row), or mask mask_rows[r] (int32 [n]): a negative id is no mask, one
                   past the last leaves the row nothing.
-    out           a tensor like `scores`, or `scores` itself; new by default."""
+    out           a tensor like `scores`, or `scores` itself (or a view of just its elements); new
+                  by default."""
     ld = _matrix('scores', scores, _FLOATS)
     n, m = scores.shape
     args = _lib.Adjust()
@@ -364,7 +373,10 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
     elif mask_rows is not None:
         raise ValueError('mask_rows needs a mask')
     if out is not scores:
-        out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores, scores, *kept)
+        same = isinstance(out, torch.Tensor) and out.data_ptr() == scores.data_ptr() and \
+            out.shape == scores.shape and out.stride() == scores.stride()
+        out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores,
+                                   *(kept if same else [scores] + kept))
     else:
         args.ld_out = ld
         if any(_overlap(out, t) for t in kept):

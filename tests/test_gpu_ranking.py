@@ -982,3 +982,15 @@ def test_recommend_adds_a_bias_in_the_precision_of_the_model():
     assert (items == want).all() and np.abs(scores - (2 + bias[want])).max() < 1e-14
     items, scores = als.recommend([0], 20, item_bias=bias, catalogue='mx4')
     assert np.abs(scores - 3.0).max() < 1e-6
+
+
+def test_adjust_into_a_view_and_into_columns_beside():
+    s = torch.randn(5, 3000, device='cuda')
+    bias = torch.randn(3000, device='cuda')
+    want = s + bias
+    both = torch.full((5, 6000), 7.0, device='cuda')
+    both[:, :3000] = s
+    rk.adjust_scores(both[:, :3000], item_bias=bias, out=both[:, 3000:])
+    assert torch.equal(both[:, 3000:], want) and torch.equal(both[:, :3000], s)
+    rk.adjust_scores(both[:, :3000], item_bias=bias, out=both[:, :3000])
+    assert torch.equal(both[:, :3000], want)

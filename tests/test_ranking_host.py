@@ -322,3 +322,47 @@ def test_item_bias_type_follows_the_scores():
                         item_bias_dtype=bias)
         assert lib.alsmi_adjust_scores(dtype, ctypes.byref(a), p, p, None) == -1
         assert b'item bias' in lib.alsmi_last_error()
+
+
+def test_outputs_beside_and_upon_the_operands():
+    """Column ranges of one matrix share its span and no element; a view of the scores is the scores.
+    Against the sets of addresses."""
+    def cells(t):
+        rows = t if t.dim() == 2 else t[None]
+        size = t.element_size()
+        return {rows[i, j].data_ptr() + b for i in range(rows.shape[0]) for j in range(rows.shape[1])
+                for b in range(size)}
+    rng = np.random.default_rng(2)
+    base = torch.zeros(4000, dtype=torch.uint8)
+    seen = set()
+    for _ in range(3000):
+        ts = []
+        for _ in range(2):
+            dtype = [torch.float32, torch.float16, torch.uint8][rng.integers(3)]
+            flat = base.view(dtype)
+            n, m, extra = (int(rng.integers(1, 6)) for _ in range(3))
+            ld = int(rng.choice([16, 20, m + extra])) // (4 if rng.random() < 0.3 else 1)
+            ld = max(ld, m)
+            at = int(rng.integers(0, 40))
+            ts.append(flat[at:at + n * ld].view(n, ld)[:, :m] if rng.random() < 0.8
+                      else flat[at:at + m])
+        meet = bool(cells(ts[0]) & cells(ts[1]))
+        apart = {t.stride(0) * t.element_size() for t in ts if t.dim() == 2 and t.shape[0] > 1}
+        assert rk._overlap(*ts) or not meet
+        if len(apart) == 1:  # exact; strides that differ may be refused where they only interleave
+            assert rk._overlap(*ts) == meet
+            seen.add(meet)
+    assert seen == {True, False}
+    both = torch.zeros(3, 32)
+    for scores, out in ((both[:, :16], both[:, 16:]), (both[:, 16:], both[:, :16]), (both, both[:]),
+                        (both[:, 4:9], both.view(3, 32)[:, 4:9]), (both[:1, :8], both[:1, 8:16])):
+        with pytest.raises(ValueError, match='HIP device'):
+            rk.adjust_scores(scores, out=out)
+    for scores, out in ((both[:, :16], both[:, 15:31]), (both[:, :16], both[:, 1:17]),
+                        (both[:2], both[1:])):
+        with pytest.raises(ValueError, match='overlap'):
+            rk.adjust_scores(scores, out=out)
+    with pytest.raises(ValueError, match='overlap'):
+        rk.adjust_scores(both, item_bias=both[0], out=both[:])
+    with pytest.raises(ValueError, match='one of'):
+        rk.adjust_scores(both, out=both.view(torch.int32))
