@@ -354,6 +354,13 @@ def topk_items(rank, users, row_table, col_table, k, max_workspace_bytes=1 << 30
     return items, scores
 
 
+def _share_memory(a, b):
+    """Whether two contiguous tensors share memory."""
+    size = lambda t: t.numel() * t.element_size()
+    return a.data_ptr() < b.data_ptr() + size(b) and b.data_ptr() < a.data_ptr() + size(a) and \
+        a.numel() > 0 and b.numel() > 0
+
+
 def score_items(rank, users, row_table, col_table, out=None):
     """The dense score block [n, n_items] of `users` (int32 device tensor) that ``topk_items``
     ranks: <row_table[users[p]], col_table[i]>, for callers that change the scores before they
@@ -369,6 +376,8 @@ def score_items(rank, users, row_table, col_table, out=None):
             out.device != device or not out.is_contiguous():
         raise ValueError('out must be contiguous [%d x %d] %s on the device of the tables'
                          % (n_sel, n_items, row_table.dtype))
+    elif any(_share_memory(out, t) for t in (users, row_table, col_table)):
+        raise ValueError('out must not overlap the operands')
     ws = torch.empty(4, dtype=torch.int32, device=device)
     here = device.index == torch.cuda.current_device()  # (changing the device costs microseconds)
     with contextlib.nullcontext() if here else torch.cuda.device(device):

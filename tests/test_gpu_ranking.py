@@ -994,3 +994,17 @@ def test_adjust_into_a_view_and_into_columns_beside():
     assert torch.equal(both[:, 3000:], want) and torch.equal(both[:, :3000], s)
     rk.adjust_scores(both[:, :3000], item_bias=bias, out=both[:, :3000])
     assert torch.equal(both[:, :3000], want)
+
+
+def test_score_items_over_its_operands_is_refused():
+    from alsmi import device as dev
+    U, V = torch.ones(6, 16, device='cuda'), torch.ones(8, 16, device='cuda')
+    users = torch.zeros(3, dtype=torch.int32, device='cuda')
+    flat = torch.zeros(64, device='cuda')
+    for args in ((users, U, V, U.view(-1)[72:].view(3, 8)), (users, U, V, V.view(-1)[:24].view(3, 8)),
+                 (flat[20:23].view(torch.int32), U, V, flat[:24].view(3, 8))):
+        with pytest.raises(ValueError, match='overlap'):
+            dev.score_items(3, *args[:3], out=args[3])
+    out = flat[24:48].view(3, 8)
+    assert dev.score_items(3, flat[20:23].view(torch.int32), U, V, out=out) is out
+    assert bool((out == 16).all()) and bool((flat[:24] == 0).all()) and bool((flat[48:] == 0).all())
