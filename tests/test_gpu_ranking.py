@@ -1008,3 +1008,107 @@ def test_score_items_over_its_operands_is_refused():
     out = flat[24:48].view(3, 8)
     assert dev.score_items(3, flat[20:23].view(torch.int32), U, V, out=out) is out
     assert bool((out == 16).all()) and bool((flat[:24] == 0).all()) and bool((flat[48:] == 0).all())
+
+
+# ------------------------------------------------------------ sums that are exact, so bit for bit
+FORMS = [  # rows, items, width: one for each form of the product, in the order of their rules
+    (1, 100, 20), (40, 100, 20), (1, 100, 60), (40, 70, 60), (3, 100, 128), (70, 130, 100),
+    (5, 300, 250), (70, 300, 250), (2, 300, 1000), (3, 100000, 300), (20, 500, 640), (40, 90000, 300),
+    (100, 16400, 300), (130, 16400, 300), (300, 9001, 544), (1020, 16300, 700), (64, 33000, 1030),
+    (129, 8300, 2080)]
+
+
+def exact_table(g, n, width, codes):
+    """Rows of random codes out of `codes` and scales of 1, 2 and 4, codes of 0 behind the width."""
+    blocks = (width + 31) // 32
+    pick = torch.tensor(codes, dtype=torch.uint8, device='cuda')
+    nibble = pick[torch.randint(0, len(codes), (n, 32 * blocks), generator=g, device='cuda')]
+    nibble[:, width:] = 0
+    scales = torch.randint(127, 130, (n, blocks), generator=g, device='cuda', dtype=torch.uint8)
+    return rk.Mx4Table((nibble[:, 0::2] | nibble[:, 1::2] << 4).contiguous(), scales, width)
+
+
+def table_values(table, dtype=F64):
+    """What codes and scales stand for, by the table of sixteen values."""
+    lut = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, 0, -.5, -1, -1.5, -2, -3, -4, -6], dtype=dtype,
+                       device='cuda')
+    both = torch.stack((table.codes & 15, table.codes >> 4), dim=-1).flatten(1)[:, :table.width]
+    unit = torch.exp2(table.scales.to(dtype) - 127).repeat_interleave(32, dim=1)[:, :table.width]
+    return lut[both.to(torch.int32)] * unit
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('m,n,width', FORMS + [(700, 2800, 65536)])
+def test_every_part_of_an_activation_counts(m, n, width, kind):
+    """One activation a row that is not zero, with as many significant bits as its type has (the last of
+    them set), and table elements that are powers of two: a score is one product and exact, so the
+    last bit of the last bf16 part has to be there.  The rows' elements lie all over the width."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(m + 3 * n + width)
+    table = exact_table(g, n, width, [1, 2, 4, 6, 9, 10, 12, 14])
+    dtype, bits = {'f32': (F32, 24), 'bf16': (BF16, 8), 'f16': (F16, 11)}[kind]
+    rows = torch.arange(m, device='cuda')
+    ends = torch.tensor([0, width - 1, width // 2], device='cuda')
+    for turn in range(2 if m * width > 1 << 22 else 8):  # few rows meet few places of the width
+        at = torch.randint(0, width, (m,), generator=g, device='cuda')
+        at[:min(m, 3)] = ends.roll(turn)[:min(m, 3)]
+        value = torch.randint(2 ** (bits - 2), 2 ** (bits - 1), (m,), generator=g, device='cuda') * 2 + 1
+        value = value * (1 - 2 * torch.randint(0, 2, (m,), generator=g, device='cuda'))
+        value = value.to(F64) * 2.0 ** -(bits // 2)
+        a = torch.zeros(m, width, dtype=dtype, device='cuda')
+        a[rows, at] = value.to(dtype)
+        byte = table.codes[:, at // 2]
+        nibble = torch.where(at % 2 == 1, byte >> 4, byte & 15).to(torch.int32)
+        power = torch.exp2(torch.tensor([0., -1, 0, 0, 1, 0, 2, 0], device='cuda')[nibble & 7].to(F64) +
+                           table.scales[:, at // 32].to(F64) - 127)
+        want = (power * (1.0 - 2.0 * (nibble >> 3).to(F64))).t() * value[:, None]
+        assert torch.equal(rk.mx4_scores(a, table, out_dtype=F32).to(F64), want)
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16', 'f16', 'mx4'])
+@pytest.mark.parametrize('m,n,width', FORMS + [(700, 2800, 65536), (1100, 2800, 65536), (130, 65536, 300),
+                                               (2048, 2049, 1024), (512, 5000, 4096), (300, 8200, 992)])
+def test_every_element_of_a_row_counts(m, n, width, kind):
+    """Small whole activations (at most 3, or codes of at most 2) against any codes (at most 24): a sum is a
+    whole number of halves, at most 65536 * 72 * 2 of them, or of quarters, at most 65536 * 48 * 4.  Both
+    are below 2^24, so fp32 sums in any order are exact and a left out element shows."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(m + n + 5 * width)
+    table = exact_table(g, n, width, list(range(16)))
+    if kind == 'mx4':
+        a = exact_table(g, m, width, [0, 1, 2, 4, 9, 10, 12])
+        a.scales.fill_(127)
+        values = table_values(a)
+    else:
+        a = torch.randint(-3, 4, (m, width), generator=g, device='cuda')
+        values = a.to(F64)
+        a = a.to({'f32': F32, 'bf16': BF16, 'f16': F16}[kind])
+    got = rk.mx4_scores(a, table, out_dtype=F32)
+    for lo in range(0, n, 20000):  # (fp64 products in parts: tables of 90000 items are 200 MB)
+        part = rk.Mx4Table(table.codes[lo:lo + 20000], table.scales[lo:lo + 20000], width)
+        assert torch.equal(got[:, lo:lo + 20000].to(F64), values @ table_values(part).t())
+
+
+@pytest.mark.parametrize('dtype', [F32, F64, F16, BF16])
+@pytest.mark.parametrize('n,m,k', [(1, 1000000, 1024), (3, 400000, 1000), (1, 10000000, 1024), (7, 300000, 513)])
+def test_topk_through_a_middle_level(n, m, k, dtype):
+    """More kept keys than one workgroup takes, so that a level in between reads keys and writes keys, into the
+    second half of the workspace; the workspace is not left."""
+    g = torch.Generator(device='cuda')
+    g.manual_seed(m + k)
+    s = torch.randn(n, m, generator=g, device='cuda', dtype=F64).to(dtype) + 0.0
+    few = torch.randint(-2, 3, (n, m), generator=g, device='cuda').to(dtype)
+    hardly = torch.full((n, m), -INF, dtype=dtype, device='cuda')
+    hardly[:, m // 3::m // 700] = s[:, m // 3::m // 700]
+    up = torch.sort(s, dim=1).values.contiguous()
+    code = rk._CODES[dtype]
+    size = rk._lib.load().alsmi_topk_rows_workspace_bytes(code, n, m, k)
+    for rows in (s, few, hardly, up, up.flip(1).contiguous()):
+        want, order = torch.sort(rows, dim=1, descending=True, stable=True)
+        items, best = rk.topk_rows(rows, k)
+        assert torch.equal(best, want[:, :k]) and torch.equal(items, order[:, :k].to(torch.int32))
+        ws = torch.full((size + 4096,), 77, dtype=torch.uint8, device='cuda')
+        items.zero_()
+        rk._call(rows.device, 'alsmi_topk_rows', code, n, m, rows.data_ptr(), m, k, items.data_ptr(),
+                 best.data_ptr(), ws.data_ptr())
+        assert torch.equal(items, order[:, :k].to(torch.int32)) and bool((ws[size:] == 77).all())
