@@ -208,8 +208,9 @@ int alsmi_score_items(int dtype, int rank, int64_t n_sel, const int32_t *users,
  * zeros); the code nearest to |x| / 2^(b-127), ties to the even code, above 6 as 6.  A block with an
  * infinity or a NaN gets byte 255 and codes 0.  1 <= width <= 2^20, codes aligned to 4 bytes.
  * alsmi_mx4_dequantize: out row i = row rows[i] of the table (row i where rows is NULL); byte 255
- * reads as NaN, and so does a row id outside 0 .. n_rows-1.  Exact in fp32, fp64 and bf16; fp16
- * rounds and overflows to infinity. */
+ * reads as NaN, and so does a row id outside 0 .. n_rows-1.  Exact in fp64; in fp32 and bf16 up to byte
+ * 252 (4 x 2^126 of byte 253, which only fp64 elements are quantised to, is past their range and
+ * becomes an infinity); fp16 rounds and overflows to infinity. */
 int alsmi_mx4_quantize(int dtype, int64_t n_rows, int64_t width, const void *x, int64_t ld_x,
                        uint8_t *codes, uint8_t *scales, void *stream);
 int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t n_rows,
@@ -218,8 +219,10 @@ int alsmi_mx4_dequantize(int dtype, int64_t n_sel, const int32_t *rows, int64_t 
 
 /* out[i, j] = sum_k a[i, k] table[j, k] for i < n_sel, j < n_items; out [n_sel x n_items] of
  * out_dtype (ALSMI_F32, F16 or BF16).  `a` has n_rows rows of `width` elements of dtype ALSMI_F32,
- * F16 or BF16 (every product exact, fp32 sums), or with ALSMI_MX4 is a table's codes and a_scales
- * its scales (a_scales is ignored otherwise).  rows as in alsmi_mx4_dequantize: a row of NaN where
+ * F16 or BF16, or with ALSMI_MX4 is a table's codes and a_scales its scales (a_scales is ignored
+ * otherwise).  Products are exact and sums fp32.  Two ranges are left out of that: bits below 2^-133 of
+ * an ALSMI_F32 activation (which those of 2^-110 and more do not have) are cut off, and beside float
+ * activations a table element past bf16's range (from byte 253 on, as above) counts as an infinity.  rows as in alsmi_mx4_dequantize: a row of NaN where
  * there is no such row.  workspace: alsmi_mx4_scores_workspace_bytes() bytes, aligned to 16 (large
  * products of float activations split them there first, 256 MiB at a time or 128 rows); may be
  * NULL where that is 0; what is enough for some rows, items and width is for fewer. */

@@ -195,7 +195,8 @@ def mx4_quantize(x):
 
 def mx4_dequantize(table, dtype=torch.float32, rows=None, out=None):
     """The values `table` stands for, [n, width] of `dtype`; with `rows` (int32) those rows in
-    that order, NaN for a row the table does not have."""
+    that order, NaN for a row the table does not have.  Exact but for float16, and for elements of
+    2^128 or more, which are infinities in float32 and bfloat16."""
     if not isinstance(table, Mx4Table):
         raise ValueError('table must be an Mx4Table')
     if dtype not in _CODES:
@@ -215,8 +216,10 @@ def mx4_scores(a, table, rows=None, out_dtype=None, out=None):
     """``a @ table.T``, [m, n] with n = len(table): the scores of the rows of `a` against every row
     of `table`.
 
-    `a` is a float32, float16 or bfloat16 tensor [m, width] (every product exact, float32 sums)
-    or another ``Mx4Table`` of the same width.  With `rows` (int32) the rows of `a` with those
+    `a` is a float32, float16 or bfloat16 tensor [m, width] or another ``Mx4Table`` of the same
+    width.  Products are exact and sums float32, except that of a float32 activation bits below
+    2^-133 are cut off and that beside float activations a table element of 2^128 or more (scale
+    bytes 253 and 254, from float64 rows) counts as an infinity.  With `rows` (int32) the rows of `a` with those
     ids, NaN for one it does not have.  The result has `out_dtype` (float32, float16 or
     bfloat16), by default that of `a`, float32 for a table."""
     if not isinstance(table, Mx4Table):

@@ -231,9 +231,11 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(int64_t n_sel,
 
 // ---- scores: out[i, j] = sum_k a[i, k] table[j, k] -----------------------------------------------
 // The table's elements have three significant bits and are exact in bf16 once scaled, so the
-// product runs on the bf16 matrix cores with fp32 sums.  The activations are split exactly into bf16
-// parts: fp32 = 3 parts of 8 significant bits each (cut, not rounded), fp16 = 2, bf16 = 1; every
-// product is then exact and the result has the accuracy of fp32 sums of the fp32 products.  (A
+// product runs on the bf16 matrix cores with fp32 sums (elements of 2^128 and more, scale bytes 253 and
+// 254, become infinities there).  The activations are split into bf16 parts: fp32 = 3 parts of 8
+// significant bits each (cut, not rounded), fp16 = 2, bf16 = 1.  Bits below bf16's smallest number,
+// 2^-133, are cut off; above it the split and every product are exact, and the result has the
+// accuracy of fp32 sums of the fp32 products.  (A
 // two-way fp16 split as in the half-sweep would take 2 parts for fp32, but needs the table's
 // scales applied after each block of 32 and the largest |a| beforehand.)
 // Matrix operands: the items are the rows of the result tile, the activations its columns, so a lane
@@ -1067,7 +1069,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx4_scores_tiled_kernel(
         load_step(0, sc0);
         for (int turn = 0; turn < turns; ++turn) {
             __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(1): this wave's codes of this step are in LDS
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's codes of this step are in LDS
             // 16 scales, eight of either step -> word g: blocks 2g, 2g + 1 of the first, then the second
             u32x4 word;
             word[0] = __builtin_amdgcn_perm(sr[2], sr[0], 0x05040100u);

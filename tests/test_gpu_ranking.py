@@ -1112,3 +1112,29 @@ def test_topk_through_a_middle_level(n, m, k, dtype):
         rk._call(rows.device, 'alsmi_topk_rows', code, n, m, rows.data_ptr(), m, k, items.data_ptr(),
                  best.data_ptr(), ws.data_ptr())
         assert torch.equal(items, order[:, :k].to(torch.int32)) and bool((ws[size:] == 77).all())
+
+
+def test_the_ends_of_the_exact_range():
+    """Elements of the two largest scales (exact in fp64, infinities from 2^128 on in fp32, bf16 and beside
+    float activations) and the smallest activations whose last bit is not cut off."""
+    codes = torch.tensor([[2, 3, 4, 5, 6, 7, 1, 0]], dtype=torch.uint8, device='cuda').repeat(3, 4)
+    codes = (codes[:, 0::2] | codes[:, 1::2] << 4).contiguous()
+    table = rk.Mx4Table(codes, gpu(np.array([[252], [253], [254]], dtype=np.uint8)), 32)
+    grid = np.tile([1, 1.5, 2, 3, 4, 6, 0.5, 0], 4)
+    value = grid * 2.0 ** np.array([[125.0], [126], [127]])
+    np.testing.assert_array_equal(host(rk.mx4_dequantize(table, F64)), value)
+    capped = np.where(value >= 2.0 ** 128, INF, value)
+    for dtype in (F32, BF16):
+        np.testing.assert_array_equal(host(rk.mx4_dequantize(table, dtype)), capped)
+    one = torch.eye(32, device='cuda')[:7] * 0.25  # each element of an item by itself
+    got = host(rk.mx4_scores(one, table))
+    np.testing.assert_array_equal(got[:, 0], 0.25 * value[0, :7])
+    assert np.isnan(got[:, 1:]).all()  # (a zero beside an infinity)
+    both = host(rk.mx4_scores(rk.mx4_quantize(one), table))  # both in 4 bits: nothing is widened
+    np.testing.assert_array_equal(both, 0.25 * value[:, :7].T)
+    small = rk.Mx4Table(codes[:1].contiguous(), gpu(np.array([[130]], dtype=np.uint8)), 32)
+    a = torch.zeros(2, 32, device='cuda')
+    a[0, 0], a[1, 0] = (2.0 ** 24 - 1) * 2.0 ** -133, (2.0 ** 24 - 1) * 2.0 ** -134
+    got = host(rk.mx4_scores(a, small))
+    assert got[0, 0] == 8 * (2.0 ** 24 - 1) * 2.0 ** -133
+    assert got[1, 0] == 8 * (2.0 ** 24 - 2) * 2.0 ** -134
