@@ -122,7 +122,7 @@ def collect(spec):
             'instruction issue / cache gather (the gathered table is cache resident)'
     roof['traffic'] = (entry['user_side']['hbm_bytes'] + entry['item_side']['hbm_bytes']) / 2
     roof['counters'] = {'kernels': kern, 'file': 'profiles/%s_summary.json' % tag,
-                        'measured': 'same gpurun call as this line (tools/profile_round.sh)'}
+                        'measured': 'same run as this line (tools/profile_round.sh)'}
     with open(os.path.join(dst, stem + '.json'), 'w') as f:
         f.write(json.dumps(line) + '\n')
     return '%s/%s' % (config, dtype), entry
