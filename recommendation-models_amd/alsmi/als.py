@@ -330,7 +330,8 @@ class ALS(BaseEstimator):
     def _remember_tables(self, U, V):
         """Keep the device copies of the factor tables together with the host arrays they
         were made from (strong references: a later array cannot reuse their identity) and a
-        signature of their contents."""
+        signature of their contents.  What was made from earlier tables goes."""
+        self._mx4 = None
         self._tables = (U, V, self.user_feats, self.item_feats,
                         self._fingerprint(self.user_feats), self._fingerprint(self.item_feats))
         return self._tables

@@ -1138,3 +1138,20 @@ def test_the_ends_of_the_exact_range():
     got = host(rk.mx4_scores(a, small))
     assert got[0, 0] == 8 * (2.0 ** 24 - 1) * 2.0 ** -133
     assert got[1, 0] == 8 * (2.0 ** 24 - 2) * 2.0 ** -134
+
+
+def test_refit_releases_the_quantised_items():
+    """The table in 4 bits, and the factor table that it was made from, go with the factors they belong to."""
+    import weakref
+    from alsmi import ALS
+    rng = np.random.default_rng(1)
+    pairs = rng.integers(0, 30, 200), rng.integers(0, 40, 200)
+    als = ALS(4, random_state=0, max_iter=1).fit(pairs, rng.random(200) + 1, shape=(30, 40))
+    als.recommend([0], 3, catalogue='mx4')
+    old = weakref.ref(als._mx4[0])
+    als.fit(pairs, rng.random(200) + 1, shape=(30, 40))
+    assert als._mx4 is None and old() is None
+    items, scores = als.recommend([0], 40, catalogue='mx4')
+    codes, scales = ro.mx4_quantize(als.item_feats.T)
+    want = (als.user_feats.T @ ro.mx4_values(codes, scales, 4).T)[0]
+    assert np.abs(scores[0] - want[items[0]]).max() < 1e-5
