@@ -9,8 +9,11 @@
 // One pass over the scores.  The sparse lists of a row are turned into bits and counters in LDS for the
 // tile of items a workgroup owns: a scan of the list, integer atomics (their order cannot change
 // the result), no sorting and no second launch.  Bound by the read and the write of the scores
-// (1024 x 26744 fp32 with exclusion, bias and masks: 35 us, 6.2 TB/s), for long lists over many
-// tiles by their scan (64 x 131072 bf16, lists of 900 on average: 13.6 us).
+// (1024 x 26744 fp32 with exclusion, bias and masks: 47 us, 4.7 TB/s, or 35 us for scores that the
+// call before left in the last-level cache), for long lists over many tiles by latencies: first
+// the lists, behind the barrier mask, penalties and biases (64 x 131072 bf16, lists of 900 on
+// average: 13.6 us; 61 % of the waves' cycles are waits, the vector instructions fill a third of
+// the time).
 #include "alsmi_common.h"
 #include "elem.h"
 

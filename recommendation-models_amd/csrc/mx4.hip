@@ -528,8 +528,9 @@ __device__ __forceinline__ bool join_waves(f32x4 (&acc)[MT][NT], int wave, int l
 // Rows of any width: a wave forms MT x NT tiles (16 activation rows x 16 items each) in steps of
 // four blocks.  KW = 1: the four waves of a workgroup take neighbouring items; KW = 4: they share
 // one tile group and take a quarter of the steps each, joined in wave order through LDS, where
-// there are too few tiles to fill the chip.  Bound by the table's bytes for a few rows (1 x 1000000 x
-// 512 bf16: 90 us, 3 TB/s), by the loads and splits of the activations else.
+// there are too few tiles to fill the chip.  Bound by the loads of each step for a few rows (none is in
+// flight across steps; 1 x 1000000 x 512 bf16: 90 us, 3 TB/s of table), by the loads and splits of
+// the activations else.
 template <typename T, typename TO, int MT, int NT, int KW>
 __global__ __launch_bounds__(256) void mx4_scores_wide_kernel(Rows rows, const T *__restrict__ a,
                                                               int width,
@@ -1217,9 +1218,9 @@ static int run_both(const Rows &rows, const void *a, const uint8_t *a_scales, co
     // (each wave on its own instead of four per row: 1 x 1000000 x 512 72 us instead of 49)
     if (one) return launch_both<TO, 1, 2, 4>(rows, a, a_scales, codes, scales, nb, o, st);
     // the tiled forms keep the loads of a long row in flight, which a few tiles cannot fill the
-    // chip with (17 x 4000 x 1024 5.6 us against 4.4, 40 x 16384 x 4096 15 against 32) and rows of
+    // chip with (17 x 4000 x 1024 5.6 us against 4.4, but 40 x 16384 x 4096 15 against 32) and rows of
     // less than a turn have no use for (256 x 4000 x 384 7.3 against 4.6, 128 x 20000 x 300 8.4
-    // against 7.2, 1024 x 26744 x 384 33 against 41)
+    // against 7.2, 1024 x 26744 x 384 in tiles of 128 x 128 33.6 against 32.2)
     const int64_t tiles = (rows.n_sel + 15) / 16 * ((o.n_items + 15) / 16);
     if (tiles < (nb >= 16 ? 2048 : 32768))
         return launch_both<TO, 2, 2, 4>(rows, a, a_scales, codes, scales, nb, o, st);
@@ -1227,10 +1228,13 @@ static int run_both(const Rows &rows, const void *a, const uint8_t *a_scales, co
     const bool aligned = (uintptr_t)a % 16 == 0 && (uintptr_t)codes % 16 == 0 &&
                          (!rows.ids || rows.n_rows * nb < (int64_t)1 << 28);
     if (!aligned || nb < 16) return launch_both<TO, 4, 4, 1>(rows, a, a_scales, codes, scales, nb, o, st);
-    // A tile of 256 x 256 fills a CU and takes 1.15 times less per score than four of 128 x 128, two
-    // of which run on a CU at a time; it loses where its last round is not full: 2048 x 16384 x
-    // 4096 86 us against 100, 512 x 32768 x 1024 21.5 against 26, but 512 x 26744 x 1024 26.3
-    // against 23.1, 300 x 65536 x 2048 53 against 45, 1000 x 8192 x 4096 38 against 28.
+    // A tile of 256 x 256 fills a CU and takes at least 1.1 times less per score than four of 128 x 128,
+    // two of which run on a CU at a time; it loses where its last round is not full: 2048 x 16384 x
+    // 4096 73 us against 95, 512 x 32768 x 1024 16.8 against 18.4, but 512 x 26744 x 1024 23.5
+    // against 19.0, 300 x 65536 x 2048 45 against 41, 1000 x 8192 x 4096 33 against 26.  The blocks
+    // behind the last whole turn do not change that (2048 x 16384 x 4000 91 against 131, x 992 44
+    // against 52 and 68 from memory), though read from memory they take their time: x 4096 takes
+    // 73 us, x 2000 59 (x 2048 44), x 1024 31.
     const int64_t t256 = (rows.n_sel + 255) / 256 * ((o.n_items + 255) / 256);
     const int64_t t128 = (rows.n_sel + 127) / 128 * ((o.n_items + 127) / 128);
     if ((t256 + 255) / 256 * 102400 <= t128 * 115)

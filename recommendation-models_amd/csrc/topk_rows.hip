@@ -9,8 +9,9 @@
 // Small k: a wave keeps its k best, sorted, one per lane, and streams over its part of the row: a key at
 //   or below the k-th best is dropped by one comparison, the few others wait in LDS until 64 of them
 //   are sorted and merged into the list at once.  Four waves per workgroup, as many workgroups per row
-//   as fill the chip; a second launch merges their lists.  Bound by the reads for many rows (1024 x
-//   26744 fp32, k = 10: 23.4 us, 4.7 TB/s), by two launches' latencies for one (1 x 1000000: 14 us).
+//   as fill the chip; a second launch merges their lists.  Many rows take the time of their reads and
+//   some more for sorting and merging hits (1024 x 26744 fp32, k = 10: 23.4 us, 4.7 TB/s; 18.8
+//   without hits, 14.7 for the reads alone), one row that of two launches (1 x 1000000: 14 us).
 // Larger k: a workgroup of 512 threads keeps the k best of its part of the row: of the first 8192 keys,
 //   held in registers, it finds the k-th largest by a radix descent over LDS histograms (2048 bins
 //   a digit), from then on only keys above it are looked at again.  Parts as many as run at once;
