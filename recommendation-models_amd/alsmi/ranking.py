@@ -347,9 +347,10 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
                 raise ValueError('%s needs a history that is not excluded' % name)
             _penalty(name, value, n, args, kept)
     if item_bias is not None:
-        if scores.dtype == torch.float64 and getattr(item_bias, 'dtype', None) == torch.float64:
-            args.item_bias_dtype = _lib.F64
-        _vector('item_bias', item_bias, torch.float64 if args.item_bias_dtype else torch.float32, m)
+        wide = torch.float32
+        if scores.dtype is torch.float64 and getattr(item_bias, 'dtype', None) is torch.float64:
+            wide, args.item_bias_dtype = torch.float64, _lib.F64
+        _vector('item_bias', item_bias, wide, m)
         kept.append(item_bias)
         args.item_bias = item_bias.data_ptr()
     if row_bias is not None:
@@ -375,7 +376,9 @@ def adjust_scores(scores, history=None, history_rows=None, repetition=None, freq
             raise ValueError('mask must have one row or one for each of the %d rows' % n)
     elif mask_rows is not None:
         raise ValueError('mask_rows needs a mask')
-    if out is not scores:
+    if out is None:
+        out, args.ld_out = scores.new_empty((n, m)), m
+    elif out is not scores:
         same = isinstance(out, torch.Tensor) and out.data_ptr() == scores.data_ptr() and \
             out.shape == scores.shape and out.stride() == scores.stride()
         out, args.ld_out = _result('out', out, (n, m), scores.dtype, scores,
