@@ -1155,3 +1155,34 @@ def test_refit_releases_the_quantised_items():
     codes, scales = ro.mx4_quantize(als.item_feats.T)
     want = (als.user_feats.T @ ro.mx4_values(codes, scales, 4).T)[0]
     assert np.abs(scores[0] - want[items[0]]).max() < 1e-5
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'float64'])
+def test_score_items_captured_and_replayed(dtype):
+    """In a graph with the steps behind it, replayed on other factors and users, with eager calls of other
+    users between the replays (each call clears and fills a scale of its own)."""
+    from alsmi import device as dev
+    rng = np.random.default_rng(3)
+    rank, n, m = 20, 400, 3000
+    draw = lambda k, size: gpu(rng.standard_normal((k, 32)) * (np.arange(32) < rank) * size).to(
+        F32 if dtype == 'float32' else F64)
+    U, V = draw(n, 1.0), draw(m, 1.0)
+    users = gpu(rng.integers(0, n, 90).astype(np.int32))
+
+    def call():
+        s = dev.score_items(rank, users, U, V)
+        return (s,) + rk.topk_rows(s, 12)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for size in (1e-3, 1e5, 1.0):
+        U.copy_(draw(n, size))
+        V.copy_(draw(m, size * 10))
+        users.copy_(gpu(rng.integers(-1, n + 1, 90).astype(np.int32)))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, call()):
+            assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) if a.is_floating_point() else \
+                torch.equal(a, b)
+        dev.score_items(rank, users[:5].clone(), U * 100, V)
