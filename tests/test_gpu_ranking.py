@@ -925,6 +925,8 @@ def test_tables_of_more_rows_than_a_launch_has_room_for():
     x.fill_(NAN)
     rk.mx4_dequantize(few, rows=ids, out=x)
     check(x, n % period)
+    del x, ids
+    torch.cuda.empty_cache()  # (54 GB at most)
 
 
 @pytest.mark.parametrize('kind', ['bf16', 'mx4'])
@@ -952,6 +954,8 @@ def test_scores_of_more_items_than_a_launch_has_room_for(kind):
         want = (value * total).to(BF16)
         assert bool((got[r, :whole].view(-1, 5) == want).all())
         assert torch.equal(got[r, whole:], want[:n % 5])
+    del table, codes, scales, got
+    torch.cuda.empty_cache()  # (85 GB)
 
 
 def test_item_bias_in_the_precision_of_fp64_scores():
